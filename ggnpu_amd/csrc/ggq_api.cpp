@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -23,6 +24,7 @@
 #include <vector>
 
 #include "../../include/ggq.h"
+#include "ggq_attn.h"
 #include "ggq_formats.h"
 #include "ggq_launch.h"
 
@@ -33,6 +35,12 @@ struct ggq_weight {
     uint32_t type = 0;
     int64_t N = 0, K = 0;
     size_t bytes = 0;
+};
+
+struct ggq_rope {
+    double* turns = nullptr;  // device, turns of each pair per position
+    int head_dim = 0, rot_dim = 0, layout = 0;
+    float mag = 1.0f;
 };
 
 namespace {
@@ -90,6 +98,7 @@ struct ggq_ctx {
     std::string msg;
     std::map<std::tuple<const void*, uint32_t, int64_t, int64_t>, ggq_weight*> cache;
     std::set<ggq_weight*> weights;
+    std::set<ggq_rope*> ropes;
     Work dev;   // workspace of the *_dev entry points
     Work host;  // workspace of the synchronous host-pointer entry points (never
                 // shared with device calls that may still run on other streams)
@@ -901,6 +910,10 @@ void ggq_destroy(ggq_ctx* c) {
         hipFree(w->dev);
         delete w;
     }
+    for (ggq_rope* r : c->ropes) {
+        hipFree(r->turns);
+        delete r;
+    }
     for (void* p : c->owned) hipFree(p);
     for (SharedLane& l : c->shared)
         if (l.ev) hipEventDestroy(l.ev);
@@ -1094,6 +1107,225 @@ int ggq_attention_decode_dev(ggq_ctx* c, const float* Q, const float* K, const f
     return hip_status(c, ggq::launch_attn_decode(Q, K, V, n_tok, n_head, n_kv_head, head_dim, ctx_len, pos0, out,
                                                  (float*)c->attn.ptr, s),
                       "attention");
+    GGQ_END(c)
+}
+
+int ggq_rope_create(ggq_ctx* c, const ggq_rope_params* p, ggq_rope** out) {
+    GGQ_GUARD(c)
+    if (!p || !out) return set_status(c, GGQ_INVALID_PARAM, "null pointer");
+    *out = nullptr;
+    const int hd = p->head_dim, rot = p->rot_dim ? p->rot_dim : hd;
+    if (hd < 8 || hd > 512 || hd % 8) return set_status(c, GGQ_INVALID_PARAM, "head_dim must be a multiple of 8 up to 512 (got %d)", hd);
+    if (rot < 8 || rot > hd || rot % 8)
+        return set_status(c, GGQ_INVALID_PARAM, "rot_dim must be a multiple of 8 up to head_dim (got %d)", rot);
+    if (p->layout != GGQ_ROPE_HALF && p->layout != GGQ_ROPE_INTERLEAVED)
+        return set_status(c, GGQ_INVALID_PARAM, "unknown layout %d", p->layout);
+    const double base = p->base == 0.0 ? 10000.0 : p->base, scale = p->position_scale == 0.0 ? 1.0 : p->position_scale;
+    const double mag = p->magnitude == 0.0 ? 1.0 : p->magnitude;
+    const bool yarn = p->yarn_factor != 0.0 && p->yarn_factor != 1.0;
+    const double fast = p->yarn_beta_fast == 0.0 ? 32.0 : p->yarn_beta_fast;
+    const double slow = p->yarn_beta_slow == 0.0 ? 1.0 : p->yarn_beta_slow;
+    if (!(base > 0.0) || !std::isfinite(base) || !std::isfinite(scale) || !std::isfinite(mag))
+        return set_status(c, GGQ_INVALID_PARAM, "base must be above 0, position_scale and magnitude finite");
+    if (yarn && !(p->yarn_factor > 1.0 && p->yarn_ctx >= 1.0 && fast > 0.0 && slow > 0.0 && base > 1.0 &&
+                  std::isfinite(p->yarn_factor) && std::isfinite(p->yarn_ctx) && std::isfinite(fast) && std::isfinite(slow)))
+        return set_status(c, GGQ_INVALID_PARAM, "yarn_factor needs to be 1 or more, with yarn_ctx, betas above 0 and base above 1");
+    const double pi = 3.14159265358979323846;
+    // the pair that turns `t` times over yarn_ctx positions: base^(2 i / rot) = yarn_ctx / (2 pi t)
+    auto pair_of = [&](double t) { return rot * std::log(p->yarn_ctx / (2.0 * pi * t)) / (2.0 * std::log(base)); };
+    double low = 0.0, high = 0.0;
+    if (yarn) {
+        low = std::max(std::floor(pair_of(fast)), 0.0);
+        high = std::min(std::ceil(pair_of(slow)), (double)(rot - 1));
+    }
+    std::vector<double> turns(rot / 2);
+    for (int i = 0; i < rot / 2; i++) {
+        double f = scale * std::pow(base, -2.0 * i / rot);
+        if (p->freq_factors) {
+            const double d = p->freq_factors[i];
+            if (!(d > 0.0) || !std::isfinite(d)) return set_status(c, GGQ_INVALID_PARAM, "freq_factors[%d] is not above 0", i);
+            f /= d;
+        }
+        if (yarn) {
+            const double ramp = std::min(1.0, std::max(0.0, (i - low) / std::max(high - low, 0.001)));
+            f = f / p->yarn_factor * ramp + f * (1.0 - ramp);
+        }
+        turns[i] = f / (2.0 * pi);
+    }
+    ggq_rope* r = new ggq_rope;
+    r->head_dim = hd;
+    r->rot_dim = rot;
+    r->layout = p->layout;
+    r->mag = (float)(yarn ? mag * (1.0 + 0.1 * std::log(p->yarn_factor)) : mag);
+    hipError_t e = hipMalloc((void**)&r->turns, sizeof(double) * turns.size());
+    if (e == hipSuccess && (e = hipMemcpy(r->turns, turns.data(), sizeof(double) * turns.size(), hipMemcpyHostToDevice)) != hipSuccess)
+        hipFree(r->turns);
+    if (e != hipSuccess) {
+        delete r;
+        return hip_status(c, e, "rope table");
+    }
+    c->ropes.insert(r);
+    *out = r;
+    return set_status(c, GGQ_OK);
+    GGQ_END(c)
+}
+
+int ggq_rope_free(ggq_ctx* c, ggq_rope* r) {
+    GGQ_GUARD(c)
+    if (!r || !c->ropes.erase(r)) return set_status(c, GGQ_INVALID_PARAM, "unknown rope handle");
+    hipError_t e = hipFree(r->turns);  // waits for queued work
+    delete r;
+    return hip_status(c, e, "rope free");
+    GGQ_END(c)
+}
+
+int ggq_rope_dev(ggq_ctx* c, const ggq_rope* rope, const ggq_rope_heads* sets, int n_sets, const int32_t* pos, int n_tok,
+                 float eps, void* stream) {
+    GGQ_GUARD(c)
+    if (!rope || !c->ropes.count(const_cast<ggq_rope*>(rope))) return set_status(c, GGQ_INVALID_PARAM, "unknown rope handle");
+    if (n_sets < 1 || n_sets > GGQ_MAX_ROPE_SETS || !sets || n_tok < 0)
+        return set_status(c, GGQ_INVALID_PARAM, "need 1 to %d sets of heads and n_tok >= 0", GGQ_MAX_ROPE_SETS);
+    ggq::RopeArgs a{};
+    for (int i = 0; i < n_sets; i++) {
+        const ggq_rope_heads& h = sets[i];
+        const int64_t row = (int64_t)h.n_head * rope->head_dim;
+        if (h.n_head < 1 || h.n_head > 65536 || h.ldx < row || h.ldo < row)
+            return set_status(c, GGQ_INVALID_PARAM, "set %d: need n_head in 1..65536 and ldx, ldo of a row or more", i);
+        if (h.out_type != GGQ_TYPE_F32 && h.out_type != GGQ_TYPE_F16)
+            return set_status(c, GGQ_INVALID_PARAM, "set %d: out_type must be F32 or F16 (got %d)", i, h.out_type);
+        if (n_tok && (!h.x || !h.out)) return set_status(c, GGQ_INVALID_PARAM, "set %d: null x/out", i);
+        if (!aligned16(h.x) || !aligned16(h.out) || !aligned16(h.norm_w) || h.ldx % 4 || h.ldo % (h.out_type == GGQ_TYPE_F16 ? 8 : 4))
+            return set_status(c, GGQ_INVALID_PARAM, "set %d: x, norm_w, out and their rows must be 16-byte aligned", i);
+        if (h.x == h.out && (h.out_type != GGQ_TYPE_F32 || h.ldx != h.ldo))
+            return set_status(c, GGQ_INVALID_PARAM, "set %d: in place takes F32 and ldo = ldx", i);
+        a.set[i] = h;
+    }
+    if (n_tok == 0) return set_status(c, GGQ_OK);
+    if (!pos) return set_status(c, GGQ_INVALID_PARAM, "null pos");
+    a.n_sets = n_sets;
+    a.n_tok = n_tok;
+    a.head_dim = rope->head_dim;
+    a.rot_dim = rope->rot_dim;
+    a.layout = rope->layout;
+    a.turns = rope->turns;
+    a.mag = rope->mag;
+    a.eps = eps;
+    a.pos = pos;
+    return hip_status(c, ggq::launch_rope(a, pick_stream(c, stream)), "rope");
+    GGQ_END(c)
+}
+
+int64_t ggq_kv_page_bytes(const ggq_kv_cache* k) {
+    if (!k || k->page_len < 1 || k->page_len % ggq::kKvTile || k->n_kv_head < 1 || k->n_kv_head > 65535 / 2) return 0;
+    if (k->head_dim != 64 && k->head_dim != 128 && k->head_dim != 256) return 0;
+    for (int t : {k->k_type, k->v_type})
+        if (t != GGQ_KV_MXFP4 && t != GGQ_KV_MXFP8) return 0;
+    const int64_t records = (int64_t)k->n_kv_head * (k->page_len / ggq::kKvTile);
+    return records > (int64_t)1 << 40 ? 0 : records * ggq::kv_record_bytes(*k);
+}
+
+static int check_kv(ggq_ctx* c, const ggq_kv_cache* k, const ggq_kv_seqs* q) {
+    if (!k || !q) return set_status(c, GGQ_INVALID_PARAM, "null cache/sequences");
+    if (!ggq_kv_page_bytes(k))
+        return set_status(c, GGQ_INVALID_PARAM,
+                          "cache: head_dim 64, 128 or 256, page_len a multiple of %d, formats MXFP4 / MXFP8 (got %d, %d, %d / %d)",
+                          ggq::kKvTile, k->head_dim, k->page_len, k->k_type, k->v_type);
+    if (!k->pages || !aligned16(k->pages) || k->n_pages < 1)
+        return set_status(c, GGQ_INVALID_PARAM, "cache: pages must be a 16-byte aligned pointer to at least one page");
+    if (q->n_seq < 0 || q->n_seq > 65535 || q->table_len < 1 || q->max_len < 0 ||
+        (int64_t)q->table_len * k->page_len > INT32_MAX)
+        return set_status(c, GGQ_INVALID_PARAM, "need n_seq in 0..65535, table_len >= 1, max_len >= 0, fewer than 2^31 positions a sequence");
+    if (q->n_seq && (!q->pages || !q->len)) return set_status(c, GGQ_INVALID_PARAM, "null page table/lengths");
+    return GGQ_OK;
+}
+
+static int kv_rows(ggq_ctx* c, const ggq_kv_cache* k, const ggq_kv_seqs* q, const ggq::KvRows& r, bool store, void* stream) {
+    const int st = check_kv(c, k, q);
+    if (st != GGQ_OK) return st;
+    if (r.type != GGQ_TYPE_F32 && r.type != GGQ_TYPE_F16)
+        return set_status(c, GGQ_INVALID_PARAM, "rows must be F32 or F16 (got %d)", r.type);
+    const int64_t row = (int64_t)k->n_kv_head * k->head_dim;
+    if (r.n_rows < 0 || r.ldk < row || r.ldv < row)
+        return set_status(c, GGQ_INVALID_PARAM, "need n_rows >= 0 and ldk, ldv of a row or more");
+    if (r.n_rows == 0 || q->n_seq == 0) return set_status(c, GGQ_OK);
+    if (!r.k || !r.v) return set_status(c, GGQ_INVALID_PARAM, "null k/v");
+    const int per = r.type == GGQ_TYPE_F32 ? 4 : 8;
+    if (!aligned16(r.k) || !aligned16(r.v) || r.ldk % per || r.ldv % per)
+        return set_status(c, GGQ_INVALID_PARAM, "k, v and their rows must be 16-byte aligned");
+    return hip_status(c, ggq::launch_kv_rows(*k, *q, r, store, pick_stream(c, stream)), store ? "kv store" : "kv load");
+}
+
+int ggq_kv_store_dev(ggq_ctx* c, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off, int n_rows,
+                     const void* k, int64_t ldk, const void* v, int64_t ldv, int type, void* stream) {
+    GGQ_GUARD(c)
+    return kv_rows(c, cache, seqs, ggq::KvRows{row_off, n_rows, const_cast<void*>(k), const_cast<void*>(v), ldk, ldv, type},
+                   true, stream);
+    GGQ_END(c)
+}
+
+int ggq_kv_load_dev(ggq_ctx* c, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off, int n_rows,
+                    void* k, int64_t ldk, void* v, int64_t ldv, int type, void* stream) {
+    GGQ_GUARD(c)
+    return kv_rows(c, cache, seqs, ggq::KvRows{row_off, n_rows, k, v, ldk, ldv, type}, false, stream);
+    GGQ_END(c)
+}
+
+// The scale of an attention call in powers of two, 1 / sqrt(head_dim) for 0.
+static float log2_scale(float scale, int head_dim) {
+    return (float)((scale == 0.0f ? 1.0 / std::sqrt((double)head_dim) : (double)scale) * 1.44269504088896340736);
+}
+
+int ggq_attention_kv_dev(ggq_ctx* c, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const float* q, int64_t ldq,
+                         int n_head, float scale, int window, float* out, int64_t ldo, void* stream) {
+    GGQ_GUARD(c)
+    const int st = check_kv(c, cache, seqs);
+    if (st != GGQ_OK) return st;
+    if (n_head < 1 || n_head > 65535 || n_head % cache->n_kv_head)
+        return set_status(c, GGQ_INVALID_PARAM, "need n_head a multiple of n_kv_head, at most 65535");
+    const int64_t row = (int64_t)n_head * cache->head_dim;
+    if (ldq < row || ldo < row || window < 0 || !std::isfinite(scale))
+        return set_status(c, GGQ_INVALID_PARAM, "need ldq, ldo of a row or more, window >= 0 and a finite scale");
+    if (seqs->n_seq == 0) return set_status(c, GGQ_OK);
+    if (!q || !out) return set_status(c, GGQ_INVALID_PARAM, "null q/out");
+    if (!aligned16(q) || ldq % 4) return set_status(c, GGQ_INVALID_PARAM, "q and its rows must be 16-byte aligned");
+    const hipStream_t s = pick_stream(c, stream);
+    ggq::KvAttnArgs a{*cache, *seqs, q, ldq, n_head, log2_scale(scale, cache->head_dim), window, out, ldo};
+    int splits = ggq::kv_attn_splits(a);
+    float* ws = nullptr;
+    if (splits > 1) {
+        ws = (float*)lane_ws(c, s, sizeof(float) * ggq::kv_attn_ws_floats(a, splits), nullptr, 0);
+        if (!ws) splits = 1;  // one workgroup a head group: slower, no workspace
+    }
+    const hipError_t e = ggq::launch_kv_attn(a, splits, ws, s);
+    lane_done(c, s);
+    return hip_status(c, e, "cache attention");
+    GGQ_END(c)
+}
+
+int ggq_attention_prompt_dev(ggq_ctx* c, const ggq_attention_prompt_params* p, void* stream) {
+    GGQ_GUARD(c)
+    if (!p) return set_status(c, GGQ_INVALID_PARAM, "null params");
+    if (p->type != GGQ_TYPE_F32 && p->type != GGQ_TYPE_F16)
+        return set_status(c, GGQ_INVALID_PARAM, "k and v must be F32 or F16 (got %d)", p->type);
+    if (p->n_head < 1 || p->n_kv_head < 1 || p->n_head % p->n_kv_head || p->n_head > 65535)
+        return set_status(c, GGQ_INVALID_PARAM, "need n_head a multiple of n_kv_head, at most 65535");
+    const int hd = p->head_dim;
+    if (hd != 64 && hd != 128 && hd != 256) return set_status(c, GGQ_INVALID_PARAM, "head_dim must be 64, 128 or 256 (got %d)", hd);
+    const int64_t qrow = (int64_t)p->n_head * hd, krow = (int64_t)p->n_kv_head * hd;
+    if (p->ldq < qrow || p->ldo < qrow || p->ldk < krow || p->ldv < krow)
+        return set_status(c, GGQ_INVALID_PARAM, "row strides must hold a row's heads");
+    if (p->n_rows < 0 || p->n_kv_rows < 0 || p->n_seq < 0 || p->window < 0 || !std::isfinite(p->scale))
+        return set_status(c, GGQ_INVALID_PARAM, "need n_rows, n_kv_rows, n_seq, window >= 0 and a finite scale");
+    if (p->n_rows == 0 || p->n_seq == 0) return set_status(c, GGQ_OK);
+    if (!p->q || !p->out || !p->q_off || (p->n_kv_rows && (!p->k || !p->v)))
+        return set_status(c, GGQ_INVALID_PARAM, "null q/k/v/out/q_off");
+    const int per = p->type == GGQ_TYPE_F32 ? 4 : 8;
+    if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || p->ldq % 4 || p->ldo % 4 ||
+        p->ldk % per || p->ldv % per)
+        return set_status(c, GGQ_INVALID_PARAM, "q, k, v, out and their rows must be 16-byte aligned");
+    ggq_attention_prompt_params a = *p;
+    a.scale = log2_scale(p->scale, hd);
+    return hip_status(c, ggq::launch_attn_prompt(a, pick_stream(c, stream)), "prompt attention");
     GGQ_END(c)
 }
 

@@ -31,6 +31,21 @@ class GgmlType(enum.IntEnum):
     IQ4_XS = 23
 
 
+class KvType(enum.IntEnum):
+    """Formats of a quantized KV cache (include/ggq.h)."""
+    MXFP4 = 4
+    MXFP8 = 8
+
+
+class RopeLayout(enum.IntEnum):
+    HALF = 0
+    INTERLEAVED = 1
+
+
+# element types of rows (GGML ids)
+TYPE_F32, TYPE_F16 = 0, 1
+
+
 class Producer(enum.IntEnum):
     RMS_NORM = 1
     SWIGLU = 2
@@ -107,6 +122,43 @@ class GemvFusedDesc(ctypes.Structure):
                 ("rms_eps", ctypes.c_float), ("silu", ctypes.c_int)]
 
 
+class RopeParams(ctypes.Structure):
+    """ggq_rope_params (include/ggq.h)."""
+    _fields_ = [("head_dim", ctypes.c_int), ("rot_dim", ctypes.c_int), ("layout", ctypes.c_int),
+                ("base", ctypes.c_double), ("position_scale", ctypes.c_double), ("freq_factors", ctypes.c_void_p),
+                ("yarn_factor", ctypes.c_double), ("yarn_ctx", ctypes.c_double), ("yarn_beta_fast", ctypes.c_double),
+                ("yarn_beta_slow", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+class RopeHeads(ctypes.Structure):
+    """ggq_rope_heads (include/ggq.h)."""
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("n_head", ctypes.c_int), ("norm_w", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("out_type", ctypes.c_int)]
+
+
+class KvCache(ctypes.Structure):
+    """ggq_kv_cache (include/ggq.h)."""
+    _fields_ = [("pages", ctypes.c_void_p), ("n_pages", ctypes.c_int), ("page_len", ctypes.c_int),
+                ("n_kv_head", ctypes.c_int), ("head_dim", ctypes.c_int), ("k_type", ctypes.c_int),
+                ("v_type", ctypes.c_int)]
+
+
+class KvSeqs(ctypes.Structure):
+    """ggq_kv_seqs (include/ggq.h)."""
+    _fields_ = [("n_seq", ctypes.c_int), ("table_len", ctypes.c_int), ("max_len", ctypes.c_int),
+                ("pages", ctypes.c_void_p), ("len", ctypes.c_void_p)]
+
+
+class AttnPromptParams(ctypes.Structure):
+    """ggq_attention_prompt_params (include/ggq.h)."""
+    _fields_ = [("type", ctypes.c_int), ("n_head", ctypes.c_int), ("n_kv_head", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("k", ctypes.c_void_p), ("ldk", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("ldv", ctypes.c_int64), ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64),
+                ("n_rows", ctypes.c_int), ("n_kv_rows", ctypes.c_int), ("n_seq", ctypes.c_int),
+                ("q_off", ctypes.c_void_p), ("kv_off", ctypes.c_void_p), ("scale", ctypes.c_float),
+                ("window", ctypes.c_int)]
+
+
 class MulMatParams(ctypes.Structure):
     """MulMatParams (include/ggnpu/backend.h:21-35)."""
     _fields_ = [
@@ -144,6 +196,15 @@ SIGNATURES = {
     "ggq_mul_mat_q8_dev": (_I, [_P, _P, _U32, _I64, _I64, _P, _P, _I, _P, _I, _P]),
     "ggq_logits_argmax_dev": (_I, [_P, _P, _U32, _I64, _I64, _P, _I, _I, _P, _P, _P, _P]),
     "ggq_attention_decode_dev": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I64, _I64, _P, _P]),
+    "ggq_rope_create": (_I, [_P, ctypes.POINTER(RopeParams), ctypes.POINTER(_P)]),
+    "ggq_rope_free": (_I, [_P, _P]),
+    "ggq_rope_dev": (_I, [_P, _P, ctypes.POINTER(RopeHeads), _I, _P, _I, ctypes.c_float, _P]),
+    "ggq_kv_page_bytes": (_I64, [ctypes.POINTER(KvCache)]),
+    "ggq_kv_store_dev": (_I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(KvSeqs), _P, _I, _P, _I64, _P, _I64, _I, _P]),
+    "ggq_kv_load_dev": (_I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(KvSeqs), _P, _I, _P, _I64, _P, _I64, _I, _P]),
+    "ggq_attention_kv_dev": (_I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(KvSeqs), _P, _I64, _I, ctypes.c_float, _I,
+                                  _P, _I64, _P]),
+    "ggq_attention_prompt_dev": (_I, [_P, ctypes.POINTER(AttnPromptParams), _P]),
     "ggq_mul_mat_q8_batch_dev": (_I, [_P, _P, _I, _U32, _I64, _P, _P, _I, _P]),
     "ggq_dequant_dev": (_I, [_P, _P, _U32, _I64, _P, _P]),
     "ggq_quantize_act_dev": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
@@ -253,6 +314,34 @@ class Context:
 
     def sync(self):
         self.check(self.lib.ggq_sync(self.h), "sync")
+
+
+class Rope:
+    """Owning handle of a ggq_rope: the frequencies of a model's heads.  `params` are the fields of ggq_rope_params;
+    freq_factors is a sequence of floats or None."""
+
+    def __init__(self, ctx, head_dim, rot_dim=0, layout=RopeLayout.HALF, base=0.0, *, freq_factors=None, **params):
+        p = RopeParams(head_dim=head_dim, rot_dim=rot_dim, layout=int(layout), base=base, **params)
+        if freq_factors is not None:
+            rot = rot_dim or head_dim
+            if len(freq_factors) != rot // 2:
+                raise ValueError(f"freq_factors: {len(freq_factors)} values for {rot // 2} pairs")
+            f = (ctypes.c_float * (rot // 2))(*freq_factors)
+            p.freq_factors = ctypes.addressof(f)
+        self.ctx, h = ctx, ctypes.c_void_p()
+        ctx.check(ctx.lib.ggq_rope_create(ctx.h, ctypes.byref(p), ctypes.byref(h)), "rope_create")
+        self.h = h
+
+    def close(self):
+        if self.h and self.ctx.h:
+            self.ctx.lib.ggq_rope_free(self.ctx.h, self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class GgufFile:

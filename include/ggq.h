@@ -236,6 +236,181 @@ int ggq_logits_argmax_dev(ggq_ctx* ctx, const void* W, uint32_t type, int64_t N,
 int ggq_attention_decode_dev(ggq_ctx* ctx, const float* Q, const float* K, const float* V, int n_tok, int n_head,
                              int n_kv_head, int head_dim, int64_t ctx_len, int64_t pos0, float* out, void* stream);
 
+/* ---- between the q/k/v and the output projections: rotary positions, a
+ * quantized KV cache, its attention, attention of whole prompts.  Element
+ * types of rows are GGML ids: */
+#define GGQ_TYPE_F32 0
+#define GGQ_TYPE_F16 1
+
+/* Rotary positions.  A handle holds the frequencies of a model's heads, made
+ * once in 64 bits: pair i of the first rot_dim values of a head turns by
+ *   pos * f_i,  f_i = position_scale * base^(-2 i / rot_dim) / freq_factors[i]
+ * and cosine and sine are multiplied by `magnitude`.  With yarn_factor > 1
+ * the pairs that turn less often than yarn_beta_fast times over yarn_ctx
+ * positions are slowed down towards f_i / yarn_factor, wholly from
+ * yarn_beta_slow times downwards, and the magnitude gets the factor
+ * 1 + 0.1 ln(yarn_factor).  A zeroed field means its default.  No
+ * counterpart as a handle: the reference computes the angles per call (its
+ * Backend::rope and main.cpp:3325-3343). */
+#define GGQ_ROPE_HALF 0        /* pairs (i, i + rot_dim / 2) */
+#define GGQ_ROPE_INTERLEAVED 1 /* pairs (2 i, 2 i + 1) */
+typedef struct ggq_rope ggq_rope;
+typedef struct {
+    int head_dim;  /* multiple of 8, at most 512 */
+    int rot_dim;   /* multiple of 8, at most head_dim; values behind it pass through (0: head_dim) */
+    int layout;    /* GGQ_ROPE_HALF or GGQ_ROPE_INTERLEAVED */
+    double base;   /* frequency base (0: 10000) */
+    double position_scale;     /* linear scaling of the positions (0: 1) */
+    const float* freq_factors; /* host memory, [rot_dim / 2] (a GGUF file's rope_freqs.weight), or NULL */
+    double yarn_factor;        /* 0 or 1: off */
+    double yarn_ctx;           /* positions the model was trained on; needed with yarn_factor > 1 */
+    double yarn_beta_fast;     /* 0: 32 */
+    double yarn_beta_slow;     /* 0: 1 */
+    double magnitude;          /* 0: 1 */
+} ggq_rope_params;
+int ggq_rope_create(ggq_ctx* ctx, const ggq_rope_params* params, ggq_rope** out);
+int ggq_rope_free(ggq_ctx* ctx, ggq_rope* rope);
+
+/* Turns the heads of n_tok rows to the positions pos[t] (device, int32; any
+ * sign), in one launch for up to GGQ_MAX_ROPE_SETS sets of heads (q and k).
+ * Per head: RMSNorm with weight norm_w first where norm_w is set (x * (1 /
+ * sqrt(mean(x^2) + eps)) * norm_w, as models with normalised q and k heads
+ * have it), then the rotation.  Row t of a set has n_head heads of head_dim
+ * values, dense, at x + t * ldx; results go to out + t * ldo as out_type (a
+ * cache slab's rows, for instance).  out may be x itself with GGQ_TYPE_F32
+ * and ldo = ldx; other overlaps are not allowed.  x, norm_w and out 16-byte
+ * aligned, ldx and ldo multiples of 4 (8 for an f16 out).  Angles are reduced
+ * in 64 bits: far positions are as exact as near ones. */
+#define GGQ_MAX_ROPE_SETS 2
+typedef struct {
+    const float* x;
+    int64_t ldx;
+    int n_head;
+    const float* norm_w; /* [head_dim] or NULL: no norm */
+    void* out;
+    int64_t ldo;
+    int out_type; /* GGQ_TYPE_F32 or GGQ_TYPE_F16 */
+} ggq_rope_heads;
+int ggq_rope_dev(ggq_ctx* ctx, const ggq_rope* rope, const ggq_rope_heads* sets, int n_sets, const int32_t* pos,
+                 int n_tok, float eps, void* stream);
+
+/* One layer's quantized KV cache: a pool of pages of page_len positions each
+ * (a multiple of 32; a page of the whole context makes it a plain slab).
+ * Blocks of 32 values along a head share a power of two 2^(byte - 127):
+ *   GGQ_KV_MXFP4  e2m1 codes: 4.25 bits a value
+ *   GGQ_KV_MXFP8  e4m3 codes: 8.25 bits a value
+ * K and V formats are chosen apart.  The scale is the smallest power of two
+ * (2^-126 at least) that rounds the block's largest magnitude to the
+ * largest code or below (amax <= 7 * 2^e, 464 * 2^e); codes are the nearest,
+ * ties to the even one.  A block with a value that is not finite gets the
+ * byte 255 and reads back as NaN.  (A magnitude above 2.9e38 may round to
+ * 2^128, which reads back as infinite.)
+ *
+ * A page holds [n_kv_head][page_len / 32] records of 32 positions of one kv
+ * head, laid out for the loads of the attention kernel: K codes, V codes, K
+ * scales, V scales.  With hd = head_dim, position p and value d of a record:
+ *   K code  lane 16 (d / (hd/4)) + p % 16, its value (p / 16) (hd/4) + d % (hd/4)
+ *   V code  lane 16 ((p % 16) / 4) + d / (hd/16), its value
+ *           (4 (p / 16) + p % 4) (hd/16) + d % (hd/16)
+ *           byte b of lane l stands at 1024 (b / 16) + 16 l + b % 16; of two
+ *           4-bit codes in a byte the first is the low one
+ *   K scale of block c: byte (16 c + p % 16) 2 + p / 16
+ *   V scale of block c: byte (4 c + (p % 16) / 4) 8 + 4 (p / 16) + p % 4
+ * No reference counterpart (the reference's cache is fp32, kv_cache.cpp). */
+#define GGQ_KV_MXFP4 4
+#define GGQ_KV_MXFP8 8
+typedef struct {
+    void* pages;  /* device, 16-byte aligned, n_pages * ggq_kv_page_bytes bytes */
+    int n_pages;
+    int page_len;
+    int n_kv_head;
+    int head_dim; /* 64, 128 or 256 */
+    int k_type, v_type;
+} ggq_kv_cache;
+/* Bytes of a page (0 if a field is not supported; pages and n_pages are not
+ * looked at). */
+int64_t ggq_kv_page_bytes(const ggq_kv_cache* cache);
+
+/* The sequences of a call: position p of sequence s stands in page
+ * pages[s * table_len + p / page_len].  An entry outside [0, n_pages) means
+ * that there is no such page: nothing is stored to it or loaded from it, and
+ * attention passes over its positions.  len[s] counts the sequence's
+ * positions, those that a store call adds included; max_len is an upper bound
+ * of them (attention reads none behind it).  A page that is read may belong
+ * to several sequences; one that is written must not. */
+typedef struct {
+    int n_seq;
+    int table_len;        /* entries of a sequence in `pages` */
+    int max_len;
+    const int32_t* pages; /* device, [n_seq][table_len] */
+    const int32_t* len;   /* device, [n_seq] */
+} ggq_kv_seqs;
+
+/* Quantizes n_rows K and V rows ([n_kv_head][head_dim] values of `type`,
+ * GGQ_TYPE_F32 or GGQ_TYPE_F16, row r at r * ldk and r * ldv) into the cache.
+ * Rows row_off[s] .. row_off[s+1]-1 (device, [n_seq + 1]; NULL: one row a
+ * sequence) are the last ones of sequence s: the last goes to position
+ * len[s] - 1.  Rows of no sequence, positions below 0 or behind the page
+ * table and positions without a page are passed over.  k and v 16-byte
+ * aligned, ldk and ldv multiples of 16 bytes. */
+int ggq_kv_store_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off,
+                     int n_rows, const void* k, int64_t ldk, const void* v, int64_t ldv, int type, void* stream);
+/* The reverse: rows row_off[s] .. row_off[s+1]-1 of k and v receive the last
+ * positions of sequence s (all of them where there are len[s] rows).  Rows
+ * for which there is nothing to load stay as they were.  Exact in fp32;
+ * GGQ_TYPE_F16 rounds once. */
+int ggq_kv_load_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off,
+                    int n_rows, void* k, int64_t ldk, void* v, int64_t ldv, int type, void* stream);
+
+/* Attention of one token of each sequence over its quantized cache: query row
+ * s (n_head heads at q + s * ldq) sits at position len[s] - 1 and sees
+ * positions 0 .. len[s]-1, with window > 0 the last `window` of them.  Query
+ * head h reads kv head h / (n_head / n_kv_head); any ratio.  out + s * ldo =
+ * softmax(q.k * scale) . V with the values the codes stand for (scale 0: 1 /
+ * sqrt(head_dim)); zeros for a row that sees nothing.  What cache positions
+ * behind len hold does not matter.  All products are exact in fp32 terms
+ * (three bf16 parts of q and of the softmax weights).  q 16-byte aligned,
+ * ldq a multiple of 4.  The positions are split over workgroups by max_len;
+ * where there is no workspace for the parts one workgroup takes them all. */
+int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const float* q, int64_t ldq,
+                         int n_head, float scale, int window, float* out, int64_t ldo, void* stream);
+
+/* Causal attention of whole prompts (prefill), packed one behind the other:
+ * rows q_off[s] .. q_off[s+1]-1 of q and out and rows kv_off[s] ..
+ * kv_off[s+1]-1 of k and v belong to sequence s (device, [n_seq + 1] each,
+ * ascending, within n_rows and n_kv_rows; kv_off NULL: the same as q_off).
+ * The last query row sees all of its sequence's keys, each row before it one
+ * less: a prompt's next chunk is n query rows against all positions so far.
+ * With window > 0 a row sees the last `window` of those only.  A row that
+ * sees nothing gets zeros; rows outside of all sequences stay as they were.
+ * Keys that a row does not see never touch it, whatever they hold.  Rows are
+ * [n_head or n_kv_head][head_dim] values, dense, with row strides ld*; q and
+ * out fp32, k and v of `type` (GGQ_TYPE_F32 or GGQ_TYPE_F16, a slab
+ * [position][n_kv_head][head_dim] as it is); head_dim 64, 128 or 256; any
+ * n_head / n_kv_head.  Replaces the per-row flash_attn loop of
+ * main.cpp:3352-3410.  Pointers 16-byte aligned, strides multiples of 16
+ * bytes. */
+typedef struct {
+    int type;
+    int n_head, n_kv_head, head_dim;
+    const float* q;
+    int64_t ldq;
+    const void* k;
+    int64_t ldk;
+    const void* v;
+    int64_t ldv;
+    float* out;
+    int64_t ldo;
+    int n_rows;    /* rows of q and out */
+    int n_kv_rows; /* rows of k and v */
+    int n_seq;
+    const int32_t* q_off;
+    const int32_t* kv_off;
+    float scale; /* 0: 1 / sqrt(head_dim) */
+    int window;  /* 0: none */
+} ggq_attention_prompt_params;
+int ggq_attention_prompt_dev(ggq_ctx* ctx, const ggq_attention_prompt_params* params, void* stream);
+
 /* C = sa[m] * sum_k qa[m][k] * w[n][k]: the GGQ_ACT_Q8_ROW matmul on
  * activations already quantized by ggq_quantize_act_dev (row mode; qa dense
  * [M][K], 16-byte aligned, sa [M]).  Lets callers quantize an input once
