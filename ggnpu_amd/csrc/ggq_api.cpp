@@ -1325,7 +1325,12 @@ int ggq_attention_prompt_dev(ggq_ctx* c, const ggq_attention_prompt_params* p, v
         return set_status(c, GGQ_INVALID_PARAM, "q, k, v, out and their rows must be 16-byte aligned");
     ggq_attention_prompt_params a = *p;
     a.scale = log2_scale(p->scale, hd);
-    return hip_status(c, ggq::launch_attn_prompt(a, pick_stream(c, stream)), "prompt attention");
+    const hipStream_t s = pick_stream(c, stream);
+    const ggq::AttnPromptPlan pl = ggq::attn_prompt_plan(a);
+    void* ws = lane_ws(c, s, pl.ws_bytes, nullptr, 0);
+    const hipError_t e = ws ? ggq::launch_attn_prompt(a, pl, ws, s) : ggq::launch_attn_prompt_rows(a, s);
+    lane_done(c, s);
+    return hip_status(c, e, "prompt attention");
     GGQ_END(c)
 }
 
