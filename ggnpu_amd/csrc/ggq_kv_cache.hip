@@ -8,6 +8,7 @@
 // happens between the cache and the matrix cores.  A scale byte of 255 gives
 // an infinite scale operand, which the conversion turns into NaN.
 #include <algorithm>
+#include <cstdlib>
 
 #include "ggq_attn.h"
 #include "ggq_launch.h"
@@ -35,40 +36,48 @@ __device__ __forceinline__ Place place_of(const ggq_kv_cache& c, const ggq_kv_se
     return Place{(uint8_t*)c.pages + r * rec_bytes, (int)(in % kKvTile)};
 }
 
-// Rows to or from the pages.  A workgroup takes 2048 values of one kv head, K
-// (z = 0) or V, a thread 8 consecutive ones; 4 threads share a block of 32.
-// The rows' sequences are found by all threads together: one strided look
-// over row_off for the first row, a step forward for each sequence that ends
-// among the rows.
-template <int HD, int BITS, bool VALUE, bool STORE, typename T>
+// Rows to or from the pages.  A workgroup takes U times 2048 values of one kv
+// head, K (z = 0) or V, a thread 8 consecutive ones of each of U rows; 4 threads share a
+// block of 32.  The rows' sequences are found by all threads together: one
+// strided look over row_off for the first row, a step forward for each
+// sequence that ends among the rows.  A row's place is three dependent
+// loads away (offsets and length, page, codes), so large calls have U = 4 of
+// them in flight a thread.
+template <int HD, int BITS, bool VALUE, bool STORE, int U, typename T>
 __device__ __forceinline__ void rows_body(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r, int64_t rec_bytes) {
-    constexpr int RPW = 2048 / HD;  // rows of a workgroup
+    constexpr int RPW = 2048 / HD;  // rows of a workgroup's pass
     constexpr int TPR = HD / 8;     // threads of a row
-    const int tid = threadIdx.x, head = blockIdx.y;
-    const int row0 = blockIdx.x * RPW, row = row0 + tid / TPR, d = tid % TPR * 8;
-    int seq = row;
-    int64_t pos = -1;
-    if (r.row_off) {
-        seq = 0;
+    const int tid = threadIdx.x, head = blockIdx.y, d = tid % TPR * 8;
+    const int row0 = blockIdx.x * RPW * U;
+    int first = 0;
+    if (r.row_off)
         for (int i = 0; i < q.n_seq; i += 256) {
             const int j = i + tid;
-            seq += __syncthreads_count(j < q.n_seq && r.row_off[j + 1] <= row0);
+            first += __syncthreads_count(j < q.n_seq && r.row_off[j + 1] <= row0);
         }
-        while (seq < q.n_seq && r.row_off[seq + 1] <= row) seq++;
-        if (row < r.n_rows && seq < q.n_seq) {
-            const int32_t a = r.row_off[seq], b = r.row_off[seq + 1];
-            if (row >= a) pos = (int64_t)q.len[seq] - b + row;
+    Place pl[U];
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        const int row = row0 + i * RPW + tid / TPR;
+        int seq = row;
+        int64_t pos = -1;
+        if (r.row_off) {
+            seq = first;
+            while (seq < q.n_seq && r.row_off[seq + 1] <= row) seq++;
+            first = seq;
+            if (row < r.n_rows && seq < q.n_seq) {
+                const int32_t a = r.row_off[seq], b = r.row_off[seq + 1];
+                if (row >= a) pos = (int64_t)q.len[seq] - b + row;
+            }
+        } else if (row < r.n_rows && row < q.n_seq) {
+            pos = (int64_t)q.len[row] - 1;
         }
-    } else if (row < r.n_rows && row < q.n_seq) {
-        pos = (int64_t)q.len[row] - 1;
+        pl[i] = Place{nullptr, 0};
+        if (pos >= 0) pl[i] = place_of(c, q, rec_bytes, seq, pos, head);
     }
-    Place pl{nullptr, 0};
-    if (pos >= 0) pl = place_of(c, q, rec_bytes, seq, pos, head);
     // codes of this thread: 8 in one run, or two runs of 4 (V of 64-wide heads)
     constexpr int RUN = VALUE && HD == 64 ? 4 : 8;
-    const int p = pl.p;
-    uint8_t* codes = pl.rec + (VALUE ? kKvTile * HD * c.k_type / 8 : 0);
-    auto at = [&](int e) {  // byte offset of the code of value e
+    auto at = [&](int p, int e) {  // byte offset of the code of value e at position p
         int lane, n;
         if (VALUE) {
             lane = 16 * (p % 16 / 4) + e / (HD / 16);
@@ -81,101 +90,142 @@ __device__ __forceinline__ void rows_body(const ggq_kv_cache& c, const ggq_kv_se
         return 1024 * (b / 16) + 16 * lane + b % 16;
     };
     const int blk = d / 32;
-    uint8_t* sc = pl.rec + kKvTile * HD * (c.k_type + c.v_type) / 8 +
-                  (VALUE ? HD + (4 * blk + p % 16 / 4) * 8 + 4 * (p / 16) + p % 4 : (16 * blk + p % 16) * 2 + p / 16);
-    T* x = (T*)(VALUE ? r.v : r.k) + (int64_t)row * (VALUE ? r.ldv : r.ldk) + (int64_t)head * HD + d;
+    auto codes_of = [&](const Place& x) { return x.rec + (VALUE ? kKvTile * HD * c.k_type / 8 : 0); };
+    auto scale_at = [&](const Place& x) {
+        const int p = x.p;
+        return x.rec + kKvTile * HD * (c.k_type + c.v_type) / 8 +
+               (VALUE ? HD + (4 * blk + p % 16 / 4) * 8 + 4 * (p / 16) + p % 4 : (16 * blk + p % 16) * 2 + p / 16);
+    };
+    auto row_at = [&](int i) {
+        return (T*)(VALUE ? r.v : r.k) + (int64_t)(row0 + i * RPW + tid / TPR) * (VALUE ? r.ldv : r.ldk) + (int64_t)head * HD + d;
+    };
+    struct alignas(16) Run { T x[16 / sizeof(T)]; };
+    constexpr int NR = 8 * sizeof(T) / 16, PR = 16 / sizeof(T);  // 16-byte runs of 8 values
     if constexpr (STORE) {
-        float v[8] = {};
-        if (pl.rec) {
+        Run in[U][NR];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = (float)x[i];
-        }
-        uint32_t m = 0;  // the largest magnitude's bits; infinities and NaN are the largest
+        for (int i = 0; i < U; i++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = max(m, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
-        m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
-        if (!pl.rec) return;
-        // smallest e with amax <= 1.75 * 2^(e + 2), or 1.8125 * 2^(e + 8)
-        const int ex = (int)(m >> 23), over = (m & 0x7FFFFFu) > (BITS == 4 ? 0x600000u : 0x680000u);
-        const bool bad = ex == 255;
-        const int byte = bad ? 255 : max(1, ex - (BITS == 4 ? 2 : 8) + over);
-        const float s = scale_of((uint32_t)byte);
-        uint32_t w[2] = {0, 0};
-        if (!bad) {
-            if constexpr (BITS == 4) {
-                w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[0], v[1], s, 0);
-                w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[2], v[3], s, 1);
-                w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[4], v[5], s, 2);
-                w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[6], v[7], s, 3);
-            } else {
+            for (int j = 0; j < NR; j++) in[i][j] = pl[i].rec ? *((const Run*)row_at(i) + j) : Run{};
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    s16x2 o = {0, 0};
-                    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, v[4 * h], v[4 * h + 1], s, false);
-                    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, v[4 * h + 2], v[4 * h + 3], s, true);
-                    w[h] = __builtin_bit_cast(uint32_t, o);
+        for (int i = 0; i < U; i++) {
+            float v[8];
+            uint32_t m = 0;  // the largest magnitude's bits; infinities and NaN are the largest
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v[j] = (float)in[i][j / PR].x[j % PR];
+                m = max(m, __builtin_bit_cast(uint32_t, v[j]) & 0x7FFFFFFFu);
+            }
+            m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
+            m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
+            if (!pl[i].rec) continue;
+            // smallest e with amax <= 1.75 * 2^(e + 2), or 1.8125 * 2^(e + 8)
+            const int ex = (int)(m >> 23), over = (m & 0x7FFFFFu) > (BITS == 4 ? 0x600000u : 0x680000u);
+            const bool bad = ex == 255;
+            const int byte = bad ? 255 : max(1, ex - (BITS == 4 ? 2 : 8) + over);
+            const float s = scale_of((uint32_t)byte);
+            uint32_t w[2] = {0, 0};
+            if (!bad) {
+                if constexpr (BITS == 4) {
+                    w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[0], v[1], s, 0);
+                    w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[2], v[3], s, 1);
+                    w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[4], v[5], s, 2);
+                    w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], v[6], v[7], s, 3);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        s16x2 o = {0, 0};
+                        o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, v[4 * h], v[4 * h + 1], s, false);
+                        o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, v[4 * h + 2], v[4 * h + 3], s, true);
+                        w[h] = __builtin_bit_cast(uint32_t, o);
+                    }
                 }
             }
+            uint8_t* codes = codes_of(pl[i]);
+            const int p = pl[i].p;
+            if constexpr (BITS == 4 && RUN == 8) {
+                *(uint32_t*)(codes + at(p, d)) = w[0];
+            } else if constexpr (BITS == 4) {
+                *(uint16_t*)(codes + at(p, d)) = (uint16_t)w[0];
+                *(uint16_t*)(codes + at(p, d + 4)) = (uint16_t)(w[0] >> 16);
+            } else if constexpr (RUN == 8) {
+                *(uint2*)(codes + at(p, d)) = make_uint2(w[0], w[1]);
+            } else {
+                *(uint32_t*)(codes + at(p, d)) = w[0];
+                *(uint32_t*)(codes + at(p, d + 4)) = w[1];
+            }
+            if (d % 32 == 0) *scale_at(pl[i]) = (uint8_t)byte;
         }
-        if constexpr (BITS == 4 && RUN == 8) {
-            *(uint32_t*)(codes + at(d)) = w[0];
-        } else if constexpr (BITS == 4) {
-            *(uint16_t*)(codes + at(d)) = (uint16_t)w[0];
-            *(uint16_t*)(codes + at(d + 4)) = (uint16_t)(w[0] >> 16);
-        } else if constexpr (RUN == 8) {
-            *(uint2*)(codes + at(d)) = make_uint2(w[0], w[1]);
-        } else {
-            *(uint32_t*)(codes + at(d)) = w[0];
-            *(uint32_t*)(codes + at(d + 4)) = w[1];
-        }
-        if (d % 32 == 0) *sc = (uint8_t)byte;
     } else {
-        if (!pl.rec) return;
-        const float s = scale_of(*sc);
-        uint32_t w[2];
-        if constexpr (BITS == 4 && RUN == 8) {
-            w[0] = *(const uint32_t*)(codes + at(d));
-        } else if constexpr (BITS == 4) {
-            w[0] = *(const uint16_t*)(codes + at(d)) | (uint32_t)*(const uint16_t*)(codes + at(d + 4)) << 16;
-        } else {
-            w[0] = *(const uint32_t*)(codes + at(d));
-            w[1] = *(const uint32_t*)(codes + (RUN == 8 ? at(d) + 4 : at(d + 4)));
-        }
-        f32x2 o[4];
-        if constexpr (BITS == 4) {
-            o[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 0);
-            o[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 1);
-            o[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 2);
-            o[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 3);
-        } else {
-            o[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], s, false);
-            o[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], s, true);
-            o[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], s, false);
-            o[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], s, true);
+        uint32_t w[U][2];
+        uint8_t sb[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            if (!pl[i].rec) continue;
+            const uint8_t* codes = codes_of(pl[i]);
+            const int p = pl[i].p;
+            sb[i] = *scale_at(pl[i]);
+            if constexpr (BITS == 4 && RUN == 8) {
+                w[i][0] = *(const uint32_t*)(codes + at(p, d));
+            } else if constexpr (BITS == 4) {
+                w[i][0] = *(const uint16_t*)(codes + at(p, d)) | (uint32_t)*(const uint16_t*)(codes + at(p, d + 4)) << 16;
+            } else if constexpr (RUN == 8) {
+                const uint2 x = *(const uint2*)(codes + at(p, d));
+                w[i][0] = x.x;
+                w[i][1] = x.y;
+            } else {
+                w[i][0] = *(const uint32_t*)(codes + at(p, d));
+                w[i][1] = *(const uint32_t*)(codes + at(p, d + 4));
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (T)o[i / 2][i % 2];
+        for (int i = 0; i < U; i++) {
+            if (!pl[i].rec) continue;
+            const float s = scale_of(sb[i]);
+            f32x2 o[4];
+            if constexpr (BITS == 4) {
+                o[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][0], s, 0);
+                o[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][0], s, 1);
+                o[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][0], s, 2);
+                o[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][0], s, 3);
+            } else {
+                o[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i][0], s, false);
+                o[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i][0], s, true);
+                o[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i][1], s, false);
+                o[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i][1], s, true);
+            }
+#pragma unroll
+            for (int j = 0; j < NR; j++) {
+                Run out;
+#pragma unroll
+                for (int e = 0; e < PR; e++) out.x[e] = (T)o[(j * PR + e) / 2][e % 2];
+                *((Run*)row_at(i) + j) = out;
+            }
+        }
     }
 }
 
-template <int HD, int KB, int VB, bool STORE, typename T>
+template <int HD, int KB, int VB, bool STORE, int U, typename T>
 __global__ __launch_bounds__(256) void kv_rows_kernel(ggq_kv_cache c, ggq_kv_seqs q, KvRows r, int64_t rec_bytes) {
-    if (blockIdx.z == 0) rows_body<HD, KB, false, STORE, T>(c, q, r, rec_bytes);
-    else rows_body<HD, VB, true, STORE, T>(c, q, r, rec_bytes);
+    if (blockIdx.z == 0) rows_body<HD, KB, false, STORE, U, T>(c, q, r, rec_bytes);
+    else rows_body<HD, VB, true, STORE, U, T>(c, q, r, rec_bytes);
+}
+
+template <int HD, int KB, int VB, int U, typename T>
+void rows_go(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r, bool store, hipStream_t s) {
+    const int per = U * 2048 / HD;
+    const dim3 grid((unsigned)((r.n_rows + per - 1) / per), (unsigned)c.n_kv_head, 2);
+    if (store) kv_rows_kernel<HD, KB, VB, true, U, T><<<grid, 256, 0, s>>>(c, q, r, kv_record_bytes(c));
+    else kv_rows_kernel<HD, KB, VB, false, U, T><<<grid, 256, 0, s>>>(c, q, r, kv_record_bytes(c));
 }
 
 template <int HD, int KB, int VB> hipError_t rows_launch(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r,
                                                          bool store, hipStream_t s) {
-    const dim3 grid((unsigned)((r.n_rows + 2048 / HD - 1) / (2048 / HD)), (unsigned)c.n_kv_head, 2);
-    const int64_t rb = kv_record_bytes(c);
-    if (r.type == GGQ_TYPE_F32) {
-        if (store) kv_rows_kernel<HD, KB, VB, true, float><<<grid, 256, 0, s>>>(c, q, r, rb);
-        else kv_rows_kernel<HD, KB, VB, false, float><<<grid, 256, 0, s>>>(c, q, r, rb);
-    } else {
-        if (store) kv_rows_kernel<HD, KB, VB, true, _Float16><<<grid, 256, 0, s>>>(c, q, r, rb);
-        else kv_rows_kernel<HD, KB, VB, false, _Float16><<<grid, 256, 0, s>>>(c, q, r, rb);
-    }
+    // four rows a thread once that leaves every CU two workgroups (16 x 4001 rows of 2 heads of 128, f16: 24.3 us with one,
+    // see the launch below; 33 rows of 8 heads are quicker with one)
+    const bool many = (int64_t)r.n_rows * c.n_kv_head * HD * 2 / (4 * 2048) >= 2 * cu_count();
+    if (r.type == GGQ_TYPE_F32) many ? rows_go<HD, KB, VB, 4, float>(c, q, r, store, s) : rows_go<HD, KB, VB, 1, float>(c, q, r, store, s);
+    else many ? rows_go<HD, KB, VB, 4, _Float16>(c, q, r, store, s) : rows_go<HD, KB, VB, 1, _Float16>(c, q, r, store, s);
     return hipGetLastError();
 }
 
@@ -209,7 +259,7 @@ hipError_t launch_kv_rows(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvR
 //   The maximum moves only when a record exceeds it by more than 8 (in powers of
 // two): the weights stay below 2^8 and the sum below 2^8 * positions, and the
 // accumulators are rescaled a few times a sequence.
-// A workgroup has 4 wavefronts that take the records of its part of the
+// A workgroup has 8 wavefronts (4 where their registers allow no more) that take the records of its part of the
 // positions in turn and add up in LDS; kv_join_kernel adds up the parts.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -256,17 +306,29 @@ __device__ __forceinline__ float rows_max(float v) {
     return fmaxf(v, __shfl_xor(v, 32, 64));
 }
 
-// Part `part` of x: x0 = bf16(x), x1 = bf16(x - x0), x2 = bf16(x - x0 - x1).
-__device__ __forceinline__ float bf16_part(float x, int part) {
-    const float x0 = (float)(__bf16)x, r1 = x - x0, x1 = (float)(__bf16)r1, r2 = r1 - x1;
-    return part == 0 ? x0 : part == 1 ? x1 : part == 2 ? (float)(__bf16)r2 : 0.0f;
+// A part of x, its upper 16 bits: three cuts of 8 bits each hold all 24, x0 = x
+// cut, x1 = (x - x0) cut, x2 = x - x0 - x1.  A lane's part is chosen by its masks:
+// what they cut off is subtracted (everything for the column that is zero).
+struct Cuts {
+    uint32_t a, b;
+};
+__device__ __forceinline__ Cuts cuts_of(int part) {
+    return Cuts{part == 0 ? 0u : part == 3 ? 0xFFFFFFFFu : 0xFFFF0000u, part == 2 ? 0xFFFF0000u : 0u};
 }
-__device__ __forceinline__ uint32_t bf16_pack(float a, float b) {  // of values that are bf16 already
+__device__ __forceinline__ float bf16_part(float x, Cuts c) {
+    x -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & c.a);
+    return x - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & c.b);
+}
+__device__ __forceinline__ uint32_t bf16_pack(float a, float b) {  // upper halves
     return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
 }
 
+// Wavefronts of a workgroup, by their registers.
+template <int HD, int NT> constexpr int kv_waves() { return HD == 256 ? 4 : 8; }
+
 template <int HD, int KB, int VB, int NT>
-__global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, float* part) {
+__global__ __launch_bounds__((kv_waves<HD, NT>() * 64)) void kv_attn_kernel(KvAttnArgs a, int splits, float* part) {
+    constexpr int NW = kv_waves<HD, NT>();
     constexpr int KW = HD * KB / 64, VW = HD * VB / 64;  // dwords of a lane's K and V codes
     constexpr int NS = HD / 32;                          // k steps of S^T, blocks of a head
     constexpr int NO = HD / 16;                          // row tiles of O^T
@@ -284,11 +346,13 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
     int64_t lo = a.window > 0 ? (int64_t)a.q.len[seq] - a.window : 0;
     if (lo < 0) lo = 0;
     const int t0 = (int)(lo / kKvTile), t1 = hi > lo ? (int)((hi + kKvTile - 1) / kKvTile) : t0;
-    const int per = (t1 - t0 + splits - 1) / splits;
+    int per = (t1 - t0 + splits - 1) / splits;
+    if (per > NW) per = (per + NW - 1) / NW * NW;
     const int first = t0 + split * per, last = min(t1, first + per);
 
     // columns: query heads hz + 4 n + r / 4, part r % 4
     const int part_i = r & 3;
+    const Cuts cut = cuts_of(part_i);
     bf16x8 qf[NT][NS];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -302,7 +366,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float c0 = h < G ? x[2 * i] * a.scale : 0.0f, c1 = h < G ? x[2 * i + 1] * a.scale : 0.0f;
-                f.w[i] = bf16_pack(bf16_part(c0, part_i), bf16_part(c1, part_i));
+                f.w[i] = bf16_pack(bf16_part(c0, cut), bf16_part(c1, cut));
             }
             qf[n][s] = f.v;
         }
@@ -322,10 +386,10 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
         uint2 vs;
         bool there;
     };
-    const int n_it = last > first + wave ? (last - first - wave + 3) / 4 : 0;  // records of this wavefront
+    const int n_it = last > first + wave ? (last - first - wave + NW - 1) / NW : 0;  // records of this wavefront
     int pages = -1;  // lane i: page of record i of the current 64
     auto look = [&](int it) {
-        const int t = first + wave + 4 * (it + lane);
+        const int t = first + wave + NW * (it + lane);
         pages = it + lane < n_it ? a.q.pages[(int64_t)seq * a.q.table_len + t / tpp] : -1;
         if (pages >= a.c.n_pages) pages = -1;
     };
@@ -333,7 +397,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
         const int page = __builtin_amdgcn_readlane(pages, it & 63);
         x.there = page >= 0;
         if (!x.there) return;
-        const int t = first + wave + 4 * it;
+        const int t = first + wave + NW * it;
         const uint8_t* rec = (const uint8_t*)a.c.pages +
                              (((int64_t)page * a.c.n_kv_head + kvh) * tpp + t % tpp) * RB;
 #pragma unroll
@@ -358,7 +422,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
     };
     auto compute = [&](int it, Rec& x) {
         if (!x.there) return;
-        const int64_t base = (int64_t)(first + wave + 4 * it) * kKvTile;
+        const int64_t base = (int64_t)(first + wave + NW * it) * kKvTile;
         const bool partial = base < lo || base + kKvTile > hi;
         // scores
         f32x4 st[2][NT];
@@ -439,7 +503,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
             for (int j = 0; j < 8; j++) {
                 const float e = __builtin_amdgcn_exp2f(sv[n][j] - mm);
                 l[n] += e;
-                w[j] = bf16_part(e, part_i);
+                w[j] = bf16_part(e, cut);
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) pf[n].w[j] = bf16_pack(w[2 * j], w[2 * j + 1]);
@@ -482,8 +546,8 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
         cur = nxt;
     }
 
-    // the four wavefronts' parts
-    __shared__ float sm[4][4 * NT], sl[4][4 * NT], so[4][4 * NT][HD];
+    // the wavefronts' parts
+    __shared__ float sm[NW][4 * NT], sl[NW][4 * NT], so[NW][4 * NT][HD];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         float s = l[n];  // of this group's positions; the quad's four lanes hold the same
@@ -500,15 +564,15 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
             }
     }
     __syncthreads();
-    for (int e = tid; e < 4 * NT * HD; e += 256) {
+    for (int e = tid; e < 4 * NT * HD; e += NW * 64) {
         const int h = e / HD, d = e % HD;
         if (hz + h >= G) break;
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; w++) mx = fmaxf(mx, sm[w][h]);
+        for (int w = 0; w < NW; w++) mx = fmaxf(mx, sm[w][h]);
         float ls = 0.0f, os = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             const float al = sm[w][h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][h] - mx);
             ls = fmaf(sl[w][h], al, ls);
             os = fmaf(so[w][h][d], al, os);
@@ -525,28 +589,56 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs a, int splits, 
     }
 }
 
-// The parts of one head: a thread a value, parts in their order.
-__global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs a, int splits, const float* part, int HD) {
-    const int head = blockIdx.x, seq = blockIdx.y, d = threadIdx.x;
+// The parts of one head: their weights first, then a thread a value and group of parts,
+// in an order that does not depend on timing.
+constexpr int kKvMaxSplits = 256;
+template <int HD> __global__ __launch_bounds__(512) void kv_join_kernel(KvAttnArgs a, int splits, const float* part) {
+    constexpr int NG = 512 / HD, B = 8;
+    __shared__ float w[kKvMaxSplits], red[8], go[NG][HD];
+    const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, d = tid % HD, grp = tid / HD;
     const float* po = part + ((int64_t)seq * a.n_head + head) * splits * (HD + 2);
-    float mx = -INFINITY;
-    for (int i = 0; i < splits; i++) mx = fmaxf(mx, po[(int64_t)i * (HD + 2) + HD]);
-    float ls = 0.0f, os = 0.0f;
-    for (int i = 0; i < splits; i++) {
-        const float* p = po + (int64_t)i * (HD + 2);
-        const float al = p[HD] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[HD] - mx);
-        ls = fmaf(p[HD + 1], al, ls);
-        os = fmaf(p[d], al, os);
+    const float2 ml = tid < splits ? *(const float2*)(po + (int64_t)tid * (HD + 2) + HD) : make_float2(-INFINITY, 0.0f);
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = mx;
+    __syncthreads();
+    mx = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) mx = fmaxf(mx, red[i]);
+    const float wt = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+    if (tid < splits) w[tid] = wt;
+    float ls = wt * ml.y;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o, 64);
+    __syncthreads();
+    if ((tid & 63) == 0) red[tid >> 6] = ls;
+    float os = 0.0f;
+    for (int i = grp; i < splits; i += NG * B) {
+        float v[B];
+#pragma unroll
+        for (int b = 0; b < B; b++) v[b] = i + b * NG < splits ? po[(int64_t)(i + b * NG) * (HD + 2) + d] : 0.0f;
+#pragma unroll
+        for (int b = 0; b < B; b++)
+            if (i + b * NG < splits) os = fmaf(v[b], w[i + b * NG], os);
     }
+    go[grp][d] = os;
+    __syncthreads();
+    if (grp) return;
+    ls = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) ls += red[i];
+#pragma unroll
+    for (int i = 1; i < NG; i++) os += go[i][d];
     a.out[(int64_t)seq * a.ldo + (int64_t)head * HD + d] = ls == 0.0f && mx == -INFINITY ? 0.0f : os / ls;
 }
 
 template <int HD, int KB, int VB> hipError_t attn_launch(const KvAttnArgs& a, int splits, float* ws, hipStream_t s) {
     const int G = a.n_head / a.c.n_kv_head;
     const dim3 grid((unsigned)splits, (unsigned)(a.c.n_kv_head * ((G + 7) / 8)), (unsigned)a.q.n_seq);
-    if (G <= 4) kv_attn_kernel<HD, KB, VB, 1><<<grid, 256, 0, s>>>(a, splits, ws);
-    else kv_attn_kernel<HD, KB, VB, 2><<<grid, 256, 0, s>>>(a, splits, ws);
-    if (splits > 1) kv_join_kernel<<<dim3((unsigned)a.n_head, (unsigned)a.q.n_seq), HD, 0, s>>>(a, splits, ws, HD);
+    if (G <= 4) kv_attn_kernel<HD, KB, VB, 1><<<grid, kv_waves<HD, 1>() * 64, 0, s>>>(a, splits, ws);
+    else kv_attn_kernel<HD, KB, VB, 2><<<grid, kv_waves<HD, 2>() * 64, 0, s>>>(a, splits, ws);
+    if (splits > 1) kv_join_kernel<HD><<<dim3((unsigned)a.n_head, (unsigned)a.q.n_seq), 512, 0, s>>>(a, splits, ws);
     return hipGetLastError();
 }
 
@@ -558,8 +650,10 @@ int kv_attn_splits(const KvAttnArgs& a) {
     int64_t span = std::min<int64_t>(a.q.max_len, (int64_t)a.q.table_len * a.c.page_len);
     if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + kKvTile);
     const int64_t records = (span + kKvTile - 1) / kKvTile;
-    const int64_t want = ((int64_t)cu_count() * 4 + wgs - 1) / wgs;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(want, records / 8));
+    int64_t want = ((int64_t)cu_count() * 2 + wgs - 1) / wgs;
+    if (const char* e = getenv("GGQ_KV_SPLITS"); e && atoi(e) > 0) want = atoi(e);
+    else want = std::min<int64_t>(want, records / 16);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(want, std::min<int64_t>(records, kKvMaxSplits)));
 }
 
 size_t kv_attn_ws_floats(const KvAttnArgs& a, int splits) {
