@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "ggq_attn.h"
+#include "ggq_attn_device.h"
 #include "ggq_launch.h"
 
 namespace ggq {
@@ -244,7 +245,6 @@ __device__ __forceinline__ void dma4(const uint8_t* src, uint32_t lane4, uint32_
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(lane4), "s"(src) : "memory");
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
 // The weight of position `at` of a unit in this lane's column.
 __device__ __forceinline__ float weight_of(const float (&e)[16], int at, int col) {
@@ -395,12 +395,13 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         }
         // to powers of two (an exponent beyond fp32's range gives a score of 0 or an infinite one either way)
         const float cs = ldexpf(1.0f, max(-126, min(127, -(qe + ke))));
-        float top = st[0];
+        float top = max3(st[0], st[1], st[2]);
 #pragma unroll
-        for (int i = 1; i < 16; i++) top = fmaxf(top, st[i]);
-        top = fmaxf(top, other_half(top)) * cs;
+        for (int i = 3; i < 15; i += 2) top = max3(top, st[i], st[i + 1]);
+        const Two th = halves(max3(top, st[15], st[15]));
+        top = max3(th.a, th.b, th.b) * cs;
         if (__any(top > m + 4.0f)) {
-            const float mn = fmaxf(m, top);
+            const float mn = max3(m, top, top);
             const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
             m = mn;
             l *= al;
@@ -487,7 +488,8 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing lands in LDS behind the end)
-    l += other_half(l);
+    const Two lh = halves(l);
+    l = lh.a + lh.b;
     if (!live) return;
     const bool none = end <= beg;
     const float inv = 1.0f / l;

@@ -11,6 +11,7 @@
 #include <cstdlib>
 
 #include "ggq_attn.h"
+#include "ggq_attn_device.h"
 #include "ggq_launch.h"
 
 namespace ggq {
@@ -302,8 +303,8 @@ __device__ __forceinline__ float quad_sum(float v) {
 }
 // Over the four groups of 16 lanes.
 __device__ __forceinline__ float rows_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    const Two x = rows16(v), y = halves(max3(x.a, x.b, x.b));
+    return max3(y.a, y.b, y.b);
 }
 
 // A part of x, its upper 16 bits: three cuts of 8 bits each hold all 24, x0 = x
@@ -470,7 +471,6 @@ __global__ __launch_bounds__((kv_waves<HD, NT>() * 64)) void kv_attn_kernel(KvAt
         float sv[NT][8], top[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            top[n] = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 float v = quad_sum(st[j / 4][n][j % 4]);
@@ -479,15 +479,15 @@ __global__ __launch_bounds__((kv_waves<HD, NT>() * 64)) void kv_attn_kernel(KvAt
                     if (pos < lo || pos >= hi) v = -INFINITY;
                 }
                 sv[n][j] = v;
-                top[n] = fmaxf(top[n], v);
             }
-            top[n] = rows_max(top[n]);
+            const float* x = sv[n];
+            top[n] = rows_max(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7])));
             move |= top[n] > m[n] + 8.0f;
         }
         if (__any(move)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const float mn = fmaxf(m[n], top[n]);
+                const float mn = max3(m[n], top[n], top[n]);
                 const float al = __builtin_amdgcn_exp2f(m[n] - (mn == -INFINITY ? 0.0f : mn));
                 m[n] = mn;
                 l[n] *= al;
@@ -633,6 +633,29 @@ template <int HD> __global__ __launch_bounds__(512) void kv_join_kernel(KvAttnAr
     a.out[(int64_t)seq * a.ldo + (int64_t)head * HD + d] = ls == 0.0f && mx == -INFINITY ? 0.0f : os / ls;
 }
 
+// Workgroups that the chip holds at once.
+template <int HD, int KB, int VB, int NT> int64_t resident() {
+    static const int64_t n = [] {
+        int r = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&r, (const void*)kv_attn_kernel<HD, KB, VB, NT>, kv_waves<HD, NT>() * 64, 0) != hipSuccess || r < 1)
+            r = 1;
+        return (int64_t)r * cu_count();
+    }();
+    return n;
+}
+
+// One round of workgroups at most, four records in a part at least; and only where
+// the rounds of records that it saves a wavefront are worth the join (in us, one sequence,
+// 8 kv heads of 128 in 4 bits: 500 positions 7.5 with one part, 8.1 with 4; 1000: 10.2,
+// 8.3 with 8; 4000: 26.3, 9.0 with 32; 16 sequences of 1000: 10.5, 11.2 with 2).
+template <int HD, int KB, int VB> int attn_splits(const KvAttnArgs& a, int64_t records) {
+    const int G = a.n_head / a.c.n_kv_head, NW = G <= 4 ? kv_waves<HD, 1>() : kv_waves<HD, 2>();
+    const int64_t wgs = (int64_t)a.q.n_seq * a.c.n_kv_head * ((G + 7) / 8);
+    const int64_t fit = G <= 4 ? resident<HD, KB, VB, 1>() : resident<HD, KB, VB, 2>();
+    const int64_t n = std::min<int64_t>(fit / wgs, (records + 3) / 4);
+    return n > 1 && records * (n - 1) > 3 * NW * n ? (int)std::min<int64_t>(n, kKvMaxSplits) : 1;
+}
+
 template <int HD, int KB, int VB> hipError_t attn_launch(const KvAttnArgs& a, int splits, float* ws, hipStream_t s) {
     const int G = a.n_head / a.c.n_kv_head;
     const dim3 grid((unsigned)splits, (unsigned)(a.c.n_kv_head * ((G + 7) / 8)), (unsigned)a.q.n_seq);
@@ -645,15 +668,15 @@ template <int HD, int KB, int VB> hipError_t attn_launch(const KvAttnArgs& a, in
 }  // namespace
 
 int kv_attn_splits(const KvAttnArgs& a) {
-    const int G = a.n_head / a.c.n_kv_head;
-    const int64_t wgs = (int64_t)a.q.n_seq * a.c.n_kv_head * ((G + 7) / 8);
-    int64_t span = std::min<int64_t>(a.q.max_len, (int64_t)a.q.table_len * a.c.page_len);
+    const ggq_kv_cache& c = a.c;
+    int64_t span = std::min<int64_t>(a.q.max_len, (int64_t)a.q.table_len * c.page_len);
     if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + kKvTile);
     const int64_t records = (span + kKvTile - 1) / kKvTile;
-    int64_t want = ((int64_t)cu_count() * 2 + wgs - 1) / wgs;
-    if (const char* e = getenv("GGQ_KV_SPLITS"); e && atoi(e) > 0) want = atoi(e);
-    else want = std::min<int64_t>(want, records / 16);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(want, std::min<int64_t>(records, kKvMaxSplits)));
+    if (const char* e = getenv("GGQ_KV_SPLITS"); e && atoi(e) > 0)
+        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(atoi(e), kKvMaxSplits), records));
+    if (c.head_dim == 64) return GGQ_BY_CACHE(64, attn_splits, a, records);
+    if (c.head_dim == 128) return GGQ_BY_CACHE(128, attn_splits, a, records);
+    return GGQ_BY_CACHE(256, attn_splits, a, records);
 }
 
 size_t kv_attn_ws_floats(const KvAttnArgs& a, int splits) {

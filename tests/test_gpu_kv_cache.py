@@ -322,6 +322,14 @@ def test_attention_is_repeatable_and_splits_do_not_overlap(ctx):
     assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("splits", ["1", "2", "7", "100000"])
+def test_attention_split_counts(ctx, monkeypatch, splits):
+    """Any number of parts (GGQ_KV_SPLITS, read at every call), empty ones among them, gives the same result."""
+    monkeypatch.setenv("GGQ_KV_SPLITS", splits)
+    attend(ctx, 21, [1500, 40, 0, 700], 8, 2, 64, 4, 8, 96)
+    attend(ctx, 22, [900, 33], 12, 2, 128, 8, 4, 64, window=300)
+
+
 def test_no_sequences(ctx):
     pool = Pool(1, 32, 1, 64, 4, 4)
     seqs = gl.KvSeqs(0, 1, 0, None, None)
