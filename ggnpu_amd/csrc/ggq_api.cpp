@@ -1316,6 +1316,8 @@ int ggq_attention_prompt_dev(ggq_ctx* c, const ggq_attention_prompt_params* p, v
         return set_status(c, GGQ_INVALID_PARAM, "row strides must hold a row's heads");
     if (p->n_rows < 0 || p->n_kv_rows < 0 || p->n_seq < 0 || p->window < 0 || !std::isfinite(p->scale))
         return set_status(c, GGQ_INVALID_PARAM, "need n_rows, n_kv_rows, n_seq, window >= 0 and a finite scale");
+    if ((int64_t)p->n_rows * (p->n_head / p->n_kv_head) + 512 > INT32_MAX)
+        return set_status(c, GGQ_INVALID_PARAM, "n_rows * (n_head / n_kv_head) must stay below 2^31");
     if (p->n_rows == 0 || p->n_seq == 0) return set_status(c, GGQ_OK);
     if (!p->q || !p->out || !p->q_off || (p->n_kv_rows && (!p->k || !p->v)))
         return set_status(c, GGQ_INVALID_PARAM, "null q/k/v/out/q_off");

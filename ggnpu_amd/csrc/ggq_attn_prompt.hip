@@ -2,7 +2,7 @@
 //
 // The keys and values a call sees are first written as planes of fp16 operands
 // (planes_kernel): 32 positions of one kv head a unit, fp32 values as hi + lo
-// under a power of two of the unit (22 bits of the unit's largest), in the
+// under a power of two of their position (22 bits of its largest), in the
 // order in which the matrix cores take them, values transposed.  attn_kernel
 // then computes per unit, with v_mfma_f32_32x32x16_f16,
 //   S^T[position][column] = K Q^T,  O^T[value][column] += V^T P^T
@@ -15,11 +15,16 @@
 //   S^T leaves a lane with 16 positions of its column, and P^T wants 8 positions a lane and
 // step of the same column: the values' planes are ordered so that these are the
 // same ones, and weights go from one product to the next in registers.
-//   Units arrive in a ring of LDS slots straight from memory
-// (global_load_lds), a barrier a unit.
+//   Units arrive straight from memory (global_load_lds) in two LDS slots for keys
+// and two for values.  A wavefront's unit has two phases, weights (VALU: maximum,
+// exponentials, split) and products (this unit's O^T, the next one's S^T); the second half of a
+// workgroup's wavefronts, which share the SIMDs with the first, runs a phase behind
+// it, so that one of two is always at the matrix cores while the other is not.
 //   The maximum moves only when a unit exceeds it by 2^4; weights are kept times
 // 2^11 (at most 2^15), so hi + lo of a small weight keeps 2^-35 of the largest.
-// The running sums are in units of the values' power of two and follow it.
+// Scores take their position's power of two back; weights take the values', relative to
+// the largest that their row has seen, whose unit the row's running sums are in: a
+// position that a row does not see has no say in what the row keeps of the others.
 // Bound: the matrix cores.
 #include <algorithm>
 
@@ -97,12 +102,22 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int kUnit = 32;  // positions
-// Bytes of a unit: 64 dwords of header, K and V planes.
-constexpr int64_t unit_bytes(int hd, int planes) { return (int64_t)planes * 2 * kUnit * hd * 2 + 256; }
-// Header: exponents of K and V (+ 512), and whether there are values that are not
-// finite, positions whose largest value is more than 2^16 below the unit's (what
-// hi + lo keep of them is less than fp32), any values but zero.
-enum { BAD_K = 1 << 20, BAD_V = 1 << 21, WIDE_K = 1 << 22, WIDE_V = 1 << 23, NO_V = 1 << 24 };
+// Header of a unit: for each position how many powers of two its K and V planes
+// are scaled beyond those of the unit's largest values, as negative numbers
+// (32 of K, 32 of V; 16 bits each where 32 would bring the LDS of a workgroup to 128 KB), then
+// dwords, all alike: those ones' exponents (+ 512), whether some values are not
+// finite (zero in the planes), whether there are any but zero.
+template <int HD> struct Head {
+    typedef int num;
+    static constexpr int bytes = 512, info = 256;
+};
+template <> struct Head<256> {
+    typedef int16_t num;
+    static constexpr int bytes = 256, info = 128;
+};
+// Bytes of a unit: header, K and V planes.
+template <int HD> constexpr int64_t unit_bytes(int planes) { return (int64_t)planes * 2 * kUnit * HD * 2 + Head<HD>::bytes; }
+enum { BAD_V = 1 << 20, NO_V = 1 << 21 };
 
 // Sequence s has the units from off[s] / 32 + s on (and as many column tiles of
 // n from off[s] * G / n + s): a bound that needs no sum over the sequences before.
@@ -139,7 +154,7 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1, V = HD / 8;  // planes, values of a thread
     constexpr int PL = kUnit * HD;                         // values of a plane
     __shared__ float sv[kUnit][HD + 1];
-    __shared__ uint32_t red[4][5];
+    __shared__ uint32_t red[4][3];
     const int tid = threadIdx.x, kvh = blockIdx.y;
     const int32_t* off = kv_off_of(a.p);
     const int64_t id = blockIdx.x;
@@ -153,55 +168,62 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
     if (u < 0 || u * kUnit >= sp.n) return;
     const int pos = tid / 8, d0 = tid % 8 * V;
     const bool in = u * kUnit + pos < sp.n;
-    const int64_t row = sp.a + u * kUnit + pos;
+    const int64_t row = sp.a + min(u * kUnit + pos, sp.n - 1);
+    struct alignas(16) Run { T x[16 / sizeof(T)]; };
+    constexpr int PR = 16 / sizeof(T), NR = V / PR;
+    const Run* kr = (const Run*)((const T*)a.p.k + row * a.p.ldk + (int64_t)kvh * HD + d0);
+    const Run* vr = (const Run*)((const T*)a.p.v + row * a.p.ldv + (int64_t)kvh * HD + d0);
+    Run kin[NR], vin[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) { kin[i] = kr[i]; vin[i] = vr[i]; }
     float k[V], v[V];
     uint32_t mk = 0, mv = 0, bad = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        k[i] = in ? (float)((const T*)a.p.k)[row * a.p.ldk + (int64_t)kvh * HD + d0 + i] : 0.0f;
-        v[i] = in ? (float)((const T*)a.p.v)[row * a.p.ldv + (int64_t)kvh * HD + d0 + i] : 0.0f;
+        k[i] = in ? (float)kin[i / PR].x[i % PR] : 0.0f;
+        v[i] = in ? (float)vin[i / PR].x[i % PR] : 0.0f;
         mk = max(mk, mag_bits(k[i]));
         mv = max(mv, mag_bits(v[i]));
-        if (!finite(k[i])) bad |= BAD_K;
         if (!finite(v[i])) {
             bad |= BAD_V;
             v[i] = 0.0f;
         }
     }
-    // the unit's largest, and the least of its positions' largest (but zero): 8 threads a position first
-    auto least = [](uint32_t x, uint32_t y) { return x && (!y || x < y) ? x : y; };
-    uint32_t nk = 0, nv = 0;
+    // the positions' largest (8 threads each), the unit's
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        if (o == 8) {
-            nk = mk;
-            nv = mv;
-        }
+    for (int o = 1; o < 8; o <<= 1) {
         mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
         mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
-        bad |= (uint32_t)__shfl_xor((int)bad, o, 64);
+    }
+    uint32_t uk = mk, uv = mv;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
         if (o >= 8) {
-            nk = least(nk, (uint32_t)__shfl_xor((int)nk, o, 64));
-            nv = least(nv, (uint32_t)__shfl_xor((int)nv, o, 64));
+            uk = max(uk, (uint32_t)__shfl_xor((int)uk, o, 64));
+            uv = max(uv, (uint32_t)__shfl_xor((int)uv, o, 64));
         }
+        bad |= (uint32_t)__shfl_xor((int)bad, o, 64);
     }
     if ((tid & 63) == 0) {
         uint32_t* r = red[tid >> 6];
-        r[0] = mk; r[1] = mv; r[2] = bad; r[3] = nk; r[4] = nv;
+        r[0] = uk; r[1] = uv; r[2] = bad;
     }
     __syncthreads();
-    mk = max(max(red[0][0], red[1][0]), max(red[2][0], red[3][0]));
-    mv = max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1]));
+    uk = max(max(red[0][0], red[1][0]), max(red[2][0], red[3][0]));
+    uv = max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1]));
     bad = red[0][2] | red[1][2] | red[2][2] | red[3][2];
-    nk = least(least(red[0][3], red[1][3]), least(red[2][3], red[3][3]));
-    nv = least(least(red[0][4], red[1][4]), least(red[2][4], red[3][4]));
-    if (P == 2 && (mk >> 23) - (nk >> 23) > 16) bad |= WIDE_K;
-    if (P == 2 && (mv >> 23) - (nv >> 23) > 16) bad |= WIDE_V;
     // fp16 values stay as they are
-    const int ke = P == 2 ? up_to_2_15(mk) : 0, ve = P == 2 ? up_to_2_15(mv) : 0;
-    uint8_t* out = a.planes + (id * a.p.n_kv_head + kvh) * unit_bytes(HD, P);
-    if (tid < 64) ((uint32_t*)out)[tid] = (uint32_t)(ke + 512) | (uint32_t)(ve + 512) << 10 | bad | (mv ? 0 : NO_V);
-    _Float16* kp = (_Float16*)(out + 256);
+    const int ku = P == 2 ? up_to_2_15(uk) : 0, vu = P == 2 ? up_to_2_15(uv) : 0;
+    const int ke = P == 2 && mk ? up_to_2_15(mk) : ku, ve = P == 2 && mv ? up_to_2_15(mv) : vu;
+    typedef typename Head<HD>::num num;
+    uint8_t* out = a.planes + (id * a.p.n_kv_head + kvh) * unit_bytes<HD>(P);
+    if (tid % 8 == 0) {
+        ((num*)out)[pos] = (num)(ku - ke);
+        ((num*)out)[32 + pos] = (num)(vu - ve);
+    }
+    if (tid < (Head<HD>::bytes - Head<HD>::info) / 4)
+        ((uint32_t*)(out + Head<HD>::info))[tid] = (uint32_t)(ku + 512) | (uint32_t)(vu + 512) << 10 | bad | (uv ? 0 : NO_V);
+    _Float16* kp = (_Float16*)(out + Head<HD>::bytes);
 #pragma unroll
     for (int i = 0; i < V; i += 8) {
         h8 hi, lo;
@@ -209,7 +231,7 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
         for (int j = 0; j < 8; j++) {
             const float x = P == 2 ? ldexpf(k[i + j], ke) : k[i + j];
             hi[j] = (_Float16)x;
-            lo[j] = finite(x) ? (_Float16)(x - (float)hi[j]) : (_Float16)0.0f;
+            lo[j] = (_Float16)(x - (float)hi[j]);  // (NaN for an infinity)
         }
         const int d = d0 + i;
         _Float16* at = kp + ((d / 16) * 64 + (d / 8 % 2) * 32 + pos) * 8;
@@ -246,124 +268,154 @@ __device__ __forceinline__ void dma4(const uint8_t* src, uint32_t lane4, uint32_
 }
 
 
-// The weight of position `at` of a unit in this lane's column.
-__device__ __forceinline__ float weight_of(const float (&e)[16], int at, int col) {
-    float w = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; i++)
-        if (8 * (i / 4) + i % 4 == (at & ~4)) w = e[i];
-    return __shfl(w, col + 32 * ((at >> 2) & 1), 64);
+// fp16 parts j and j + 1 of a pair of values.
+__device__ __forceinline__ void split_pair(float a, float b, h8& hi, h8& lo, int j) {
+    const h2 p = {(_Float16)a, (_Float16)b};
+    hi[j] = p[0];
+    hi[j + 1] = p[1];
+    lo[j] = (_Float16)fmaf((float)p[0], -1.0f, a);
+    lo[j + 1] = (_Float16)fmaf((float)p[1], -1.0f, b);
 }
 
-// Wavefronts and LDS slots of a workgroup, at most 128 KB for what global_load_lds addresses:
-// three units of 128-wide fp32 heads.  256-wide heads need twice the registers.
+// Wavefronts of a workgroup: two a SIMD, or one of 256-wide heads, whose sums and
+// queries take more than half of the registers.
 template <int HD> constexpr int waves_of() { return HD == 256 ? 4 : 8; }
-template <int HD, int P> constexpr int slots_of() { return HD * P >= 512 ? 2 : HD * P == 256 ? 3 : 4; }
+
+// All of this wavefront's reads of LDS are done, and with `loads` its loads into it; then
+// the workgroup's.
+__device__ __forceinline__ void phase_end(bool loads) {
+    if (loads) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
 template <int HD, typename T>
 __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a) {
-    constexpr int P = sizeof(T) == 4 ? 2 : 1, NW = waves_of<HD>(), S = slots_of<HD, P>();
-    constexpr int UB = (int)unit_bytes(HD, P), PL = kUnit * HD * 2;  // bytes of a unit, of a plane
-    constexpr int LD = (UB - 256) / 1024 / NW;                       // loads of a wavefront a unit, and the header
+    constexpr int P = sizeof(T) == 4 ? 2 : 1, NW = waves_of<HD>(), PL = kUnit * HD * 2;  // PL: bytes of a plane
+    constexpr int64_t UB = unit_bytes<HD>(P);
+    typedef typename Head<HD>::num num;
+    constexpr int HB = Head<HD>::bytes, KB = HB + P * PL, VB = P * PL;          // LDS bytes of a unit's header and keys, of its values
+    constexpr int KC = P * PL / 1024, LD = 2 * KC / NW;      // 1 KB loads of the keys; of a wavefront a unit (and the header)
     constexpr int KS = HD / 16, DB = HD / 32;
-    static_assert((UB - 256) % (1024 * NW) == 0 && (S - 1) * UB + UB - 1024 < 128 * 1024, "ring");
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[S * UB];
+    static_assert(2 * KC % NW == 0 && 2 * (KB + VB) - 1024 < 128 * 1024, "LDS that global_load_lds addresses");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * (KB + VB)];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, h = lane >> 5;
+    const bool behind = NW == 8 && wave >= 4;  // runs a phase behind the others
     const ggq_attention_prompt_params& p = a.p;
-    const int kvh = blockIdx.x % p.n_kv_head, split = blockIdx.y;
-    const int64_t id = a.tiles - 1 - blockIdx.x / p.n_kv_head;  // late rows see most: first
+    const int kvh = blockIdx.x % p.n_kv_head, split = blockIdx.y, G = a.G;
+    const int id = a.tiles - 1 - (int)(blockIdx.x / p.n_kv_head);  // late rows see most: first
     constexpr int NC = NW * 32;
     int seq = 0;
     for (int i = 1; i < p.n_seq; i += NW * 64) {
         const int j = i + tid;
-        seq += __syncthreads_count(j < p.n_seq && bound_of(max((int64_t)p.q_off[j], (int64_t)0) * a.G, NC, j) <= id);
+        seq += __syncthreads_count(j < p.n_seq && (int)((uint32_t)max(min(p.q_off[j], p.n_rows), 0) * G / NC) + j <= id);
     }
     const Span qs = span_of(p.q_off, seq, p.n_rows), ks = span_of(kv_off_of(p), seq, p.n_kv_rows);
-    const int64_t f0 = (id - bound_of(qs.a * a.G, NC, seq)) * NC, nf = qs.n * a.G;
+    // (n_rows * G fits 31 bits: the caller sees to it)
+    const int nf = (int)qs.n * G, f0 = (id - ((int)((uint32_t)qs.a * G / NC) + seq)) * NC;
     if (f0 < 0 || f0 >= nf) return;
-    const int64_t shift = ks.n - qs.n + 1;  // row i sees positions below shift + i
-    const int64_t i0 = f0 / a.G, i1 = (min(nf, f0 + NC) - 1) / a.G;
-    const int64_t wg_end = min(max(shift + i1, (int64_t)0), ks.n);
-    const int64_t wg_beg = p.window ? max(shift + i0 - p.window, (int64_t)0) : 0;
-    const int all0 = (int)(wg_beg / kUnit), all1 = (int)((wg_end + kUnit - 1) / kUnit);
+    const int n_keys = (int)ks.n, shift = n_keys - (int)qs.n + 1;  // row i sees positions below shift + i
+    const int i0 = (int)((uint32_t)f0 / G), i1 = (int)((uint32_t)(min(nf, f0 + NC) - 1) / G);
+    const int wg_end = min(max(shift + i1, 0), n_keys);
+    const int wg_beg = p.window ? max(shift + i0 - p.window, 0) : 0;
+    const int all0 = wg_beg / kUnit, all1 = (wg_end + kUnit - 1) / kUnit;
     const int per = (max(all1 - all0, 0) + a.splits - 1) / a.splits;
-    const int u0 = all0 + split * per, u1 = min(all1, u0 + per);
+    const int u0 = all0 + split * per, u1 = min(all1, u0 + per), n = u1 - u0;
+
+    // loads for iteration it: the keys of its next but one unit, the values of its next
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const uint8_t* units = a.planes + ((bound_of(ks.a, kUnit, seq) + u0) * p.n_kv_head + kvh) * UB;
+    auto fetch = [&](int it) {  // (outside of what there is, the nearest unit: the same number of loads each time)
+        const uint8_t* ksrc = units + (int64_t)min(it + 2, n - 1) * p.n_kv_head * UB;
+        const uint8_t* vsrc = units + (int64_t)max(min(it + 1, n - 1), 0) * p.n_kv_head * UB + KB;
+        const uint32_t kdst = lds_at + (it & 1) * KB, vdst = lds_at + 2 * KB + ((it + 1) & 1) * VB;
+        dma4(ksrc, (uint32_t)lane * 4u, kdst);
+        if constexpr (HB == 512) dma4(ksrc + 256, (uint32_t)lane * 4u, kdst + 256u);
+#pragma unroll
+        for (int j = 0; j < LD; j++) {
+            const int c = wave * LD + j;
+            if (c < KC) dma16(ksrc + HB + c * 1024, (uint32_t)lane * 16u, kdst + (uint32_t)(HB + c * 1024));
+            else dma16(vsrc + (c - KC) * 1024, (uint32_t)lane * 16u, vdst + (uint32_t)(c - KC) * 1024u);
+        }
+    };
+    if (n > 0) {
+        fetch(-2);
+        fetch(-1);
+    }
 
     // this lane's column
-    const int64_t f = f0 + wave * 32 + col;
+    const int f = f0 + wave * 32 + col;
     const bool live = f < nf;
-    const int64_t qi = live ? f / a.G : i1;
-    const int head = kvh * a.G + (live ? (int)(f % a.G) : 0);
-    const int end = live ? (int)min(max(shift + qi, (int64_t)0), ks.n) : 0;
-    const int beg = live && p.window ? (int)max(shift + qi - p.window, (int64_t)0) : 0;
-    int wend = end, wbeg = live ? beg : INT32_MAX, fend = live ? end : INT32_MAX, fbeg = beg;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        wend = max(wend, __shfl_xor(wend, o, 64));
-        wbeg = min(wbeg, __shfl_xor(wbeg, o, 64));
-        fend = min(fend, __shfl_xor(fend, o, 64));
-        fbeg = max(fbeg, __shfl_xor(fbeg, o, 64));
-    }
-    wend = __builtin_amdgcn_readfirstlane(wend);
-    wbeg = __builtin_amdgcn_readfirstlane(wbeg);
-    fend = __builtin_amdgcn_readfirstlane(fend);
-    fbeg = __builtin_amdgcn_readfirstlane(fbeg);
+    const int qi = live ? (int)((uint32_t)f / G) : i1;
+    const int head = kvh * G + (live ? f - qi * G : 0);
+    const int end = live ? min(max(shift + qi, 0), n_keys) : 0;
+    const int beg = live && p.window ? max(shift + qi - p.window, 0) : 0;
+    // rows ascend with the columns: the first and the last live one bound what the wavefront sees
+    const int fl = f0 + wave * 32, last = min(fl + 31, nf - 1);
+    const bool any = fl < nf, full = fl + 31 < nf;
+    const int ra = any ? (int)((uint32_t)fl / G) : 0, rb = any ? (int)((uint32_t)last / G) : 0;
+    const int wend = any ? min(max(shift + rb, 0), n_keys) : 0, wbeg = p.window ? max(shift + ra - p.window, 0) : 0;
+    const int fend = full ? min(max(shift + ra, 0), n_keys) : 0;  // (with columns that are no rows: masked throughout)
+    const int fbeg = p.window ? max(shift + rb - p.window, 0) : 0;
 
     const float* qrow = p.q + (qs.a + qi) * p.ldq + (int64_t)head * HD;
     h8 qh[KS], ql[KS];
     int qe;
     {
+        float4 x[2 * KS];
         uint32_t m = 0;
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int s = 0; s < 2 * KS; s++) x[s] = *(const float4*)(qrow + 16 * (s / 2) + 8 * h + 4 * (s % 2));
 #pragma unroll
-            for (int j = 0; j < 8; j++) m = max(m, mag_bits(qrow[16 * s + 8 * h + j] * p.scale));
+        for (int s = 0; s < 2 * KS; s++) {
+            x[s] = make_float4(x[s].x * p.scale, x[s].y * p.scale, x[s].z * p.scale, x[s].w * p.scale);
+            m = max(max(max(m, mag_bits(x[s].x)), mag_bits(x[s].y)), max(mag_bits(x[s].z), mag_bits(x[s].w)));
+        }
         m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
         qe = up_to_2_15(m);
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int s = 0; s < KS; s++) {
+            const float v[8] = {x[2 * s].x, x[2 * s].y, x[2 * s].z, x[2 * s].w, x[2 * s + 1].x, x[2 * s + 1].y, x[2 * s + 1].z, x[2 * s + 1].w};
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float x = live ? ldexpf(qrow[16 * s + 8 * h + j] * p.scale, qe) : 0.0f;
-                qh[s][j] = (_Float16)x;
-                ql[s][j] = finite(x) ? (_Float16)(x - (float)qh[s][j]) : (_Float16)0.0f;
-            }
+            for (int j = 0; j < 8; j += 2)  // (NaN for an infinity, and so is its row)
+                split_pair(ldexpf(v[j], qe), ldexpf(v[j + 1], qe), qh[s], ql[s], j);
+        }
     }
 
-    const uint32_t ring_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
-    const uint8_t* units = a.planes + (bound_of(ks.a, kUnit, seq) * p.n_kv_head + kvh) * UB;
-    auto fetch = [&](int i) {  // unit u0 + i (past the end the last one: every unit the same number of loads)
-        const int u = min(u0 + i, u1 - 1), slot = i % S * UB;
-        const uint8_t* src = units + (int64_t)u * p.n_kv_head * UB;
-#pragma unroll
-        for (int j = 0; j < LD; j++)
-            dma16(src + 256 + (wave * LD + j) * 1024, (uint32_t)lane * 16u, ring_at + (uint32_t)(slot + 256 + (wave * LD + j) * 1024));
-        dma4(src, (uint32_t)lane * 4u, ring_at + (uint32_t)slot);
-    };
-
-    f16v o[DB];
+    f16v o[DB], st;
 #pragma unroll
     for (int d = 0; d < DB; d++) o[d] = f16v{};
     float m = -INFINITY, l = 0.0f;
-    int ve = 0, least = 1 << 20;  // exponent of the sums' unit; the least one of the values so far
-    bool first = true;
-    const int n = u1 - u0;
-    if (n > 0) {
-#pragma unroll
-        for (int i = 0; i < S - 1; i++) fetch(i);
-    }
-    for (int it = 0; it < n; it++) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * (LD + 1)) : "memory");
-        fetch(it + S - 1);
+    // the column's sums are in units of 2^-ve; the least exponent of the values it saw
+    constexpr int kNone = 1 << 20;
+    int ve = 0, least = kNone;
+    uint32_t info = 0, bad = 0;
+    int dk[16];
+    auto skips = [&](int it) {  // none of the wavefront's columns sees anything of the unit
         const int base = (u0 + it) * kUnit;
-        if (base >= wend || base + kUnit <= wbeg) continue;
-        const uint8_t* slot = ring + it % S * UB;
-        const uint32_t info = __builtin_amdgcn_readfirstlane(*(const uint32_t*)slot);
-        const int ke = (int)(info & 1023u) - 512, ve_u = (int)(info >> 10 & 1023u) - 512;
-        const h8* kp = (const h8*)(slot + 256) + lane;
-        const bool masked = base + kUnit > fend || base < fbeg;  // for a column of this wavefront
-        f16v st = {};
+        return base >= wend || base + kUnit <= wbeg;
+    };
+    auto masks = [&](int it) {  // one of them does not see all of it
+        const int base = (u0 + it) * kUnit;
+        return base + kUnit > fend || base < fbeg;
+    };
+    // this lane's 16 of a header's 32 numbers
+    auto numbers = [&](const uint8_t* from, int (&x)[16]) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            struct alignas(4 * sizeof(num)) Four { num x[4]; };
+            const Four v = *(const Four*)(from + sizeof(num) * (2 * i + 4 * h));
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[i + j] = v.x[j];
+        }
+    };
+    int dv[P == 2 ? 16 : 1];
+    auto scores = [&](int it) {
+        const uint8_t* slot = lds + (it & 1) * KB;
+        info = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(slot + Head<HD>::info));
+        if (skips(it)) return;
+        const h8* kp = (const h8*)(slot + HB) + lane;
+        st = f16v{};
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const h8 kh = kp[s * 64];
@@ -371,30 +423,36 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[s], st, 0, 0, 0);
             if constexpr (P == 2) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kp[s * 64 + PL / 16], qh[s], st, 0, 0, 0);
         }
-        if (info & BAD_K || (masked && info & WIDE_K)) {
-            // keys that are not finite, or hidden ones that leave the others few bits: the products as they are
-            const T* kr = (const T*)p.k + (ks.a + base) * p.ldk + (int64_t)kvh * HD;
-#pragma unroll 1
-            for (int i = 0; i < 16; i++) {
-                const int at = 8 * (i / 4) + 4 * h + i % 4;
-                if (base + at >= ks.n) continue;
-                float s = 0.0f;
-#pragma unroll 1
-                for (int d = 0; d < HD; d++) s = fmaf(qrow[d] * p.scale, (float)kr[at * p.ldk + d], s);
-                s = ldexpf(s, qe + ke);
-#pragma unroll
-                for (int j = 0; j < 16; j++) st[j] = j == i ? s : st[j];
-            }
+        // (the slot is loaded over before the weights of the wavefronts behind)
+        if constexpr (P == 2) {
+            numbers(slot, dk);
+            numbers(slot + 32 * sizeof(num), dv);
         }
+    };
+    h8 ph[2], pl[2];
+    auto weights = [&](int it) {
+        const int base = (u0 + it) * kUnit;
+        const bool masked = masks(it);
+        const int ku = (int)(info & 1023u) - 512, vu = (int)(info >> 10 & 1023u) - 512;
+        bad |= info;
+        if constexpr (P == 2) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) st[i] = ldexpf(st[i], dk[i]);
+        }
+        int vmin = vu;  // of the values that the column sees
         if (masked) {
+            int most = -kNone;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int at = base + 8 * (i / 4) + 4 * h + i % 4;
-                if (at >= end || at < beg) st[i] = -INFINITY;
+                const bool out = at >= end || at < beg;
+                if (out) st[i] = -INFINITY;
+                if constexpr (P == 2) most = max(most, out ? -kNone : dv[i]);
             }
+            if constexpr (P == 2) vmin = vu - max(most, __shfl_xor(most, 32, 64));
         }
         // to powers of two (an exponent beyond fp32's range gives a score of 0 or an infinite one either way)
-        const float cs = ldexpf(1.0f, max(-126, min(127, -(qe + ke))));
+        const float cs = ldexpf(1.0f, max(-126, min(127, -(qe + ku))));
         float top = max3(st[0], st[1], st[2]);
 #pragma unroll
         for (int i = 3; i < 15; i += 2) top = max3(top, st[i], st[i + 1]);
@@ -408,109 +466,95 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
 #pragma unroll
             for (int d = 0; d < DB; d++) o[d] *= al;
         }
-        float pscale = 1.0f;
         if constexpr (P == 2) {
-            if (!(info & NO_V)) {
-                // the sums follow the values' unit when those get larger, or smaller by more than
-                // 2^8 (but stay within 2^64 of the largest so far); less than that, weights shrink
-                least = min(least, ve_u);
-                const int to = first || ve_u < ve || ve_u > ve + 8 ? min(ve_u, least + 64) : ve;
-                first = false;
-                if (to != ve) {
-#pragma unroll
-                    for (int d = 0; d < DB; d++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[d][i] = ldexpf(o[d][i], to - ve);
-                    ve = to;
-                }
-                if (to != ve_u) pscale = ldexpf(1.0f, max(-126, to - ve_u));
-            }
-        }
-        const float ref = m == -INFINITY ? 0.0f : m - 11.0f;
-        float e[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            e[i] = __builtin_amdgcn_exp2f(fmaf(st[i], cs, -ref));
-            l += e[i];
-        }
-        if (P == 2 && pscale != 1.0f) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) e[i] *= pscale;
-        }
-        const h8* vp = kp + P * PL / 16;
-        if (P == 2 && masked && info & WIDE_V) {
-            // hidden values that leave the others few bits: the products as they are
-            const T* vr = (const T*)p.v + (ks.a + base) * p.ldv + (int64_t)kvh * HD;
-            const float un = 1.0f / pscale;
-#pragma unroll 1
-            for (int at = 0; at < kUnit; at++) {
-                const float w = weight_of(e, at, col) * un;
-                if (base + at >= end || base + at < beg) continue;
+            // the sums follow the values' unit when those get larger, or smaller by more than
+            // 2^8 (but stay within 2^64 of the largest so far); less than that, weights shrink
+            const bool some = !(info & NO_V) && vmin < kNone / 2;
+            const bool first = least == kNone;
+            least = some ? min(least, vmin) : least;
+            const int to = some && (first || vmin < ve || vmin > ve + 8) ? min(vmin, least + 64) : ve;
+            if (__any(to != ve)) {
 #pragma unroll
                 for (int d = 0; d < DB; d++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        o[d][i] = fmaf(w, ldexpf((float)vr[at * p.ldv + 32 * d + 8 * (i / 4) + 4 * h + i % 4], ve), o[d][i]);
+                    for (int i = 0; i < 16; i++) o[d][i] = ldexpf(o[d][i], to - ve);
+                ve = to;
             }
-            continue;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m - 11.0f;
+        float e[16], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            e[i] = __builtin_amdgcn_exp2f(fmaf(st[i], cs, -ref));
+            sum[i & 1] += e[i];
+        }
+        l += sum[0] + sum[1];
+        if constexpr (P == 2) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) e[i] = ldexpf(e[i], dv[i] + (ve - vu));
         }
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            h8 ph, pl;
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                ph[j] = (_Float16)e[8 * t + j];
-                pl[j] = (_Float16)(e[8 * t + j] - (float)ph[j]);
-            }
+            for (int j = 0; j < 8; j += 2) split_pair(e[8 * t + j], e[8 * t + j + 1], ph[t], pl[t], j);
+    };
+    auto sums = [&](int it) {
+        const h8* vp = (const h8*)(lds + 2 * KB + (it & 1) * VB) + lane;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int d = 0; d < DB; d++) {
                 const h8 vh = vp[(2 * d + t) * 64];
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[d], 0, 0, 0);
-                if constexpr (P == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vp[(2 * d + t) * 64 + PL / 16], ph, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[t], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[t], o[d], 0, 0, 0);
+                if constexpr (P == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vp[(2 * d + t) * 64 + PL / 16], ph[t], o[d], 0, 0, 0);
             }
+    };
+    // Phases of the workgroup, by number: the wavefronts in front have weights(i) in 2 i and
+    // products(i) in 2 i + 1, those behind one later.  In 2 i + 1 nobody uses the keys of unit i or
+    // the values of unit i - 1 any more, and everybody loads over them; what was loaded is waited for at the end
+    // of 2 i + 2, before the first wavefronts need it.
+    if (n > 0) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LD + HB / 256) : "memory");
+        scores(0);
+        if (behind) phase_end(true);
+        for (int it = 0; it < n; it++) {
+            if (behind) fetch(it);
+            const bool on = !skips(it);
+            if (on) weights(it);
+            phase_end(!behind);
+            if (!behind) fetch(it);
+            if (on) sums(it);
+            if (it + 1 < n) scores(it + 1);
+            phase_end(behind);
         }
-        if (info & BAD_V) {
-            // values that are not finite are zero in the planes: here they come, to the rows that see them
-            const T* vr = (const T*)p.v + (ks.a + base) * p.ldv + (int64_t)kvh * HD;
-#pragma unroll 1
-            for (int at = 0; at < kUnit; at++) {
-                const float w = weight_of(e, at, col);
-                if (base + at >= end || base + at < beg) continue;
+        if (!behind) phase_end(true);
+    }
+    const Two lh = halves(l);
+    l = lh.a + lh.b;
+    if (!live) return;
+    if (bad & BAD_V) {
+        // infinities and NaN among the values are zero in the planes: here they come, to the rows that see them
+        for (int u = u0; u < u1; u++) {
+            if (!(*(const uint32_t*)(units + (int64_t)(u - u0) * p.n_kv_head * UB + Head<HD>::info) & BAD_V)) continue;
+            for (int at = max(u * kUnit, beg); at < min((u + 1) * kUnit, end); at++) {
+                const T* vr = (const T*)p.v + (ks.a + at) * p.ldv + (int64_t)kvh * HD + 4 * h;
 #pragma unroll
                 for (int d = 0; d < DB; d++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float v = (float)vr[at * p.ldv + 32 * d + 8 * (i / 4) + 4 * h + i % 4];
-                        if (!finite(v)) o[d][i] += w * v;
+                        const float v = (float)vr[32 * d + 8 * (i / 4) + i % 4];
+                        if (!finite(v)) o[d][i] += v;
                     }
             }
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing lands in LDS behind the end)
-    const Two lh = halves(l);
-    l = lh.a + lh.b;
-    if (!live) return;
-    const bool none = end <= beg;
     const float inv = 1.0f / l;
-    if (a.splits == 1) {
-        float* out = p.out + (qs.a + qi) * p.ldo + (int64_t)head * HD + 4 * h;
-#pragma unroll
-        for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                float4 r;
-                r.x = none ? 0.0f : ldexpf(o[d][i] * inv, -ve);
-                r.y = none ? 0.0f : ldexpf(o[d][i + 1] * inv, -ve);
-                r.z = none ? 0.0f : ldexpf(o[d][i + 2] * inv, -ve);
-                r.w = none ? 0.0f : ldexpf(o[d][i + 3] * inv, -ve);
-                *(float4*)(out + 32 * d + 2 * i) = r;
-            }
-        return;
-    }
-    // this part's weighted mean, its maximum and its sum
+    const bool none = end <= beg;
     float* part = a.part + (((qs.a + qi) * p.n_head + head) * a.splits + split) * (HD + 4);
-    const bool empty = m == -INFINITY && l == 0.0f;
+    const bool whole = a.splits == 1, empty = whole ? none : m == -INFINITY && l == 0.0f;
+    // the row's result, or this part's weighted mean with its maximum and its sum
+    float* out = (whole ? p.out + (qs.a + qi) * p.ldo + (int64_t)head * HD : part) + 4 * h;
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -520,30 +564,38 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             r.y = empty ? 0.0f : ldexpf(o[d][i + 1] * inv, -ve);
             r.z = empty ? 0.0f : ldexpf(o[d][i + 2] * inv, -ve);
             r.w = empty ? 0.0f : ldexpf(o[d][i + 3] * inv, -ve);
-            *(float4*)(part + 32 * d + 2 * i + 4 * h) = r;
+            *(float4*)(out + 32 * d + 2 * i) = r;
         }
-    if (h == 0) { part[HD] = m; part[HD + 1] = l; }
+    if (!whole && h == 0) { part[HD] = m; part[HD + 1] = l; }
 }
 
-// The parts of one row's head, in their order.
+// The parts of one row's head, in their order: a wavefront each, HD / 64 values a lane.
 template <int HD> __global__ __launch_bounds__(256) void attn_join_kernel(PromptArgs a) {
+    constexpr int DPL = HD / 64;
     const ggq_attention_prompt_params& p = a.p;
-    const int row = blockIdx.x, d = threadIdx.x;
-    const int seq = seq_of(p.q_off, p.n_seq, row);
-    if (seq >= p.n_seq || row < p.q_off[seq] || d >= HD) return;
-    for (int head = blockIdx.y; head < p.n_head; head += gridDim.y) {
-        const float* q = a.part + ((int64_t)row * p.n_head + head) * a.splits * (HD + 4);
-        float mx = -INFINITY;
-        for (int i = 0; i < a.splits; i++) mx = fmaxf(mx, q[(int64_t)i * (HD + 4) + HD]);
-        float ls = 0.0f, os = 0.0f;
-        for (int i = 0; i < a.splits; i++) {
-            const float* x = q + (int64_t)i * (HD + 4);
-            const float w = x[HD] == -INFINITY && x[HD + 1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[HD] - mx) * x[HD + 1];
-            ls += w;
-            os = fmaf(x[d], w, os);
-        }
-        p.out[(int64_t)row * p.ldo + (int64_t)head * HD + d] = mx == -INFINITY && ls == 0.0f ? 0.0f : os / ls;
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = (int)(w / p.n_head), head = (int)(w % p.n_head), lane = threadIdx.x & 63;
+    if (row >= p.n_rows) return;
+    bool in = false;  // a row of some sequence
+    for (int i = 0; i < p.n_seq && !in; i += 64) {
+        const int j = i + lane;
+        in = __any(j < p.n_seq && p.q_off[j] <= row && row < p.q_off[j + 1]);
     }
+    if (!in) return;
+    const float* q = a.part + w * a.splits * (HD + 4);
+    float mx = -INFINITY;
+    for (int i = 0; i < a.splits; i++) mx = fmaxf(mx, q[(int64_t)i * (HD + 4) + HD]);
+    float ls = 0.0f, os[DPL] = {};
+    for (int i = 0; i < a.splits; i++) {
+        const float* x = q + (int64_t)i * (HD + 4);
+        const float wt = x[HD] == -INFINITY && x[HD + 1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[HD] - mx) * x[HD + 1];
+        ls += wt;
+#pragma unroll
+        for (int d = 0; d < DPL; d++) os[d] = fmaf(x[lane + 64 * d], wt, os[d]);
+    }
+    float* out = p.out + (int64_t)row * p.ldo + (int64_t)head * HD + lane;
+#pragma unroll
+    for (int d = 0; d < DPL; d++) out[64 * d] = mx == -INFINITY && ls == 0.0f ? 0.0f : os[d] / ls;
 }
 
 }  // namespace
@@ -555,16 +607,19 @@ int64_t tiles_of(const ggq_attention_prompt_params& p) {
     return (int64_t)p.n_rows * (p.n_head / p.n_kv_head) / nc + p.n_seq;
 }
 size_t planes_bytes(const ggq_attention_prompt_params& p) {
-    return (size_t)(units_of(p) * p.n_kv_head * unit_bytes(p.head_dim, p.type == GGQ_TYPE_F32 ? 2 : 1));
+    const int planes = p.type == GGQ_TYPE_F32 ? 2 : 1;
+    return (size_t)(units_of(p) * p.n_kv_head) *
+           (p.head_dim == 64 ? unit_bytes<64>(planes) : p.head_dim == 128 ? unit_bytes<128>(planes) : unit_bytes<256>(planes));
 }
 }  // namespace
 
 AttnPromptPlan attn_prompt_plan(const ggq_attention_prompt_params& p) {
     AttnPromptPlan pl{};
-    // few tiles: the positions in parts, while each keeps 8 units
-    const int64_t wgs = tiles_of(p) * p.n_kv_head, units = units_of(p);
-    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cu_count() / wgs, units / 8));
-    if (p.n_rows > 65535) pl.splits = 1;
+    // few tiles: the positions in parts of four units at least, where that saves a workgroup
+    // more units than the join costs
+    const int64_t wgs = tiles_of(p) * p.n_kv_head, units = units_of(p) / p.n_seq;
+    const int64_t n = std::min<int64_t>(cu_count() / wgs, units / 4);
+    pl.splits = n > 1 && units * (n - 1) > 8 * n ? (int)n : 1;
     pl.ws_bytes = (planes_bytes(p) + 255) / 256 * 256;
     if (pl.splits > 1) pl.ws_bytes += sizeof(float) * (size_t)p.n_rows * p.n_head * pl.splits * (p.head_dim + 4);
     return pl;
@@ -582,7 +637,7 @@ hipError_t launch_attn_prompt(const ggq_attention_prompt_params& p, const AttnPr
 #define L(HD_, T_)                                                               \
     planes_kernel<HD_, T_><<<pre, 256, 0, s>>>(a);                               \
     attn_kernel<HD_, T_><<<grid, waves_of<HD_>() * 64, 0, s>>>(a);               \
-    if (pl.splits > 1) attn_join_kernel<HD_><<<dim3((unsigned)p.n_rows, (unsigned)std::min(p.n_head, 8)), HD_, 0, s>>>(a)
+    if (pl.splits > 1) attn_join_kernel<HD_><<<dim3((unsigned)(((int64_t)p.n_rows * p.n_head + 3) / 4)), 256, 0, s>>>(a)
 #define BY_T(HD_)                                        \
     if (p.type == GGQ_TYPE_F32) { L(HD_, float); }       \
     else { L(HD_, _Float16); }

@@ -383,7 +383,8 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * less: a prompt's next chunk is n query rows against all positions so far.
  * With window > 0 a row sees the last `window` of those only.  A row that
  * sees nothing gets zeros; rows outside of all sequences stay as they were.
- * Keys that a row does not see do not count, whatever they hold.  Rows are
+ * Keys that a row does not see do not count, whatever they hold; a query or
+ * seen key that is not finite makes the row's result NaN.  Rows are
  * [n_head or n_kv_head][head_dim] values, dense, with row strides ld*; q and
  * out fp32, k and v of `type` (GGQ_TYPE_F32 or GGQ_TYPE_F16, a slab
  * [position][n_kv_head][head_dim] as it is); head_dim 64, 128 or 256; any
