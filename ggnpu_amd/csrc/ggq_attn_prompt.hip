@@ -106,7 +106,9 @@ constexpr int kUnit = 32;  // positions
 // are scaled beyond those of the unit's largest values, as negative numbers
 // (32 of K, 32 of V; 16 bits each where 32 would bring the LDS of a workgroup to 128 KB), then
 // dwords, all alike: those ones' exponents (+ 512), whether some values are not
-// finite (zero in the planes), whether there are any but zero.
+// finite (zero in the planes), whether there are any but zero, whether any of
+// the numbers before is not zero.  (Up to 2^8 below the unit's largest hi + lo
+// keep all that matters: zero.)
 template <int HD> struct Head {
     typedef int num;
     static constexpr int bytes = 512, info = 256;
@@ -117,7 +119,7 @@ template <> struct Head<256> {
 };
 // Bytes of a unit: header, K and V planes.
 template <int HD> constexpr int64_t unit_bytes(int planes) { return (int64_t)planes * 2 * kUnit * HD * 2 + Head<HD>::bytes; }
-enum { BAD_V = 1 << 20, NO_V = 1 << 21 };
+enum { BAD_V = 1 << 20, NO_V = 1 << 21, OWN_K = 1 << 22, OWN_V = 1 << 23 };
 
 // Sequence s has the units from off[s] / 32 + s on (and as many column tiles of
 // n from off[s] * G / n + s): a bound that needs no sum over the sequences before.
@@ -214,7 +216,10 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
     bad = red[0][2] | red[1][2] | red[2][2] | red[3][2];
     // fp16 values stay as they are
     const int ku = P == 2 ? up_to_2_15(uk) : 0, vu = P == 2 ? up_to_2_15(uv) : 0;
-    const int ke = P == 2 && mk ? up_to_2_15(mk) : ku, ve = P == 2 && mv ? up_to_2_15(mv) : vu;
+    int ke = P == 2 && mk ? up_to_2_15(mk) : ku, ve = P == 2 && mv ? up_to_2_15(mv) : vu;
+    if (ke <= ku + 8) ke = ku;
+    if (ve <= vu + 8) ve = vu;
+    const int own_k = __syncthreads_or(ke != ku), own_v = __syncthreads_or(ve != vu);
     typedef typename Head<HD>::num num;
     uint8_t* out = a.planes + (id * a.p.n_kv_head + kvh) * unit_bytes<HD>(P);
     if (tid % 8 == 0) {
@@ -222,7 +227,8 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
         ((num*)out)[32 + pos] = (num)(vu - ve);
     }
     if (tid < (Head<HD>::bytes - Head<HD>::info) / 4)
-        ((uint32_t*)(out + Head<HD>::info))[tid] = (uint32_t)(ku + 512) | (uint32_t)(vu + 512) << 10 | bad | (uv ? 0 : NO_V);
+        ((uint32_t*)(out + Head<HD>::info))[tid] = (uint32_t)(ku + 512) | (uint32_t)(vu + 512) << 10 | bad | (uv ? 0 : NO_V) |
+                                                    (own_k ? OWN_K : 0) | (own_v ? OWN_V : 0);
     _Float16* kp = (_Float16*)(out + Head<HD>::bytes);
 #pragma unroll
     for (int i = 0; i < V; i += 8) {
@@ -268,13 +274,16 @@ __device__ __forceinline__ void dma4(const uint8_t* src, uint32_t lane4, uint32_
 }
 
 
-// fp16 parts j and j + 1 of a pair of values.
-__device__ __forceinline__ void split_pair(float a, float b, h8& hi, h8& lo, int j) {
-    const h2 p = {(_Float16)a, (_Float16)b};
-    hi[j] = p[0];
-    hi[j + 1] = p[1];
-    lo[j] = (_Float16)fmaf((float)p[0], -1.0f, a);
-    lo[j + 1] = (_Float16)fmaf((float)p[1], -1.0f, b);
+// fp16 parts j and j + 1 of a pair of values: hi cut, lo rounded (2^-22 of the value).
+// minus1 is -1 where the compiler does not see it, which makes value - hi one
+// instruction on the packed halves (v_fma_mix_f32).
+__device__ __forceinline__ void split_pair(float a, float b, h2 minus1, h8& hi, h8& lo, int j) {
+    const auto p = __builtin_amdgcn_cvt_pkrtz(a, b);
+    const h2 q = __builtin_bit_cast(h2, p);
+    hi[j] = q[0];
+    hi[j + 1] = q[1];
+    lo[j] = (_Float16)fmaf((float)q[0], (float)minus1[0], a);
+    lo[j + 1] = (_Float16)fmaf((float)q[1], (float)minus1[1], b);
 }
 
 // Wavefronts of a workgroup: two a SIMD, or one of 256-wide heads, whose sums and
@@ -322,21 +331,26 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     const int per = (max(all1 - all0, 0) + a.splits - 1) / a.splits;
     const int u0 = all0 + split * per, u1 = min(all1, u0 + per), n = u1 - u0;
 
-    // loads for iteration it: the keys of its next but one unit, the values of its next
+    // loads for iteration it: the keys of its next but one unit, the values of its next (outside of what
+    // there is, the nearest unit: the same number of loads each time).  A wavefront has LD KB in a row,
+    // of the keys in the first half of the wavefronts, of the values in the second.
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const uint8_t* units = a.planes + ((bound_of(ks.a, kUnit, seq) + u0) * p.n_kv_head + kvh) * UB;
-    auto fetch = [&](int it) {  // (outside of what there is, the nearest unit: the same number of loads each time)
-        const uint8_t* ksrc = units + (int64_t)min(it + 2, n - 1) * p.n_kv_head * UB;
-        const uint8_t* vsrc = units + (int64_t)max(min(it + 1, n - 1), 0) * p.n_kv_head * UB + KB;
-        const uint32_t kdst = lds_at + (it & 1) * KB, vdst = lds_at + 2 * KB + ((it + 1) & 1) * VB;
-        dma4(ksrc, (uint32_t)lane * 4u, kdst);
-        if constexpr (HB == 512) dma4(ksrc + 256, (uint32_t)lane * 4u, kdst + 256u);
+    const int64_t stride = p.n_kv_head * UB;
+    static_assert(KC % LD == 0, "a wavefront loads of one kind");
+    const bool of_k = wave * LD < KC;
+    const uint8_t* const mine = units + (of_k ? HB + wave * LD * 1024 : KB + (wave * LD - KC) * 1024);
+    const uint32_t to = lds_at + (of_k ? (uint32_t)(HB + wave * LD * 1024) : (uint32_t)(2 * KB + (wave * LD - KC) * 1024));
+    auto fetch = [&](int it) {
+        const int uk = min(it + 2, n - 1), uv = max(min(it + 1, n - 1), 0);
+        const uint8_t* src = mine + (of_k ? uk : uv) * stride;
+        const uint32_t dst = to + (uint32_t)(of_k ? (it & 1) * KB : ((it + 1) & 1) * VB);
+        const uint8_t* head = units + uk * stride;
+        const uint32_t hdst = lds_at + (uint32_t)((it & 1) * KB);
+        dma4(head, (uint32_t)lane * 4u, hdst);
+        if constexpr (HB == 512) dma4(head + 256, (uint32_t)lane * 4u, hdst + 256u);
 #pragma unroll
-        for (int j = 0; j < LD; j++) {
-            const int c = wave * LD + j;
-            if (c < KC) dma16(ksrc + HB + c * 1024, (uint32_t)lane * 16u, kdst + (uint32_t)(HB + c * 1024));
-            else dma16(vsrc + (c - KC) * 1024, (uint32_t)lane * 16u, vdst + (uint32_t)(c - KC) * 1024u);
-        }
+        for (int j = 0; j < LD; j++) dma16(src + j * 1024, (uint32_t)lane * 16u, dst + (uint32_t)j * 1024u);
     };
     if (n > 0) {
         fetch(-2);
@@ -358,6 +372,8 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     const int fend = full ? min(max(shift + ra, 0), n_keys) : 0;  // (with columns that are no rows: masked throughout)
     const int fbeg = p.window ? max(shift + rb - p.window, 0) : 0;
 
+    h2 minus1 = {(_Float16)-1.0f, (_Float16)-1.0f};
+    asm volatile("" : "+v"(minus1));
     const float* qrow = p.q + (qs.a + qi) * p.ldq + (int64_t)head * HD;
     h8 qh[KS], ql[KS];
     int qe;
@@ -378,7 +394,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             const float v[8] = {x[2 * s].x, x[2 * s].y, x[2 * s].z, x[2 * s].w, x[2 * s + 1].x, x[2 * s + 1].y, x[2 * s + 1].z, x[2 * s + 1].w};
 #pragma unroll
             for (int j = 0; j < 8; j += 2)  // (NaN for an infinity, and so is its row)
-                split_pair(ldexpf(v[j], qe), ldexpf(v[j + 1], qe), qh[s], ql[s], j);
+                split_pair(ldexpf(v[j], qe), ldexpf(v[j + 1], qe), minus1, qh[s], ql[s], j);
         }
     }
 
@@ -390,7 +406,6 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     constexpr int kNone = 1 << 20;
     int ve = 0, least = kNone;
     uint32_t info = 0, bad = 0;
-    int dk[16];
     auto skips = [&](int it) {  // none of the wavefront's columns sees anything of the unit
         const int base = (u0 + it) * kUnit;
         return base >= wend || base + kUnit <= wbeg;
@@ -425,8 +440,13 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         }
         // (the slot is loaded over before the weights of the wavefronts behind)
         if constexpr (P == 2) {
-            numbers(slot, dk);
-            numbers(slot + 32 * sizeof(num), dv);
+            if (info & OWN_K) {
+                int dk[16];
+                numbers(slot, dk);
+#pragma unroll
+                for (int i = 0; i < 16; i++) st[i] = ldexpf(st[i], dk[i]);
+            }
+            if (info & OWN_V) numbers(slot + 32 * sizeof(num), dv);
         }
     };
     h8 ph[2], pl[2];
@@ -435,10 +455,6 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         const bool masked = masks(it);
         const int ku = (int)(info & 1023u) - 512, vu = (int)(info >> 10 & 1023u) - 512;
         bad |= info;
-        if constexpr (P == 2) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) st[i] = ldexpf(st[i], dk[i]);
-        }
         int vmin = vu;  // of the values that the column sees
         if (masked) {
             int most = -kNone;
@@ -447,7 +463,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
                 const int at = base + 8 * (i / 4) + 4 * h + i % 4;
                 const bool out = at >= end || at < beg;
                 if (out) st[i] = -INFINITY;
-                if constexpr (P == 2) most = max(most, out ? -kNone : dv[i]);
+                if constexpr (P == 2) most = max(most, out ? -kNone : info & OWN_V ? dv[i] : 0);
             }
             if constexpr (P == 2) vmin = vu - max(most, __shfl_xor(most, 32, 64));
         }
@@ -481,22 +497,27 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
                 ve = to;
             }
         }
-        const float ref = m == -INFINITY ? 0.0f : m - 11.0f;
+        // the weights in the sums' unit (at most the values': ve <= vu for what the column sees;
+        // below 2^-100 of it they are nothing)
+        const int c = P == 2 ? max(min(ve - vu, 0), -100) : 0;
+        const float ref = m == -INFINITY ? 0.0f : m - 11.0f - (float)c;
         float e[16], sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             e[i] = __builtin_amdgcn_exp2f(fmaf(st[i], cs, -ref));
             sum[i & 1] += e[i];
         }
-        l += sum[0] + sum[1];
+        l += P == 2 ? ldexpf(sum[0] + sum[1], -c) : sum[0] + sum[1];
         if constexpr (P == 2) {
+            if (info & OWN_V) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) e[i] = ldexpf(e[i], dv[i] + (ve - vu));
+                for (int i = 0; i < 16; i++) e[i] = ldexpf(e[i], dv[i] + (ve - vu - c));
+            }
         }
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) split_pair(e[8 * t + j], e[8 * t + j + 1], ph[t], pl[t], j);
+            for (int j = 0; j < 8; j += 2) split_pair(e[8 * t + j], e[8 * t + j + 1], minus1, ph[t], pl[t], j);
     };
     auto sums = [&](int it) {
         const h8* vp = (const h8*)(lds + 2 * KB + (it & 1) * VB) + lane;
