@@ -303,13 +303,14 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     constexpr int64_t UB = unit_bytes<HD>(P);
     typedef typename Head<HD>::num num;
     constexpr int HB = Head<HD>::bytes, KB = HB + P * PL, VB = P * PL;          // LDS bytes of a unit's header and keys, of its values
-    constexpr int KC = P * PL / 1024, LD = 2 * KC / NW;      // 1 KB loads of the keys; of a wavefront a unit (and the header)
+    constexpr int KC = P * PL / 1024, LD = 2 * KC / 4;       // 1 KB loads of the keys; of a loading wavefront a unit (and the header)
     constexpr int KS = HD / 16, DB = HD / 32;
-    static_assert(2 * KC % NW == 0 && 2 * (KB + VB) - 1024 < 128 * 1024, "LDS that global_load_lds addresses");
+    static_assert(2 * KC % 4 == 0 && 2 * (KB + VB) - 1024 < 128 * 1024, "LDS that global_load_lds addresses");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * (KB + VB)];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, h = lane >> 5;
     const bool behind = NW == 8 && wave >= 4;  // runs a phase behind the others
+    const bool loads = NW == 4 || behind;      // (those have time while the others are at the matrix cores)
     const ggq_attention_prompt_params& p = a.p;
     const int kvh = blockIdx.x % p.n_kv_head, split = blockIdx.y, G = a.G;
     const int id = a.tiles - 1 - (int)(blockIdx.x / p.n_kv_head);  // late rows see most: first
@@ -332,15 +333,15 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     const int u0 = all0 + split * per, u1 = min(all1, u0 + per), n = u1 - u0;
 
     // loads for iteration it: the keys of its next but one unit, the values of its next (outside of what
-    // there is, the nearest unit: the same number of loads each time).  A wavefront has LD KB in a row,
-    // of the keys in the first half of the wavefronts, of the values in the second.
+    // there is, the nearest unit: the same number of loads each time).  Two of the four wavefronts
+    // that load take the keys, two the values, LD KB in a row each.
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const uint8_t* units = a.planes + ((bound_of(ks.a, kUnit, seq) + u0) * p.n_kv_head + kvh) * UB;
     const int64_t stride = p.n_kv_head * UB;
-    static_assert(KC % LD == 0, "a wavefront loads of one kind");
-    const bool of_k = wave * LD < KC;
-    const uint8_t* const mine = units + (of_k ? HB + wave * LD * 1024 : KB + (wave * LD - KC) * 1024);
-    const uint32_t to = lds_at + (of_k ? (uint32_t)(HB + wave * LD * 1024) : (uint32_t)(2 * KB + (wave * LD - KC) * 1024));
+    const int share = wave & 3;
+    const bool of_k = share < 2;
+    const uint8_t* const mine = units + (of_k ? HB + share * LD * 1024 : KB + (share * LD - KC) * 1024);
+    const uint32_t to = lds_at + (of_k ? (uint32_t)(HB + share * LD * 1024) : (uint32_t)(2 * KB + (share * LD - KC) * 1024));
     auto fetch = [&](int it) {
         const int uk = min(it + 2, n - 1), uv = max(min(it + 1, n - 1), 0);
         const uint8_t* src = mine + (of_k ? uk : uv) * stride;
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
 #pragma unroll
         for (int j = 0; j < LD; j++) dma16(src + j * 1024, (uint32_t)lane * 16u, dst + (uint32_t)j * 1024u);
     };
-    if (n > 0) {
+    if (n > 0 && loads) {
         fetch(-2);
         fetch(-1);
     }
@@ -425,19 +426,30 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         }
     };
     int dv[P == 2 ? 16 : 1];
+    auto open = [&](int it) { info = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(lds + (it & 1) * KB + Head<HD>::info)); };
     auto scores = [&](int it) {
-        const uint8_t* slot = lds + (it & 1) * KB;
-        info = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(slot + Head<HD>::info));
-        if (skips(it)) return;
-        const h8* kp = (const h8*)(slot + HB) + lane;
-        st = f16v{};
+        const h8* kp = (const h8*)(lds + (it & 1) * KB + HB) + lane;
+        // two sums in turn where no other wavefront fills the wait of a product for the one before it
+        // (256-wide heads, 2048 rows: 238 -> 221 us; 128-wide ones do without: 166 -> 170)
+        constexpr int NA = NW == 8 ? 1 : 2;
+        f16v sa[NA] = {};
+        int turn = 0;
+        auto add = [&](h8 x, h8 y) {
+            sa[turn % NA] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, sa[turn % NA], 0, 0, 0);
+            turn++;
+        };
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const h8 kh = kp[s * 64];
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[s], st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[s], st, 0, 0, 0);
-            if constexpr (P == 2) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kp[s * 64 + PL / 16], qh[s], st, 0, 0, 0);
+            add(kh, qh[s]);
+            add(kh, ql[s]);
+            if constexpr (P == 2) add(kp[s * 64 + PL / 16], qh[s]);
         }
+        st = sa[0];
+        if constexpr (NA == 2) st += sa[1];
+    };
+    auto powers = [&](int it) {
+        const uint8_t* slot = lds + (it & 1) * KB;
         // (the slot is loaded over before the weights of the wavefronts behind)
         if constexpr (P == 2) {
             if (info & OWN_K) {
@@ -524,32 +536,53 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int d = 0; d < DB; d++) {
-                const h8 vh = vp[(2 * d + t) * 64];
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[t], o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[t], o[d], 0, 0, 0);
-                if constexpr (P == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vp[(2 * d + t) * 64 + PL / 16], ph[t], o[d], 0, 0, 0);
+            for (int d0 = 0; d0 < DB; d0 += 2) {
+                h8 vh[2];
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    vh[d] = vp[(2 * (d0 + d) + t) * 64];
+                    o[d0 + d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[d], ph[t], o[d0 + d], 0, 0, 0);
+                }
+#pragma unroll
+                for (int d = 0; d < 2; d++) o[d0 + d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[d], pl[t], o[d0 + d], 0, 0, 0);
+                if constexpr (P == 2) {
+#pragma unroll
+                    for (int d = 0; d < 2; d++)
+                        o[d0 + d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vp[(2 * (d0 + d) + t) * 64 + PL / 16], ph[t], o[d0 + d], 0, 0, 0);
+                }
             }
     };
     // Phases of the workgroup, by number: the wavefronts in front have weights(i) in 2 i and
     // products(i) in 2 i + 1, those behind one later.  In 2 i + 1 nobody uses the keys of unit i or
-    // the values of unit i - 1 any more, and everybody loads over them; what was loaded is waited for at the end
-    // of 2 i + 2, before the first wavefronts need it.
+    // the values of unit i - 1 any more: those behind load over them, and wait at the end
+    // of 2 i + 2, before the ones in front need what came.  (Without any behind, all do so in
+    // weights(i) and at the end of products(i).)
     if (n > 0) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LD + HB / 256) : "memory");
-        scores(0);
+        open(0);
+        if (!skips(0)) {
+            scores(0);
+            powers(0);
+        }
         if (behind) phase_end(true);
         for (int it = 0; it < n; it++) {
-            if (behind) fetch(it);
+            if (loads) fetch(it);
             const bool on = !skips(it);
             if (on) weights(it);
-            phase_end(!behind);
-            if (!behind) fetch(it);
-            if (on) sums(it);
-            if (it + 1 < n) scores(it + 1);
-            phase_end(behind);
+            else ph[0] = ph[1] = pl[0] = pl[1] = h8{};
+            phase_end(false);
+            __builtin_amdgcn_s_setprio(1);
+            const bool next = it + 1 < n && !skips(it + 1);
+            if (it + 1 < n) open(it + 1);
+            if (on || next) {  // (in one piece, so that the second's reads of LDS go beside the first's products)
+                sums(it);
+                scores(it + 1);
+            }
+            if (next) powers(it + 1);
+            __builtin_amdgcn_s_setprio(0);
+            phase_end(loads);
         }
-        if (!behind) phase_end(true);
+        if (NW == 8 && !behind) phase_end(false);
     }
     const Two lh = halves(l);
     l = lh.a + lh.b;
