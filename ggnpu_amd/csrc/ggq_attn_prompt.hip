@@ -577,6 +577,16 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             if (on || next) {  // (in one piece, so that the second's reads of LDS go beside the first's products)
                 sums(it);
                 scores(it + 1);
+                // operands are read AHEAD of their products: a read takes longer than the two products that
+                // the compiler would leave it
+                constexpr int AHEAD = 8, NG = KS + 2 * DB;  // reads; operands (each of P planes, P + 1 products)
+                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+                for (int i = 0; i < NG - AHEAD / P; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, P + 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, P, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, (P + 1) * (AHEAD / P), 0);
             }
             if (next) powers(it + 1);
             __builtin_amdgcn_s_setprio(0);
