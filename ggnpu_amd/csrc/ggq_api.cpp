@@ -1316,8 +1316,9 @@ int ggq_attention_prompt_dev(ggq_ctx* c, const ggq_attention_prompt_params* p, v
         return set_status(c, GGQ_INVALID_PARAM, "row strides must hold a row's heads");
     if (p->n_rows < 0 || p->n_kv_rows < 0 || p->n_seq < 0 || p->window < 0 || !std::isfinite(p->scale))
         return set_status(c, GGQ_INVALID_PARAM, "need n_rows, n_kv_rows, n_seq, window >= 0 and a finite scale");
-    if ((int64_t)p->n_rows * (p->n_head / p->n_kv_head) + 512 > INT32_MAX)
-        return set_status(c, GGQ_INVALID_PARAM, "n_rows * (n_head / n_kv_head) must stay below 2^31");
+    if (((int64_t)p->n_rows * (p->n_head / p->n_kv_head) / 4 + p->n_seq) * p->n_kv_head > INT32_MAX ||
+        (int64_t)p->n_rows * (p->n_head / p->n_kv_head) + 512 > INT32_MAX)
+        return set_status(c, GGQ_INVALID_PARAM, "n_rows * n_head is too large");
     if (p->n_rows == 0 || p->n_seq == 0) return set_status(c, GGQ_OK);
     if (!p->q || !p->out || !p->q_off || (p->n_kv_rows && (!p->k || !p->v)))
         return set_status(c, GGQ_INVALID_PARAM, "null q/k/v/out/q_off");
@@ -1329,8 +1330,8 @@ int ggq_attention_prompt_dev(ggq_ctx* c, const ggq_attention_prompt_params* p, v
     a.scale = log2_scale(p->scale, hd);
     const hipStream_t s = pick_stream(c, stream);
     const ggq::AttnPromptPlan pl = ggq::attn_prompt_plan(a);
-    void* ws = lane_ws(c, s, pl.ws_bytes, nullptr, 0);
-    const hipError_t e = ws ? ggq::launch_attn_prompt(a, pl, ws, s) : ggq::launch_attn_prompt_rows(a, s);
+    void* ws = pl.few ? nullptr : lane_ws(c, s, pl.ws_bytes, nullptr, 0);
+    const hipError_t e = ws ? ggq::launch_attn_prompt(a, pl, ws, s) : ggq::launch_attn_prompt_few(a, s);
     lane_done(c, s);
     return hip_status(c, e, "prompt attention");
     GGQ_END(c)

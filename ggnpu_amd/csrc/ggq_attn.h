@@ -53,13 +53,14 @@ size_t kv_attn_ws_floats(const KvAttnArgs& a, int splits);
 hipError_t launch_kv_attn(const KvAttnArgs& a, int splits, float* ws, hipStream_t s);
 
 // Causal attention of packed prompts: on the matrix cores with ws_bytes of
-// workspace, or row by row without one.
+// workspace, or (few rows and keys, or no workspace) on the VALU without one.
 struct AttnPromptPlan {
+    bool few;
     int splits;
     size_t ws_bytes;
 };
 AttnPromptPlan attn_prompt_plan(const ggq_attention_prompt_params& p);
 hipError_t launch_attn_prompt(const ggq_attention_prompt_params& p, const AttnPromptPlan& pl, void* ws, hipStream_t s);
-hipError_t launch_attn_prompt_rows(const ggq_attention_prompt_params& p, hipStream_t s);
+hipError_t launch_attn_prompt_few(const ggq_attention_prompt_params& p, hipStream_t s);
 
 }  // namespace ggq

@@ -27,6 +27,8 @@
 // position that a row does not see has no say in what the row keeps of the others.
 // Bound: the matrix cores.
 #include <algorithm>
+#include <cstdlib>
+#include <type_traits>
 
 #include "ggq_attn.h"
 #include "ggq_attn_device.h"
@@ -34,67 +36,6 @@
 
 namespace ggq {
 namespace {
-
-// The sequence of a row: the number of offsets behind the first one that are not above it.  All threads
-// of the workgroup call it.
-__device__ __forceinline__ int seq_of(const int32_t* off, int n_seq, int row) {
-    int s = 0;
-    for (int i = 0; i < n_seq; i += 256) {
-        const int j = i + (int)threadIdx.x;
-        s += __syncthreads_count(j < n_seq && off[j + 1] <= row);
-    }
-    return s;
-}
-
-// One query row of four heads, a wavefront a head.  64 positions at a time: a
-// lane has a position for the scores, HD / 64 values for the sum.
-template <int HD, typename T>
-__global__ __launch_bounds__(256) void attn_rows_kernel(ggq_attention_prompt_params a) {
-    constexpr int DPL = HD / 64;
-    __shared__ float sq[4][HD], sp[4][64];
-    const int row = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int head = blockIdx.y * 4 + wave;
-    const int seq = seq_of(a.q_off, a.n_seq, row);
-    if (seq >= a.n_seq || row < a.q_off[seq]) return;
-    if (head >= a.n_head) return;
-    const int32_t* kvo = a.kv_off ? a.kv_off : a.q_off;
-    const int64_t k0 = max(kvo[seq], 0), k1 = min(kvo[seq + 1], a.n_kv_rows);
-    // behind the last position it sees
-    const int64_t end = min(k1, k1 - ((int64_t)a.q_off[seq + 1] - 1 - row));
-    int64_t beg = k0;
-    if (a.window > 0) beg = max(beg, end - a.window);
-    const int kvh = head / (a.n_head / a.n_kv_head);
-    const float* q = a.q + (int64_t)row * a.ldq + (int64_t)head * HD;
-    for (int i = lane; i < HD; i += 64) sq[wave][i] = q[i] * a.scale;
-    __builtin_amdgcn_wave_barrier();
-    float m = -INFINITY, l = 0.0f, o[DPL] = {};
-    for (int64_t j0 = beg; j0 < end; j0 += 64) {
-        const int n = (int)min<int64_t>(64, end - j0);
-        float s = -INFINITY;
-        if (lane < n) {
-            const T* k = (const T*)a.k + (j0 + lane) * a.ldk + (int64_t)kvh * HD;
-            s = 0.0f;
-            for (int i = 0; i < HD; i++) s = fmaf(sq[wave][i], (float)k[i], s);
-        }
-        float mx = s;
-        for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn;
-        const float al = exp2f(m - ref), p = lane < n ? exp2f(s - ref) : 0.0f;
-        float ps = p;
-        for (int off = 32; off > 0; off >>= 1) ps += __shfl_xor(ps, off, 64);
-        l = l * al + ps;
-        m = mn;
-        sp[wave][lane] = p;
-        __builtin_amdgcn_wave_barrier();
-        for (int i = 0; i < DPL; i++) o[i] *= al;
-        const T* v = (const T*)a.v + j0 * a.ldv + (int64_t)kvh * HD + lane;
-        for (int j = 0; j < n; j++)
-            for (int i = 0; i < DPL; i++) o[i] = fmaf(sp[wave][j], (float)v[j * a.ldv + 64 * i], o[i]);
-        __builtin_amdgcn_wave_barrier();
-    }
-    float* out = a.out + (int64_t)row * a.ldo + (int64_t)head * HD + lane;
-    for (int i = 0; i < DPL; i++) out[64 * i] = end <= beg ? 0.0f : o[i] / l;
-}
 
 // ------------------------------------------------------------ matrix cores
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -150,6 +91,147 @@ __device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uin
 
 // Exponent that brings a magnitude into [2^14, 2^15).
 __device__ __forceinline__ int up_to_2_15(uint32_t bits) { return bits ? 141 - (int)(bits >> 23) : 0; }
+
+// Few rows, few keys, or no workspace: kCols columns of one sequence and kv head a
+// workgroup, on the VALU in fp32.  The four wavefronts take 16 positions each in turn, keys
+// and values in flight together; four lanes share a position for the scores (its key
+// against all columns' queries), a lane has HD / 64 values for the sums, and the
+// wavefronts' sums meet in LDS.  One launch of few dependent loads.
+constexpr int kCols = 4;
+template <int HD, typename T>
+__global__ __launch_bounds__(256) void attn_few_kernel(PromptArgs a) {
+    constexpr int DPL = HD / 64, C = kCols, PR = 16 / sizeof(T);
+    static_assert(C == 4, "a quad of lanes writes a position's weights");
+    __shared__ __attribute__((aligned(16))) float sq[C][HD], sp[4][16][C], so[4][C][HD], sm[4][C], sl[4][C];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const ggq_attention_prompt_params& p = a.p;
+    const int kvh = blockIdx.x % p.n_kv_head, G = a.G;
+    const int id = a.tiles - 1 - (int)(blockIdx.x / p.n_kv_head);
+    int seq = 0;
+    for (int i = 1; i < p.n_seq; i += 256) {
+        const int j = i + tid;
+        seq += __syncthreads_count(j < p.n_seq && (int)((uint32_t)max(min(p.q_off[j], p.n_rows), 0) * G / C) + j <= id);
+    }
+    const Span qs = span_of(p.q_off, seq, p.n_rows), ks = span_of(kv_off_of(p), seq, p.n_kv_rows);
+    const int nf = (int)qs.n * G, f0 = (id - ((int)((uint32_t)qs.a * G / C) + seq)) * C;
+    if (f0 < 0 || f0 >= nf) return;
+    const int n_keys = (int)ks.n, shift = n_keys - (int)qs.n + 1, nc = min(C, nf - f0);
+    int beg[C], end[C], first = n_keys, last = 0, all = n_keys, none = 0;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int qi = (int)((uint32_t)min(f0 + c, nf - 1) / G);
+        end[c] = min(max(shift + qi, 0), n_keys);
+        beg[c] = p.window ? min(max(shift + qi - p.window, 0), n_keys) : 0;
+        first = min(first, beg[c]);
+        last = max(last, end[c]);
+        none = max(none, beg[c]);  // every column sees [none, all)
+        all = min(all, end[c]);
+    }
+    for (int e = tid; e < C * HD; e += 256) {
+        const int f = min(f0 + e / HD, nf - 1), qi = (int)((uint32_t)f / G);
+        sq[e / HD][e % HD] = p.q[(qs.a + qi) * p.ldq + (int64_t)(kvh * G + f - qi * G) * HD + e % HD] * p.scale;
+    }
+    __syncthreads();
+    const T* kb = (const T*)p.k + ks.a * p.ldk + (int64_t)kvh * HD;
+    const T* vb = (const T*)p.v + ks.a * p.ldv + (int64_t)kvh * HD + lane * DPL;
+    float m[C], l[C], o[C][DPL];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        m[c] = -INFINITY;
+        l[c] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DPL; d++) o[c][d] = 0.0f;
+    }
+    struct alignas(16) Run { T x[PR]; };
+    struct alignas(DPL * sizeof(T)) Vals { T x[DPL]; };
+    constexpr int NR = HD / 4 / PR;  // runs of a lane: the ones 4 i + lane % 4 of its key
+    const int quad = lane & 3, at = lane >> 2;
+    for (int base = first + wave * 16; base < last; base += 64) {
+        const int pos = base + at, n = min(16, last - base);
+        const Run* kr = (const Run*)(kb + (int64_t)min(pos, last - 1) * p.ldk) + quad;
+        Run k[NR];
+#pragma unroll
+        for (int i = 0; i < NR; i++) k[i] = kr[4 * i];
+        constexpr int VJ = HD == 256 ? 8 : 16;  // values in flight
+        Vals v[VJ];
+        auto values = [&](int j0) {
+#pragma unroll
+            for (int j = 0; j < VJ; j++) v[j] = *(const Vals*)(vb + (int64_t)(base + min(j0 + j, n - 1)) * p.ldv);
+        };
+        values(0);
+        float s[C] = {};
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int j = 0; j < PR; j++) s[c] = fmaf(sq[c][(4 * i + quad) * PR + j], (float)k[i].x[j], s[c]);
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float t = s[c];
+            t += __shfl_xor(t, 1, 64);
+            t += __shfl_xor(t, 2, 64);
+            if (pos < beg[c] || pos >= end[c]) t = -INFINITY;
+            float mx = t;
+            mx = max3(mx, __shfl_xor(mx, 4, 64), mx);
+            mx = max3(mx, __shfl_xor(mx, 8, 64), mx);
+            const Two x = rows16(mx), y = halves(max3(x.a, x.b, x.b));
+            mx = max3(y.a, y.b, y.b);
+            const float mn = max3(m[c], mx, mx), ref = mn == -INFINITY ? 0.0f : mn;
+            const float al = __builtin_amdgcn_exp2f(m[c] - ref), e = __builtin_amdgcn_exp2f(t - ref);
+            m[c] = mn;
+            l[c] = l[c] * al + (quad == 0 ? e : 0.0f);  // (a lane's share)
+            if (quad == c) sp[wave][at][c] = e;
+#pragma unroll
+            for (int d = 0; d < DPL; d++) o[c][d] *= al;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const bool seen = base >= none && base + 16 <= all;  // by every column
+        auto add = [&](auto whole) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                if (j == VJ) values(j);
+                const float4 w = *(const float4*)sp[wave][j];
+                const float wc[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int d = 0; d < DPL; d++) {
+                        // (a value that is not seen may be anything)
+                        const float t = fmaf(wc[c], (float)v[j % VJ].x[d], o[c][d]);
+                        o[c][d] = whole || wc[c] != 0.0f ? t : o[c][d];
+                    }
+            }
+        };
+        if (seen) add(std::true_type{});
+        else add(std::false_type{});
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+#pragma unroll
+        for (int o_ = 1; o_ < 64; o_ <<= 1) l[c] += __shfl_xor(l[c], o_, 64);
+        if (lane == 0) { sm[wave][c] = m[c]; sl[wave][c] = l[c]; }
+#pragma unroll
+        for (int d = 0; d < DPL; d++) so[wave][c][lane * DPL + d] = o[c][d];
+    }
+    __syncthreads();
+    for (int e = tid; e < nc * HD; e += 256) {
+        const int c = e / HD, d = e % HD, f = f0 + c, qi = (int)((uint32_t)f / G);
+        const float mx = max3(max3(sm[0][c], sm[1][c], sm[2][c]), sm[3][c], sm[3][c]);
+        float ls = 0.0f, os = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float al = sm[w][c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][c] - mx);
+            ls = fmaf(sl[w][c], al, ls);
+            os = fmaf(so[w][c][d], al, os);
+        }
+        bool sees = false;
+#pragma unroll
+        for (int i = 0; i < C; i++) sees |= i == c && beg[i] < end[i];
+        p.out[(qs.a + qi) * p.ldo + (int64_t)(kvh * G + f - qi * G) * HD + d] = sees ? os / ls : 0.0f;
+    }
+}
 
 template <int HD, typename T>
 __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
@@ -679,6 +761,17 @@ size_t planes_bytes(const ggq_attention_prompt_params& p) {
 
 AttnPromptPlan attn_prompt_plan(const ggq_attention_prompt_params& p) {
     AttnPromptPlan pl{};
+    // The VALU's one launch up to 2^27 products of rows, heads, keys and values, while a wavefront
+    // does not go through the keys too often (us, few -> matrix cores; fp32, heads x kv heads x width):
+    //   19 rows: 32x8x64 7.2 -> 11.6, 16x2x256 10.0 -> 24.9; 128 rows: 32x8x128 18.6 -> 26.6
+    //   256 rows: 32x8x64 23.6 -> 24.6, 32x8x128 (2^28) 43.9 -> 34.2; 40 prompts of 150 rows,
+    //   8x8x64 (2^27.6) 62.7 -> 40.5; 512 rows 4x1x128 23.2 -> 31.0; 1000 rows 2x1x64 32.7 -> 27.1
+    //   one row: 501 keys 32x8x128 21.8 -> 23.5, 2001 keys 68 -> 40
+    const char* env = getenv("GGQ_PROMPT_MFMA");
+    const double keys = (double)p.n_kv_rows / p.n_seq;
+    if (env && *env) pl.few = atoi(env) == 0;
+    else pl.few = keys <= 640 && keys * p.n_rows * p.n_head * p.head_dim <= (double)(1 << 27) * 1.01;
+    if (pl.few) return pl;
     // few tiles: the positions in parts of four units at least, where that saves a workgroup
     // more units than the join costs
     const int64_t wgs = tiles_of(p) * p.n_kv_head, units = units_of(p) / p.n_seq;
@@ -713,11 +806,16 @@ hipError_t launch_attn_prompt(const ggq_attention_prompt_params& p, const AttnPr
     return hipGetLastError();
 }
 
-hipError_t launch_attn_prompt_rows(const ggq_attention_prompt_params& p, hipStream_t s) {
-    const dim3 grid((unsigned)p.n_rows, (unsigned)((p.n_head + 3) / 4));
-#define L(HD_)                                                                       \
-    if (p.type == GGQ_TYPE_F32) attn_rows_kernel<HD_, float><<<grid, 256, 0, s>>>(p); \
-    else attn_rows_kernel<HD_, _Float16><<<grid, 256, 0, s>>>(p)
+hipError_t launch_attn_prompt_few(const ggq_attention_prompt_params& p, hipStream_t s) {
+    PromptArgs a{};
+    a.p = p;
+    a.G = p.n_head / p.n_kv_head;
+    a.splits = 1;
+    a.tiles = (int)((int64_t)p.n_rows * a.G / kCols + p.n_seq);
+    const dim3 grid((unsigned)(a.tiles * (int64_t)p.n_kv_head));
+#define L(HD_)                                                                    \
+    if (p.type == GGQ_TYPE_F32) attn_few_kernel<HD_, float><<<grid, 256, 0, s>>>(a); \
+    else attn_few_kernel<HD_, _Float16><<<grid, 256, 0, s>>>(a)
     if (p.head_dim == 64) { L(64); }
     else if (p.head_dim == 128) { L(128); }
     else { L(256); }

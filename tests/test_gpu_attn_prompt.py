@@ -11,12 +11,19 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.fixture(scope="module")
-def ctx():
+def gpu():
     import torch
     assert torch.cuda.is_available()
     c = gl.Context(0)
     yield c
     c.close()
+
+
+@pytest.fixture(params=["", "0", "1"], ids=["rule", "valu", "mfma"])
+def ctx(gpu, request, monkeypatch):
+    """Every test on the route of the rule and on both routes (GGQ_PROMPT_MFMA, read at every call)."""
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", request.param)
+    return gpu
 
 
 def t(a):
