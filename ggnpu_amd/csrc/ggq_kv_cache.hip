@@ -27,54 +27,74 @@ struct Place {
     uint8_t* rec;  // null: there is none
     int p;         // 0..31
 };
-__device__ __forceinline__ Place place_of(const ggq_kv_cache& c, const ggq_kv_seqs& q, int64_t rec_bytes, int seq,
-                                          int64_t pos, int head) {
+template <uint32_t RB>
+__device__ __forceinline__ Place place_of(const ggq_kv_cache& c, const ggq_kv_seqs& q, int seq, int64_t pos, int head) {
     if (pos < 0 || pos >= (int64_t)q.table_len * c.page_len) return Place{nullptr, 0};
-    const uint32_t at = (uint32_t)(pos / c.page_len), in = (uint32_t)(pos % c.page_len);
-    const int32_t page = q.pages[(int64_t)seq * q.table_len + at];
+    const uint32_t at = (uint32_t)pos / (uint32_t)c.page_len, in = (uint32_t)pos - at * (uint32_t)c.page_len;
+    const int32_t page = q.pages[(uint64_t)(uint32_t)seq * (uint32_t)q.table_len + at];
     if (page < 0 || page >= c.n_pages) return Place{nullptr, 0};
-    const int64_t r = ((int64_t)page * c.n_kv_head + head) * (c.page_len / kKvTile) + in / kKvTile;
-    return Place{(uint8_t*)c.pages + r * rec_bytes, (int)(in % kKvTile)};
+    // (fewer than 2^32 records: they have a kilobyte or more)
+    const uint32_t r = ((uint32_t)page * (uint32_t)c.n_kv_head + (uint32_t)head) * ((uint32_t)c.page_len / kKvTile) + in / kKvTile;
+    return Place{(uint8_t*)c.pages + (uint64_t)r * RB, (int)(in % kKvTile)};
 }
 
 // Rows to or from the pages.  A workgroup takes U times 2048 values of one kv
 // head, K (z = 0) or V, a thread 8 consecutive ones of each of U rows; 4 threads share a
 // block of 32.  The rows' sequences are found by all threads together: one
 // strided look over row_off for the first row, a step forward for each
-// sequence that ends among the rows.  A row's place is three dependent
+// sequence that ends among the rows (in LDS for up to 256).  A row's place is three dependent
 // loads away (offsets and length, page, codes), so large calls have U = 4 of
 // them in flight a thread.
-template <int HD, int BITS, bool VALUE, bool STORE, int U, typename T>
-__device__ __forceinline__ void rows_body(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r, int64_t rec_bytes) {
+template <int HD, int KB, int VB, bool VALUE, bool STORE, int U, typename T>
+__device__ __forceinline__ void rows_body(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r) {
+    constexpr int BITS = VALUE ? VB : KB;
+    constexpr uint32_t RB = kKvTile * HD * (KB + VB) / 8 + 2 * HD;
+    constexpr int kNear = 256;  // sequences whose offsets and lengths are looked up in LDS
+    __shared__ int32_t s_off[kNear + 1], s_len[kNear];
     constexpr int RPW = 2048 / HD;  // rows of a workgroup's pass
     constexpr int TPR = HD / 8;     // threads of a row
     const int tid = threadIdx.x, head = blockIdx.y, d = tid % TPR * 8;
     const int row0 = blockIdx.x * RPW * U;
     int first = 0;
-    if (r.row_off)
+    const bool near = q.n_seq <= kNear;
+    if (r.row_off) {
         for (int i = 0; i < q.n_seq; i += 256) {
             const int j = i + tid;
-            first += __syncthreads_count(j < q.n_seq && r.row_off[j + 1] <= row0);
-        }
-    Place pl[U];
-#pragma unroll
-    for (int i = 0; i < U; i++) {
-        const int row = row0 + i * RPW + tid / TPR;
-        int seq = row;
-        int64_t pos = -1;
-        if (r.row_off) {
-            seq = first;
-            while (seq < q.n_seq && r.row_off[seq + 1] <= row) seq++;
-            first = seq;
-            if (row < r.n_rows && seq < q.n_seq) {
-                const int32_t a = r.row_off[seq], b = r.row_off[seq + 1];
-                if (row >= a) pos = (int64_t)q.len[seq] - b + row;
+            int32_t o = 0, l = 0;
+            if (j < q.n_seq) {
+                o = r.row_off[j + 1];
+                if (near) l = q.len[j];
             }
-        } else if (row < r.n_rows && row < q.n_seq) {
-            pos = (int64_t)q.len[row] - 1;
+            if (near && j < q.n_seq) {
+                s_off[j + 1] = o;
+                s_len[j] = l;
+                if (j == 0) s_off[0] = r.row_off[0];
+            }
+            first += __syncthreads_count(j < q.n_seq && o <= row0);
         }
-        pl[i] = Place{nullptr, 0};
-        if (pos >= 0) pl[i] = place_of(c, q, rec_bytes, seq, pos, head);
+    }
+    Place pl[U];
+    auto find = [&](auto off, auto len) {  // (apart for LDS and memory: one access for both would be a generic one)
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int row = row0 + i * RPW + tid / TPR;
+            int64_t pos = -1;
+            while (first < q.n_seq && off(first + 1) <= row) first++;
+            if (row < r.n_rows && first < q.n_seq && row >= off(first)) pos = (int64_t)len(first) - off(first + 1) + row;
+            pl[i] = pos >= 0 ? place_of<RB>(c, q, first, pos, head) : Place{nullptr, 0};
+        }
+    };
+    if (!r.row_off) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int row = row0 + i * RPW + tid / TPR;
+            const bool in = row < r.n_rows && row < q.n_seq;
+            pl[i] = in ? place_of<RB>(c, q, row, (int64_t)q.len[row] - 1, head) : Place{nullptr, 0};
+        }
+    } else if (near) {
+        find([&](int i) { return s_off[i]; }, [&](int i) { return s_len[i]; });
+    } else {
+        find([&](int i) { return r.row_off[i]; }, [&](int i) { return q.len[i]; });
     }
     // codes of this thread: 8 in one run, or two runs of 4 (V of 64-wide heads)
     constexpr int RUN = VALUE && HD == 64 ? 4 : 8;
@@ -91,15 +111,14 @@ __device__ __forceinline__ void rows_body(const ggq_kv_cache& c, const ggq_kv_se
         return 1024 * (b / 16) + 16 * lane + b % 16;
     };
     const int blk = d / 32;
-    auto codes_of = [&](const Place& x) { return x.rec + (VALUE ? kKvTile * HD * c.k_type / 8 : 0); };
+    auto codes_of = [&](const Place& x) { return x.rec + (VALUE ? kKvTile * HD * KB / 8 : 0); };
     auto scale_at = [&](const Place& x) {
         const int p = x.p;
-        return x.rec + kKvTile * HD * (c.k_type + c.v_type) / 8 +
+        return x.rec + kKvTile * HD * (KB + VB) / 8 +
                (VALUE ? HD + (4 * blk + p % 16 / 4) * 8 + 4 * (p / 16) + p % 4 : (16 * blk + p % 16) * 2 + p / 16);
     };
-    auto row_at = [&](int i) {
-        return (T*)(VALUE ? r.v : r.k) + (int64_t)(row0 + i * RPW + tid / TPR) * (VALUE ? r.ldv : r.ldk) + (int64_t)head * HD + d;
-    };
+    T* const row_base = (T*)(VALUE ? r.v : r.k) + (int64_t)(row0 + tid / TPR) * (VALUE ? r.ldv : r.ldk) + head * HD + d;
+    auto row_at = [&](int i) { return row_base + (int64_t)(i * RPW) * (VALUE ? r.ldv : r.ldk); };
     struct alignas(16) Run { T x[16 / sizeof(T)]; };
     constexpr int NR = 8 * sizeof(T) / 16, PR = 16 / sizeof(T);  // 16-byte runs of 8 values
     if constexpr (STORE) {
@@ -207,17 +226,17 @@ __device__ __forceinline__ void rows_body(const ggq_kv_cache& c, const ggq_kv_se
 }
 
 template <int HD, int KB, int VB, bool STORE, int U, typename T>
-__global__ __launch_bounds__(256) void kv_rows_kernel(ggq_kv_cache c, ggq_kv_seqs q, KvRows r, int64_t rec_bytes) {
-    if (blockIdx.z == 0) rows_body<HD, KB, false, STORE, U, T>(c, q, r, rec_bytes);
-    else rows_body<HD, VB, true, STORE, U, T>(c, q, r, rec_bytes);
+__global__ __launch_bounds__(256) void kv_rows_kernel(ggq_kv_cache c, ggq_kv_seqs q, KvRows r) {
+    if (blockIdx.z == 0) rows_body<HD, KB, VB, false, STORE, U, T>(c, q, r);
+    else rows_body<HD, KB, VB, true, STORE, U, T>(c, q, r);
 }
 
 template <int HD, int KB, int VB, int U, typename T>
 void rows_go(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r, bool store, hipStream_t s) {
     const int per = U * 2048 / HD;
     const dim3 grid((unsigned)((r.n_rows + per - 1) / per), (unsigned)c.n_kv_head, 2);
-    if (store) kv_rows_kernel<HD, KB, VB, true, U, T><<<grid, 256, 0, s>>>(c, q, r, kv_record_bytes(c));
-    else kv_rows_kernel<HD, KB, VB, false, U, T><<<grid, 256, 0, s>>>(c, q, r, kv_record_bytes(c));
+    if (store) kv_rows_kernel<HD, KB, VB, true, U, T><<<grid, 256, 0, s>>>(c, q, r);
+    else kv_rows_kernel<HD, KB, VB, false, U, T><<<grid, 256, 0, s>>>(c, q, r);
 }
 
 template <int HD, int KB, int VB> hipError_t rows_launch(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r,
