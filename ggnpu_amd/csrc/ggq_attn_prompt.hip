@@ -71,6 +71,7 @@ struct PromptArgs {
     uint8_t* planes;
     float* part;
     int G, tiles, splits;
+    int kv0, kvn;  // the kv heads of this launch, whose planes there is room for
 };
 
 // A sequence's rows of an offset array, held inside [0, n].
@@ -239,7 +240,7 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
     constexpr int PL = kUnit * HD;                         // values of a plane
     __shared__ float sv[kUnit][HD + 1];
     __shared__ uint32_t red[4][3];
-    const int tid = threadIdx.x, kvh = blockIdx.y;
+    const int tid = threadIdx.x, kvh = a.kv0 + blockIdx.y;
     const int32_t* off = kv_off_of(a.p);
     const int64_t id = blockIdx.x;
     int seq = 0;
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
     if (ve <= vu + 8) ve = vu;
     const int own_k = __syncthreads_or(ke != ku), own_v = __syncthreads_or(ve != vu);
     typedef typename Head<HD>::num num;
-    uint8_t* out = a.planes + (id * a.p.n_kv_head + kvh) * unit_bytes<HD>(P);
+    uint8_t* out = a.planes + (id * a.kvn + (kvh - a.kv0)) * unit_bytes<HD>(P);
     if (tid % 8 == 0) {
         ((num*)out)[pos] = (num)(ku - ke);
         ((num*)out)[32 + pos] = (num)(vu - ve);
@@ -394,8 +395,8 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     const bool behind = NW == 8 && wave >= 4;  // runs a phase behind the others
     const bool loads = NW == 4 || behind;      // (those have time while the others are at the matrix cores)
     const ggq_attention_prompt_params& p = a.p;
-    const int kvh = blockIdx.x % p.n_kv_head, split = blockIdx.y, G = a.G;
-    const int id = a.tiles - 1 - (int)(blockIdx.x / p.n_kv_head);  // late rows see most: first
+    const int kvi = (int)(blockIdx.x % (unsigned)a.kvn), kvh = a.kv0 + kvi, split = blockIdx.y, G = a.G;
+    const int id = a.tiles - 1 - (int)(blockIdx.x / (unsigned)a.kvn);  // late rows see most: first
     constexpr int NC = NW * 32;
     int seq = 0;
     for (int i = 1; i < p.n_seq; i += NW * 64) {
@@ -418,8 +419,8 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     // there is, the nearest unit: the same number of loads each time).  Two of the four wavefronts
     // that load take the keys, two the values, LD KB in a row each.
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    const uint8_t* units = a.planes + ((bound_of(ks.a, kUnit, seq) + u0) * p.n_kv_head + kvh) * UB;
-    const int64_t stride = p.n_kv_head * UB;
+    const uint8_t* units = a.planes + ((bound_of(ks.a, kUnit, seq) + u0) * a.kvn + kvi) * UB;
+    const int64_t stride = a.kvn * UB;
     const int share = wave & 3;
     const bool of_k = share < 2;
     const uint8_t* const mine = units + (of_k ? HB + share * LD * 1024 : KB + (share * LD - KC) * 1024);
@@ -682,7 +683,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     if (bad & BAD_V) {
         // infinities and NaN among the values are zero in the planes: here they come, to the rows that see them
         for (int u = u0; u < u1; u++) {
-            if (!(*(const uint32_t*)(units + (int64_t)(u - u0) * p.n_kv_head * UB + Head<HD>::info) & BAD_V)) continue;
+            if (!(*(const uint32_t*)(units + (u - u0) * stride + Head<HD>::info) & BAD_V)) continue;
             for (int at = max(u * kUnit, beg); at < min((u + 1) * kUnit, end); at++) {
                 const T* vr = (const T*)p.v + (ks.a + at) * p.ldv + (int64_t)kvh * HD + 4 * h;
 #pragma unroll
@@ -752,11 +753,17 @@ int64_t tiles_of(const ggq_attention_prompt_params& p) {
     const int nc = (p.head_dim == 256 ? 4 : 8) * 32;
     return (int64_t)p.n_rows * (p.n_head / p.n_kv_head) / nc + p.n_seq;
 }
-size_t planes_bytes(const ggq_attention_prompt_params& p) {
+// Planes of one kv head, and how many heads' there are at a time: 256 MB of them, or
+// one head's.
+size_t head_bytes(const ggq_attention_prompt_params& p) {
     const int planes = p.type == GGQ_TYPE_F32 ? 2 : 1;
-    return (size_t)(units_of(p) * p.n_kv_head) *
+    return (size_t)units_of(p) *
            (p.head_dim == 64 ? unit_bytes<64>(planes) : p.head_dim == 128 ? unit_bytes<128>(planes) : unit_bytes<256>(planes));
 }
+int heads_at_once(const ggq_attention_prompt_params& p) {
+    return (int)std::max<size_t>(1, std::min<size_t>((size_t)p.n_kv_head, (size_t(256) << 20) / head_bytes(p)));
+}
+size_t planes_bytes(const ggq_attention_prompt_params& p) { return (head_bytes(p) * heads_at_once(p) + 255) / 256 * 256; }
 }  // namespace
 
 AttnPromptPlan attn_prompt_plan(const ggq_attention_prompt_params& p) {
@@ -773,11 +780,15 @@ AttnPromptPlan attn_prompt_plan(const ggq_attention_prompt_params& p) {
     else pl.few = keys <= 640 && keys * p.n_rows * p.n_head * p.head_dim <= (double)(1 << 27) * 1.01;
     if (pl.few) return pl;
     // few tiles: the positions in parts of four units at least, where that saves a workgroup
-    // more units than the join costs
+    // more units than the join costs (us with 1, 2, 3, 4 .. parts; * the rule's: 512 rows 32x8x128 49, 44,
+    // 41*; 16x2x256 66, 53, 50, 48*; 5 packed prompts 12x2x128 f16 49, 46*, 57; one row of 4001 keys
+    // 227, 128, .., 46 with 16, 50 with 31*)
     const int64_t wgs = tiles_of(p) * p.n_kv_head, units = units_of(p) / p.n_seq;
     const int64_t n = std::min<int64_t>(cu_count() / wgs, units / 4);
-    pl.splits = n > 1 && units * (n - 1) > 8 * n ? (int)n : 1;
-    pl.ws_bytes = (planes_bytes(p) + 255) / 256 * 256;
+    pl.splits = n > 1 && units * (n - 1) > 4 * n ? (int)n : 1;
+    if (const char* e = getenv("GGQ_PROMPT_SPLITS"); e && atoi(e) > 0)
+        pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(atoi(e), 256), units_of(p)));
+    pl.ws_bytes = planes_bytes(p);
     if (pl.splits > 1) pl.ws_bytes += sizeof(float) * (size_t)p.n_rows * p.n_head * pl.splits * (p.head_dim + 4);
     return pl;
 }
@@ -786,14 +797,17 @@ hipError_t launch_attn_prompt(const ggq_attention_prompt_params& p, const AttnPr
     PromptArgs a{};
     a.p = p;
     a.planes = (uint8_t*)ws;
-    a.part = (float*)((char*)ws + (planes_bytes(p) + 255) / 256 * 256);
+    a.part = (float*)((char*)ws + planes_bytes(p));
     a.G = p.n_head / p.n_kv_head;
     a.splits = pl.splits;
     a.tiles = (int)tiles_of(p);
-    const dim3 pre((unsigned)units_of(p), (unsigned)p.n_kv_head), grid((unsigned)(a.tiles * (int64_t)p.n_kv_head), (unsigned)pl.splits);
-#define L(HD_, T_)                                                               \
-    planes_kernel<HD_, T_><<<pre, 256, 0, s>>>(a);                               \
-    attn_kernel<HD_, T_><<<grid, waves_of<HD_>() * 64, 0, s>>>(a);               \
+    const int at_once = heads_at_once(p);
+#define L(HD_, T_)                                                                                                        \
+    for (a.kv0 = 0; a.kv0 < p.n_kv_head; a.kv0 += at_once) {                                                              \
+        a.kvn = std::min(at_once, p.n_kv_head - a.kv0);                                                                   \
+        planes_kernel<HD_, T_><<<dim3((unsigned)units_of(p), (unsigned)a.kvn), 256, 0, s>>>(a);                           \
+        attn_kernel<HD_, T_><<<dim3((unsigned)(a.tiles * (int64_t)a.kvn), (unsigned)pl.splits), waves_of<HD_>() * 64, 0, s>>>(a); \
+    }                                                                                                                     \
     if (pl.splits > 1) attn_join_kernel<HD_><<<dim3((unsigned)(((int64_t)p.n_rows * p.n_head + 3) / 4)), 256, 0, s>>>(a)
 #define BY_T(HD_)                                        \
     if (p.type == GGQ_TYPE_F32) { L(HD_, float); }       \

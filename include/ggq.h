@@ -86,7 +86,8 @@ int ggq_sync(ggq_ctx* ctx);
  * is too small it fails with GGQ_ERROR and says so in
  * ggq_last_error_message.  Size the workspace before a capture by running
  * the captured calls once outside it, or with ggq_reserve.
- * Matmuls of 5 rows and more also use a buffer per stream (streams from the
+ * Matmuls of 5 rows and more, attention of prompts and over a quantized cache
+ * also use a buffer per stream (streams from the
  * ninth on share eight, and their calls wait for one another where they meet
  * on one), and other kernels where it cannot be had: the same products, rounded
  * in another order, in several times the time.  A stream's work is complete
@@ -383,8 +384,9 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * less: a prompt's next chunk is n query rows against all positions so far.
  * With window > 0 a row sees the last `window` of those only.  A row that
  * sees nothing gets zeros; rows outside of all sequences stay as they were.
- * Keys that a row does not see do not count, whatever they hold; a query or
- * seen key that is not finite makes the row's result NaN.  Rows are
+ * Keys that a row does not see do not count, whatever they hold; a row that
+ * sees a key which is not finite, or whose query is not, has no defined
+ * result (the others keep theirs).  Rows are
  * [n_head or n_kv_head][head_dim] values, dense, with row strides ld*; q and
  * out fp32, k and v of `type` (GGQ_TYPE_F32 or GGQ_TYPE_F16, a slab
  * [position][n_kv_head][head_dim] as it is); head_dim 64, 128 or 256; any
