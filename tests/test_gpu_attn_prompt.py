@@ -211,6 +211,33 @@ def test_prompt_many_sequences(ctx):
     run(ctx, 19, off, None, 2, 1, 64)
 
 
+@pytest.mark.parametrize("splits", ["1", "2", "5", "1000"])
+def test_prompt_split_counts(gpu, monkeypatch, splits):
+    """Any number of parts of the positions (GGQ_PROMPT_SPLITS), empty ones among them, rows of no sequence left alone."""
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", "1")
+    monkeypatch.setenv("GGQ_PROMPT_SPLITS", splits)
+    run(gpu, 30, [0, 40, 41, 41, 60], [0, 300, 700, 710, 729], 6, 2, 64, 0, behind=3)
+    run(gpu, 31, [2, 90], [0, 260], 4, 1, 128, 1, window=100)
+    run(gpu, 32, [0, 20], [0, 7], 2, 2, 64)
+
+
+def test_prompt_not_finite_queries_and_keys_stay_in_their_rows(ctx):
+    rng = np.random.default_rng(33)
+    n, n_head, n_kv, hd = 80, 4, 2, 64
+    q, k, v = inputs(rng, n, n, n_head, n_kv, hd)
+    q2, k2 = q.copy(), k.copy()
+    q2[11, 64 * 2 + 5] = np.nan  # row 11, head 2
+    q2[12, 3] = np.inf  # row 12, head 0
+    k2[50, 64 + 7] = np.nan  # key 50 of kv head 1: heads 2 and 3 from row 50 on
+    got = call(ctx, q2, k2, v, n_head, n_kv, hd, 0, [0, n], None).reshape(n, n_head, hd)
+    assert np.isnan(got[11, 2]).all() and not np.isfinite(got[12, 0]).any() and np.isnan(got[50:, 2:]).all()
+    good = np.ones((n, n_head), bool)
+    good[11, 2] = good[12, 0] = False
+    good[50:, 2:] = False
+    want, tol = au.attention(q.reshape(n, n_head, hd), k.reshape(n, n_kv, hd), v.reshape(n, n_kv, hd), 0)
+    au.check(got[good], want[good], tol[good])
+
+
 def test_prompt_refusals(ctx):
     import torch
     x = torch.zeros(8192, device="cuda")
