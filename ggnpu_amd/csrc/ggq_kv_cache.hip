@@ -241,8 +241,8 @@ void rows_go(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r, bool 
 
 template <int HD, int KB, int VB> hipError_t rows_launch(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r,
                                                          bool store, hipStream_t s) {
-    // four rows a thread once that leaves every CU two workgroups (16 x 4001 rows of 2 heads of 128, f16: 24.3 us with one,
-    // see the launch below; 33 rows of 8 heads are quicker with one)
+    // four rows a thread once that leaves every CU two workgroups: their loads overlap (16 x 4001 rows of 2 heads of
+    // 128 into fp16: 24.3 us with one row, 18.7 with four); below that one row, for the shorter chain
     const bool many = (int64_t)r.n_rows * c.n_kv_head * HD * 2 / (4 * 2048) >= 2 * cu_count();
     if (r.type == GGQ_TYPE_F32) many ? rows_go<HD, KB, VB, 4, float>(c, q, r, store, s) : rows_go<HD, KB, VB, 1, float>(c, q, r, store, s);
     else many ? rows_go<HD, KB, VB, 4, _Float16>(c, q, r, store, s) : rows_go<HD, KB, VB, 1, _Float16>(c, q, r, store, s);
@@ -281,6 +281,10 @@ hipError_t launch_kv_rows(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvR
 // accumulators are rescaled a few times a sequence.
 // A workgroup has 8 wavefronts (4 where their registers allow no more) that take the records of its part of the
 // positions in turn and add up in LDS; kv_join_kernel adds up the parts.
+// Bound: HBM with 128-wide heads (64 sequences of up to 8191 positions, K in 8
+// and V in 4 bits: 566 MB in 103 us, 5.5 TB/s); with 64-wide ones the VALU, whose
+// work on scores does not shrink with the head (131001 positions: 238
+// instructions a record, 71 MB in 20.5 us and 3 us for the join).
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
