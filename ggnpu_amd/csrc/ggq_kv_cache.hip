@@ -284,7 +284,7 @@ hipError_t launch_kv_rows(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvR
 // Bound: HBM with 128-wide heads (64 sequences of up to 8191 positions, K in 8
 // and V in 4 bits: 566 MB in 103 us, 5.5 TB/s); with 64-wide ones the VALU, whose
 // work on scores does not shrink with the head (131001 positions: 238
-// instructions a record, 71 MB in 20.5 us and 3 us for the join).
+// instructions a record, 71 MB in 21 us and 4 us for the join).
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -14,8 +14,8 @@
 // are the same for all heads of a row: they are made once and used for
 // `passes` groups of heads.
 //
-// Bound: HBM (2049 rows of 24 heads of 128 with norms: 50 MB in 10.9 us, 4.6
-// TB/s); one token 3.6 us, a launch with two dependent loads.
+// Bound: HBM (2049 rows of 24 heads of 128 with norms: 50 MB in 11.2 us, 4.5
+// TB/s); one token 3.8 us, a launch with two dependent loads.
 #include "ggq_attn.h"
 #include "ggq_launch.h"
 
