@@ -640,8 +640,9 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     // Phases of the workgroup, by number: the wavefronts in front have weights(i) in 2 i and
     // products(i) in 2 i + 1, those behind one later.  In 2 i + 1 nobody uses the keys of unit i or
     // the values of unit i - 1 any more: those behind load over them, and wait at the end
-    // of 2 i + 2, before the ones in front need what came.  (Without any behind, all do so in
-    // weights(i) and at the end of products(i).)
+    // of 2 i + 2, before the ones in front need what came.  Without any behind, all do so in
+    // weights(i) and at the end of products(i); the first scores are then a phase of their own, because
+    // the loads of weights(0) go over their keys, and its end is where the values of unit 0 have come.
     if (n > 0) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LD + HB / 256) : "memory");
         open(0);
@@ -649,7 +650,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             scores(0);
             powers(0);
         }
-        if (behind) phase_end(true);
+        if (NW == 4 || behind) phase_end(true);
         for (int it = 0; it < n; it++) {
             if (loads) fetch(it);
             const bool on = !skips(it);

@@ -1,0 +1,67 @@
+"""Prompt attention where it could go wrong unseen: calls that follow each other without a wait, against themselves and
+against 64 bits."""
+import numpy as np
+import pytest
+
+import ggnpu_amd.lib as gl
+from tests import attn_util as au
+from tests.gpu_util import host, stream_handle
+from tests.test_gpu_attn_prompt import inputs, t
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    import torch
+    assert torch.cuda.is_available()
+    c = gl.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("type", [0, 1])
+@pytest.mark.parametrize("n_head,n_kv,q_off,kv_off,window", [
+    (8, 8, [0, 369], None, 0),
+    (2, 2, [0, 700, 1200], None, 0),
+    (4, 1, [0, 40, 41, 100], [0, 900, 2100, 2200], 0),
+    (5, 1, [0, 300], None, 14),  # wavefronts that skip the first units
+    (16, 2, [0, 205], [0, 413], 82),
+    (6, 2, [0, 3, 20, 22], [0, 3, 20, 22], 0),  # one unit, or less
+])
+def test_prompt_calls_in_a_row(gpu, monkeypatch, hd, type, n_head, n_kv, q_off, kv_off, window):
+    """Two inputs in turn through one workspace, nothing waited for between the calls: every result is its input's first
+    one bit for bit, and that one within the bound of 64 bits."""
+    import torch
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", "1")
+    rng = np.random.default_rng(hd + type)
+    ko = q_off if kv_off is None else kv_off
+    qo, kvo = t(np.array(q_off, np.int32)), t(np.array(ko, np.int32))
+    data = [inputs(rng, q_off[-1], ko[-1], n_head, n_kv, hd, type) for _ in range(2)]
+    on_gpu = [[t(x) for x in d] for d in data]
+
+    def call(i, out):
+        q, k, v = on_gpu[i]
+        p = gl.AttnPromptParams(type=type, n_head=n_head, n_kv_head=n_kv, head_dim=hd, q=q.data_ptr(), ldq=n_head * hd,
+                                k=k.data_ptr(), ldk=n_kv * hd, v=v.data_ptr(), ldv=n_kv * hd, out=out.data_ptr(), ldo=n_head * hd,
+                                n_rows=q_off[-1], n_kv_rows=ko[-1], n_seq=len(q_off) - 1, q_off=qo.data_ptr(),
+                                kv_off=kvo.data_ptr(), window=window)
+        gpu.check(gpu.lib.ggq_attention_prompt_dev(gpu.h, p, stream_handle()), "prompt attention")
+
+    outs = [torch.zeros((q_off[-1], n_head * hd), device="cuda") for _ in range(24)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        call(i % 2, out)
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert torch.equal(out, outs[i % 2]), i
+    for i in (0, 1):
+        q, k, v = data[i]
+        got = host(outs[i])
+        for s in range(len(q_off) - 1):
+            n, m = q_off[s + 1] - q_off[s], ko[s + 1] - ko[s]
+            kk, vv = (x[ko[s]:ko[s + 1]].reshape(m, n_kv, hd) for x in (k, v))
+            for r in {0, n // 3, n // 2, n - 1}:
+                want, tol = au.attention(q[q_off[s] + r].reshape(1, n_head, hd), kk, vv, m - n + r, window)
+                au.check(got[q_off[s] + r].reshape(1, n_head, hd), want, tol)
