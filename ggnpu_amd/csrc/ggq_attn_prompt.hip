@@ -84,6 +84,9 @@ __device__ __forceinline__ Span span_of(const int32_t* off, int s, int64_t most)
     const int64_t a = min(max((int64_t)off[s], (int64_t)0), most), b = min(max((int64_t)off[s + 1], (int64_t)0), most);
     return Span{a, b > a ? b - a : 0};
 }
+// The first position that a row with `below` positions at or before its own sees (below < 1: none are).  A window
+// may be anything up to INT32_MAX: nothing is subtracted from a negative number.
+__device__ __forceinline__ int first_of(int below, int window) { return window ? max(max(below, 0) - window, 0) : 0; }
 __device__ __forceinline__ const int32_t* kv_off_of(const ggq_attention_prompt_params& p) { return p.kv_off ? p.kv_off : p.q_off; }
 
 __device__ __forceinline__ uint32_t mag_bits(float v) {  // 0 for what is not finite
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(PromptArgs a) {
     for (int c = 0; c < C; c++) {
         const int qi = (int)((uint32_t)min(f0 + c, nf - 1) / G);
         end[c] = min(max(shift + qi, 0), n_keys);
-        beg[c] = p.window ? min(max(shift + qi - p.window, 0), n_keys) : 0;
+        beg[c] = min(first_of(shift + qi, p.window), n_keys);
         first = min(first, beg[c]);
         last = max(last, end[c]);
         none = max(none, beg[c]);  // every column sees [none, all)
@@ -412,7 +415,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     const int n_keys = (int)ks.n, shift = n_keys - (int)qs.n + 1;  // row i sees positions below shift + i
     const int i0 = (int)((uint32_t)f0 / G), i1 = (int)((uint32_t)(min(nf, f0 + NC) - 1) / G);
     const int wg_end = min(max(shift + i1, 0), n_keys);
-    const int wg_beg = p.window ? max(shift + i0 - p.window, 0) : 0;
+    const int wg_beg = first_of(shift + i0, p.window);
     const int all0 = wg_beg / kUnit, all1 = (wg_end + kUnit - 1) / kUnit;
     const int per = (max(all1 - all0, 0) + a.splits - 1) / a.splits;
     const int u0 = all0 + split * per, u1 = min(all1, u0 + per), n = u1 - u0;
@@ -449,14 +452,14 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     const int qi = live ? (int)((uint32_t)f / G) : i1;
     const int head = kvh * G + (live ? f - qi * G : 0);
     const int end = live ? min(max(shift + qi, 0), n_keys) : 0;
-    const int beg = live && p.window ? max(shift + qi - p.window, 0) : 0;
+    const int beg = live ? first_of(shift + qi, p.window) : 0;
     // rows ascend with the columns: the first and the last live one bound what the wavefront sees
     const int fl = f0 + wave * 32, last = min(fl + 31, nf - 1);
     const bool any = fl < nf, full = fl + 31 < nf;
     const int ra = any ? (int)((uint32_t)fl / G) : 0, rb = any ? (int)((uint32_t)last / G) : 0;
-    const int wend = any ? min(max(shift + rb, 0), n_keys) : 0, wbeg = p.window ? max(shift + ra - p.window, 0) : 0;
+    const int wend = any ? min(max(shift + rb, 0), n_keys) : 0, wbeg = first_of(shift + ra, p.window);
     const int fend = full ? min(max(shift + ra, 0), n_keys) : 0;  // (with columns that are no rows: masked throughout)
-    const int fbeg = p.window ? max(shift + rb - p.window, 0) : 0;
+    const int fbeg = first_of(shift + rb, p.window);
 
     h2 minus1 = {(_Float16)-1.0f, (_Float16)-1.0f};
     asm volatile("" : "+v"(minus1));

@@ -1,12 +1,12 @@
 """Prompt attention where it could go wrong unseen: calls that follow each other without a wait, against themselves and
-against 64 bits."""
+against 64 bits; windows of any size, on the route of the rule and on both routes."""
 import numpy as np
 import pytest
 
 import ggnpu_amd.lib as gl
 from tests import attn_util as au
 from tests.gpu_util import host, stream_handle
-from tests.test_gpu_attn_prompt import inputs, t
+from tests.test_gpu_attn_prompt import inputs, run, t
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +18,12 @@ def gpu():
     c = gl.Context(0)
     yield c
     c.close()
+
+
+@pytest.fixture(params=["", "0", "1"], ids=["rule", "valu", "mfma"])
+def ctx(gpu, request, monkeypatch):
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", request.param)
+    return gpu
 
 
 @pytest.mark.parametrize("hd", [64, 128, 256])
@@ -65,3 +71,18 @@ def test_prompt_calls_in_a_row(gpu, monkeypatch, hd, type, n_head, n_kv, q_off, 
             for r in {0, n // 3, n // 2, n - 1}:
                 want, tol = au.attention(q[q_off[s] + r].reshape(1, n_head, hd), kk, vv, m - n + r, window)
                 au.check(got[q_off[s] + r].reshape(1, n_head, hd), want, tol)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 8])
+def test_prompt_windows_of_any_size(ctx, window):
+    """A window far above every length is none, also where the first rows come before all keys."""
+    run(ctx, 40, [0, 20], [0, 7], 4, 2, 64, window=window)
+    run(ctx, 41, [0, 30, 50, 53], [0, 5, 25, 90], 3, 1, 128, 1, window=window)
+    run(ctx, 42, [0, 1010], [0, 1000], 4, 1, 64, window=window, rows=[0, 8, 9, 10, 11, 500, 1009])
+    run(ctx, 43, [0, 300], [0, 200], 4, 2, 256, window=window, rows=[0, 98, 99, 100, 101, 131, 132, 299])
+
+
+@pytest.mark.parametrize("window", [1, 33])
+def test_prompt_windows_and_rows_that_see_nothing(ctx, window):
+    run(ctx, 46, [0, 90, 100, 140], [0, 50, 50, 200], 4, 2, 64, window=window)
+    run(ctx, 47, [0, 90], [0, 50], 3, 1, 256, 1, window=window)
