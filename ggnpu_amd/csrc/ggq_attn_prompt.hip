@@ -62,6 +62,8 @@ template <> struct Head<256> {
 };
 // Bytes of a unit: header, K and V planes.
 template <int HD> constexpr int64_t unit_bytes(int planes) { return (int64_t)planes * 2 * kUnit * HD * 2 + Head<HD>::bytes; }
+// Exponents between that of an all-zero row of values and its unit's (an int16_t with the sign changed).
+constexpr int kZero = 4096;
 enum { BAD_V = 1 << 20, NO_V = 1 << 21, OWN_K = 1 << 22, OWN_V = 1 << 23 };
 
 // Sequence s has the units from off[s] / 32 + s on (and as many column tiles of
@@ -307,6 +309,9 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
     int ke = P == 2 && mk ? up_to_2_15(mk) : ku, ve = P == 2 && mv ? up_to_2_15(mv) : vu;
     if (ke <= ku + 8) ke = ku;
     if (ve <= vu + 8) ve = vu;
+    // values that are all zero have any exponent: one that stands for no value (of a unit with others: hidden ones
+    // must not lend it theirs)
+    if (P == 2 && in && !mv && uv) ve = vu + kZero;
     const int own_k = __syncthreads_or(ke != ku), own_v = __syncthreads_or(ve != vu);
     typedef typename Head<HD>::num num;
     uint8_t* out = a.planes + (id * a.kvn + (kvh - a.kv0)) * unit_bytes<HD>(P);
@@ -555,7 +560,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         const bool masked = masks(it);
         const int ku = (int)(info & 1023u) - 512, vu = (int)(info >> 10 & 1023u) - 512;
         bad |= info;
-        int vmin = vu;  // of the values that the column sees
+        int vmin = vu;  // of the values that the column sees (above kZero / 2: zeros only, or nothing)
         if (masked) {
             int most = -kNone;
 #pragma unroll
@@ -585,7 +590,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         if constexpr (P == 2) {
             // the sums follow the values' unit when those get larger, or smaller by more than
             // 2^8 (but stay within 2^64 of the largest so far); less than that, weights shrink
-            const bool some = !(info & NO_V) && vmin < kNone / 2;
+            const bool some = !(info & NO_V) && vmin < kZero / 2;  // (exponents of values are within 2^9)
             const bool first = least == kNone;
             least = some ? min(least, vmin) : least;
             const int to = some && (first || vmin < ve || vmin > ve + 8) ? min(vmin, least + 64) : ve;

@@ -1,12 +1,13 @@
 """Prompt attention where it could go wrong unseen: calls that follow each other without a wait, against themselves and
-against 64 bits; windows of any size, on the route of the rule and on both routes."""
+against 64 bits; windows of any size, values and keys of any size that a row does not see, on the route of the rule and on both
+routes."""
 import numpy as np
 import pytest
 
 import ggnpu_amd.lib as gl
 from tests import attn_util as au
 from tests.gpu_util import host, stream_handle
-from tests.test_gpu_attn_prompt import inputs, run, t
+from tests.test_gpu_attn_prompt import call as attend, inputs, run, t
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,25 @@ def test_prompt_windows_of_any_size(ctx, window):
 def test_prompt_windows_and_rows_that_see_nothing(ctx, window):
     run(ctx, 46, [0, 90, 100, 140], [0, 50, 50, 200], 4, 2, 64, window=window)
     run(ctx, 47, [0, 90], [0, 50], 3, 1, 256, 1, window=window)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_unseen_values_beside_zero_rows(ctx, hd):
+    """Value rows of zeros among the seen ones, values of any size among the unseen ones of the same 32 positions."""
+    rng = np.random.default_rng(44)
+    n, n_head, n_kv = 100, 4, 2
+    q, k, v = inputs(rng, n, n, n_head, n_kv, hd)
+    v[[0, 40, 95]] = 0
+    v[64:70] = 0  # rows 64 .. 69 see nothing but zeros of their last 32 positions
+    for bad in (1e4, 1e6, 1e12, -3e38):
+        v2 = v.copy()
+        v2[[59, 70, 99], ::5] = bad
+        got = attend(ctx, q, k, v2, n_head, n_kv, hd, 0, [0, n], [0, n])
+        for i in (0, 1, 31, 32, 40, 41, 58):
+            want, tol = au.attention(q[i:i + 1].reshape(1, n_head, hd), k.reshape(n, n_kv, hd), v.reshape(n, n_kv, hd), i)
+            au.check(got[i:i + 1].reshape(1, n_head, hd), want, tol)
+        # a window whose rows see the large value no more: positions 60 .. 69 for row 69, among them six rows of zeros
+        got = attend(ctx, q, k, v2, n_head, n_kv, hd, 0, [0, n], [0, n], window=10)
+        for i in (58, 69, 82, 97):
+            want, tol = au.attention(q[i:i + 1].reshape(1, n_head, hd), k.reshape(n, n_kv, hd), v.reshape(n, n_kv, hd), i, 10)
+            au.check(got[i:i + 1].reshape(1, n_head, hd), want, tol)
