@@ -545,11 +545,12 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         const uint8_t* slot = lds + (it & 1) * KB;
         // (the slot is loaded over before the weights of the wavefronts behind)
         if constexpr (P == 2) {
-            if (info & OWN_K) {
+            if (info & OWN_K) {  // (scores in one step: the unit's exponent may be that of hidden keys, far from the seen ones')
+                const int ku = (int)(info & 1023u) - 512;
                 int dk[16];
                 numbers(slot, dk);
 #pragma unroll
-                for (int i = 0; i < 16; i++) st[i] = ldexpf(st[i], dk[i]);
+                for (int i = 0; i < 16; i++) st[i] = ldexpf(st[i], dk[i] - ku - qe);
             }
             if (info & OWN_V) numbers(slot + 32 * sizeof(num), dv);
         }
@@ -572,8 +573,9 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             }
             if constexpr (P == 2) vmin = vu - max(most, __shfl_xor(most, 32, 64));
         }
-        // to powers of two (an exponent beyond fp32's range gives a score of 0 or an infinite one either way)
-        const float cs = ldexpf(1.0f, max(-126, min(127, -(qe + ku))));
+        // to powers of two, where powers() has not (an exponent beyond fp32's range gives a score of 0 or an infinite one
+        // either way)
+        const float cs = P == 2 && (info & OWN_K) ? 1.0f : ldexpf(1.0f, max(-126, min(127, -(qe + ku))));
         float top = max3(st[0], st[1], st[2]);
 #pragma unroll
         for (int i = 3; i < 15; i += 2) top = max3(top, st[i], st[i + 1]);

@@ -109,3 +109,20 @@ def test_prompt_unseen_values_beside_zero_rows(ctx, hd):
         for i in (58, 69, 82, 97):
             want, tol = au.attention(q[i:i + 1].reshape(1, n_head, hd), k.reshape(n, n_kv, hd), v.reshape(n, n_kv, hd), i, 10)
             au.check(got[i:i + 1].reshape(1, n_head, hd), want, tol)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_unseen_keys_beside_small_ones(ctx, hd):
+    """Small keys under large queries, keys of any size among the unseen ones of the same 32 positions."""
+    rng = np.random.default_rng(45)
+    n, n_head, n_kv = 100, 4, 2
+    q, k, v = inputs(rng, n, n, n_head, n_kv, hd)
+    for size in (1.0, 1e10, 1e18):
+        qs, ks = (q * np.float32(size)).astype(np.float32), (k * np.float32(1 / size)).astype(np.float32)
+        for bad in (1e6, 1e20, -3e38):
+            k2 = ks.copy()
+            k2[59:, ::7] = bad
+            got = attend(ctx, qs, k2, v, n_head, n_kv, hd, 0, [0, n], [0, n])
+            for i in (0, 31, 32, 45, 58):
+                want, tol = au.attention(qs[i:i + 1].reshape(1, n_head, hd), ks.reshape(n, n_kv, hd), v.reshape(n, n_kv, hd), i)
+                au.check(got[i:i + 1].reshape(1, n_head, hd), want, tol)
