@@ -23,8 +23,9 @@
 //   The maximum moves only when a unit exceeds it by 2^4; weights are kept times
 // 2^11 (at most 2^15), so hi + lo of a small weight keeps 2^-35 of the largest.
 // Scores take their position's power of two back; weights take the values', relative to
-// the largest that their row has seen, whose unit the row's running sums are in: a
-// position that a row does not see has no say in what the row keeps of the others.
+// the unit of the row's running sums, which follows the largest product of weight and value
+// that the row has seen: neither a position that it does not see nor one of next to no
+// weight has a say in what it keeps of the others.
 // Bound: the matrix cores, at the clock that their load leaves (8191 rows of 32
 // heads of 128 in fp32: 1.37 ms, 1.2 PFLOP/s of fp16 products, what the
 // library's matmul reaches; a unit 5100 cycles, three fifths of them products).
@@ -496,7 +497,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
 #pragma unroll
     for (int d = 0; d < DB; d++) o[d] = f16v{};
     float m = -INFINITY, l = 0.0f;
-    // the column's sums are in units of 2^-ve; the least exponent of the values it saw
+    // the column's sums are in units of 2^-ve; `least`: the unit in which what they hold would be at its limit
     constexpr int kNone = 1 << 20;
     int ve = 0, least = kNone;
     uint32_t info = 0, bad = 0;
@@ -561,17 +562,12 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         const bool masked = masks(it);
         const int ku = (int)(info & 1023u) - 512, vu = (int)(info >> 10 & 1023u) - 512;
         bad |= info;
-        int vmin = vu;  // of the values that the column sees (above kZero / 2: zeros only, or nothing)
         if (masked) {
-            int most = -kNone;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int at = base + 8 * (i / 4) + 4 * h + i % 4;
-                const bool out = at >= end || at < beg;
-                if (out) st[i] = -INFINITY;
-                if constexpr (P == 2) most = max(most, out ? -kNone : info & OWN_V ? dv[i] : 0);
+                if (at >= end || at < beg) st[i] = -INFINITY;
             }
-            if constexpr (P == 2) vmin = vu - max(most, __shfl_xor(most, 32, 64));
         }
         // to powers of two, where powers() has not (an exponent beyond fp32's range gives a score of 0 or an infinite one
         // either way)
@@ -584,18 +580,35 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         if (__any(top > m + 4.0f)) {
             const float mn = max3(m, top, top);
             const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            if (P == 2 && m > -INFINITY) least = min(least + (int)fminf(mn - m, 4096.0f), kNone);  // (so much do the sums shrink)
             m = mn;
             l *= al;
 #pragma unroll
             for (int d = 0; d < DB; d++) o[d] *= al;
         }
+        // the weights' power of two besides 2^(11 - m)
+        int c = 0;
         if constexpr (P == 2) {
-            // the sums follow the values' unit when those get larger, or smaller by more than
-            // 2^8 (but stay within 2^64 of the largest so far); less than that, weights shrink
-            const bool some = !(info & NO_V) && vmin < kZero / 2;  // (exponents of values are within 2^9)
-            const bool first = least == kNone;
-            least = some ? min(least, vmin) : least;
-            const int to = some && (first || vmin < ve || vmin > ve + 8) ? min(vmin, least + 64) : ve;
+            // In the sums' unit a position's weight times value is 2^(s - m + ve - its exponent): `heavy` is the largest
+            // s - m - (exponent - vu) that the column sees, `roof` the ve up to which its weight stays within 2^15.
+            float heavy = top - m;
+            if (info & OWN_V) {
+                heavy = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; i++) heavy = fmaxf(heavy, fmaf(st[i], cs, (float)dv[i]));
+                const Two x = halves(heavy);
+                heavy = fmaxf(x.a, x.b) - m;
+            }
+            // (below: zeros only, nothing, or weights that are)
+            const bool some = !(info & NO_V) && heavy > -kZero / 2;
+            const int roof = vu + 4 - (int)ceilf(fmaxf(heavy, -(float)kZero));
+            // The sums move to a smaller unit when weights would pass 2^15, to a larger one when what there is to add
+            // (for values of one size: the values) gets smaller by more than 2^8, but stay within 2^64 of the largest that
+            // they hold; less than that, weights shrink.
+            const bool first = least >= kNone;
+            least = some ? min(least, roof) : least;
+            const int up = info & OWN_V ? roof - 4 : vu;
+            const int to = !some ? ve : first ? up : roof < ve ? roof - 4 : up > ve + 8 ? min(up, least + 64) : ve;
             if (__any(to != ve)) {
 #pragma unroll
                 for (int d = 0; d < DB; d++)
@@ -603,10 +616,9 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
                     for (int i = 0; i < 16; i++) o[d][i] = ldexpf(o[d][i], to - ve);
                 ve = to;
             }
+            // (below 2^-100 weights are nothing)
+            c = some && !(info & OWN_V) ? max(ve - vu, -100) : 0;
         }
-        // the weights in the sums' unit (at most the values': ve <= vu for what the column sees;
-        // below 2^-100 of it they are nothing)
-        const int c = P == 2 ? max(min(ve - vu, 0), -100) : 0;
         const float ref = m == -INFINITY ? 0.0f : m - 11.0f - (float)c;
         float e[16], sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -618,7 +630,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         if constexpr (P == 2) {
             if (info & OWN_V) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) e[i] = ldexpf(e[i], dv[i] + (ve - vu - c));
+                for (int i = 0; i < 16; i++) e[i] = ldexpf(e[i], dv[i] + (ve - vu));
             }
         }
 #pragma unroll

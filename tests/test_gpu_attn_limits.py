@@ -126,3 +126,42 @@ def test_prompt_unseen_keys_beside_small_ones(ctx, hd):
             for i in (0, 31, 32, 45, 58):
                 want, tol = au.attention(qs[i:i + 1].reshape(1, n_head, hd), ks.reshape(n, n_kv, hd), v.reshape(n, n_kv, hd), i)
                 au.check(got[i:i + 1].reshape(1, n_head, hd), want, tol)
+
+
+def weighted(q, k, v, scale, floor):
+    """fp64 attention of one row over all of k, v (one head) and the bound of each value: the score of a position is off by
+    (hd / 4 + 8) roundings of its own sum of magnitudes, which its weight and the sum of weights take over; the sum over positions
+    adds 32 + n / 16 roundings of its magnitudes; a weight is off by `floor` of the largest at most besides."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    s = k @ q * scale
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    ds = au.U32 * (k.shape[1] / 4 + 8) * (np.abs(k) @ np.abs(q)) * scale
+    out = p @ v
+    return out, (p * (ds + au.U32 * (32 + len(k) / 16))) @ np.abs(v) + p @ ds * np.abs(out) + floor * np.abs(v).sum(0) + 1e-37
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("type", [0, 1])
+@pytest.mark.parametrize("where", [[0], [5], [40], [98], range(0, 32), range(32, 64), range(64, 96), [3, 31, 32, 60, 64, 90],
+                                   [*range(0, 32), 40, 70, 96]])
+def test_prompt_large_values_of_little_weight(ctx, hd, type, where):
+    """Values of up to 2^100 (fp16: 2^12 beside 2^-6) that a row sees with a weight of next to nothing, before, among and
+    behind the ones that make its result."""
+    rng = np.random.default_rng(hd + len(where) + where[0])
+    n, n_head = 100, 2
+    u = rng.standard_normal(hd)
+    u *= np.sqrt(hd) / np.linalg.norm(u)
+    q = (np.tile(u, (n, n_head)) * (1 + 0.1 * rng.random((n, 1)))).astype(np.float32)
+    for bits, nats in ((14, 12), (18, 14), (18, 30)) if type else ((20, 15), (24, 25), (40, 40), (70, 55), (100, 80)):
+        k = 0.3 * rng.standard_normal((n, hd))
+        v = rng.standard_normal((n, hd)) * (2.0 ** -6 if type else 1.0)
+        for i in where:
+            k[i] = -u / np.sqrt(hd) * nats
+            v[i] *= 2.0 ** bits
+        k, v = (x.astype(np.float16 if type else np.float32) for x in (k, v))
+        got = attend(ctx, q, k, v, n_head, 1, hd, type, [0, n], [0, n])
+        for i in (33, 63, 64, 97, 99):
+            want, tol = weighted(q[i, :hd], k[:i + 1], v[:i + 1], hd ** -0.5, 2.0 ** -36 if type else 0.0)
+            for h in range(n_head):
+                au.check(got[i, h * hd:(h + 1) * hd], want, tol)
