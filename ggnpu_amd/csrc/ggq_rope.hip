@@ -10,7 +10,8 @@
 //
 // The angle of pair i at position p is p * turns_i turns.  The product is taken
 // in 64 bits and its whole turns are dropped there, so the 32-bit sine and
-// cosine see an angle within half a turn at any position.  A lane's pairs
+// cosine see an angle within half a turn at any position; what that loses of the
+// angle (up to 2^-25 of half a turn) is put back along the tangent.  A lane's pairs
 // are the same for all heads of a row: they are made once and used for
 // `passes` groups of heads.
 //
@@ -42,11 +43,12 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int heads, int pa
         const double p = (double)a.pos[t];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const double turn = p * a.turns[4 * u + j];
+            const double turn = p * a.turns[4 * u + j], half = 2.0 * (turn - rint(turn));
+            const float at = (float)half, rest = (float)((half - (double)at) * 3.14159265358979323846);
             float s, c;
-            sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
-            cs[j] = c * a.mag;
-            sn[j] = s * a.mag;
+            sincospif(at, &s, &c);
+            cs[j] = fmaf(-s, rest, c) * a.mag;
+            sn[j] = fmaf(c, rest, s) * a.mag;
         }
     }
     const int n0 = a.set[0].n_head;
