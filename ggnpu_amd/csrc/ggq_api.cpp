@@ -110,6 +110,7 @@ struct ggq_ctx {
     Buffer aside;                // memory for captures, its first aside_used bytes in use
     size_t aside_used = 0, aside_total = 0;  // (total: outgrown allocations too)
     size_t lane_need = 0;        // the largest buffer an eager call asked for
+    size_t aside_need = 0;       // what memory for captures is sized by, lane_need or more
     size_t aside_refused = SIZE_MAX;  // memory for captures that could not be had
     Buffer io;  // staging of host A / C for the synchronous entry points
     Buffer logits;  // vocab projection output when the caller does not keep it
@@ -185,12 +186,14 @@ void* alloc_beside_captures(size_t bytes) {
     return nullptr;
 }
 
-// Bytes to allocate so that at least `bytes` are set aside for captures, with
-// room for `copies` of them; 0 when they are, or when the bound does not allow it.
-size_t aside_short(const ggq_ctx* c, size_t bytes, size_t copies) {
-    if (c->aside.size - c->aside_used >= bytes || !bytes) return 0;
+// Bytes to allocate so that at least `least` times `bytes` are set aside for captures,
+// with room for `copies` times; 0 when they are, or when the bound allows no more than there is.
+size_t aside_short(const ggq_ctx* c, size_t bytes, size_t copies, size_t least = 1) {
+    const size_t left = c->aside.size - c->aside_used;
+    if (!bytes || left >= bytes * least) return 0;
     bytes = align256(bytes);
-    return bytes * std::min(copies, (kCaptureBytes - c->aside_total) / bytes);
+    const size_t n = bytes * std::min(copies, (kCaptureBytes - c->aside_total) / bytes);
+    return n > left ? n : 0;
 }
 void set_aside(ggq_ctx* c, void* p, size_t bytes) {
     c->aside = Buffer{p, bytes};
@@ -224,8 +227,12 @@ struct Want {
 // for it).
 bool grow_lane(ggq_ctx* c, Buffer& b, size_t bytes, const Want* wants, int n_wants) {
     c->lane_need = std::max(c->lane_need, bytes);
-    // for eight captures in a row, two where that would be more than 256 MB
-    size_t aside = aside_short(c, c->lane_need, std::min<size_t>(8, std::max<size_t>(2, (size_t(256) << 20) / c->lane_need)));
+    // for eight captures in a row, two where that would be more than 256 MB: all of them when calls get larger
+    // (by twice then, so that calls that get larger one by one seldom allocate), one between captures
+    const bool larger = c->lane_need > c->aside_need;
+    if (larger) c->aside_need = std::max(c->lane_need, 2 * c->aside_need);
+    const size_t copies = std::min<size_t>(8, std::max<size_t>(2, (size_t(256) << 20) / c->aside_need));
+    size_t aside = larger ? aside_short(c, c->aside_need, copies, copies) : aside_short(c, c->lane_need, copies);
     if (aside >= c->aside_refused) aside = 0;  // not tried on each call anew
     const size_t lane = Want{&b, bytes}.grown();
     size_t spare = 0;
