@@ -1,12 +1,16 @@
-"""The attention operators where calls could meet: captured and eager calls that need workspace in flight together."""
+"""The attention operators where calls could meet: captured and eager calls that need workspace in flight together, threads of
+one context; and 256-wide prompts, whose units, wavefronts and schedule are their own, in parts, chunks, windows, captures
+and groups of heads."""
+import threading
+
 import numpy as np
 import pytest
 
 import ggnpu_amd.lib as gl
 from tests import attn_util as au
 from tests.gpu_util import host
-from tests.test_gpu_attn_prompt import t
-from tests.test_gpu_attn_together import Layer, _buffers, stream
+from tests.test_gpu_attn_prompt import run, t
+from tests.test_gpu_attn_together import Layer, _buffers, _token_step, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +86,112 @@ def test_graphs_and_streams_with_planes_and_parts(ctx, monkeypatch, hd):
         torch.cuda.synchronize()
         for i in range(4):
             assert torch.equal(bufs[i]["out"], want[i][0]) and torch.equal(prompts[i][3], want[i][1]), i
+
+
+def test_threads_with_planes_and_parts(ctx, monkeypatch):
+    """Threads of one context, each on its stream, whose calls all take workspace."""
+    import torch
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", "1")
+    monkeypatch.setenv("GGQ_KV_SPLITS", "7")
+    gen = _generator(51)
+    lays = [Layer(ctx, 2, 2, 1024, 8, 2, 128, 4, 4, seed=i) for i in range(3)]
+    data, prompts, want, errs = [], [], [], []
+    for i, x in enumerate(lays):
+        x.len.copy_(t(np.array([1500, 41 + i], np.int32)))
+        k, v = (torch.randn((1541 + i, 2, 128), device="cuda", generator=gen) for _ in range(2))
+        b = _buffers(x, 2, 30 + i)
+        x.store(k, v, t(np.array([0, 1500, 1541 + i], np.int32)), stream())
+        p = _prompt_of(x, 300 + 60 * i, gen)
+        _token_step(x, b, stream())
+        x.prompt(*p[:4], p[4], p[4], stream())
+        torch.cuda.synchronize()
+        want.append((b["out"].clone(), p[3].clone()))
+        data.append(b)
+        prompts.append(p)
+
+    def go(i):
+        try:
+            s = torch.cuda.Stream()
+            for _ in range(20):
+                p = prompts[i]
+                lays[i].prompt(*p[:4], p[4], p[4], s.cuda_stream)
+                _token_step(lays[i], data[i], s.cuda_stream)
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errs.append(e)
+    torch.cuda.synchronize()
+    ts = [threading.Thread(target=go, args=(i,)) for i in range(3)]
+    for x in ts:
+        x.start()
+    for x in ts:
+        x.join()
+    assert not errs
+    for b, p, (a, c) in zip(data, prompts, want):
+        assert torch.equal(b["out"], a) and torch.equal(p[3], c)
+
+
+@pytest.fixture(params=["", "1"], ids=["rule", "mfma"])
+def route(request, monkeypatch):
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", request.param)
+
+
+@pytest.mark.parametrize("type", [0, 1])
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 65, 127, 129, 300])
+def test_wide_heads_lengths(ctx, route, n, type):
+    run(ctx, n, [0, n], None, 3, 1, 256, type, rows=[0, n // 2, n - 2, n - 1] if n > 2 else None)
+
+
+@pytest.mark.parametrize("type", [0, 1])
+@pytest.mark.parametrize("window", [0, 1, 33, 64, 200])
+def test_wide_heads_windows_and_chunks(ctx, route, window, type):
+    run(ctx, window, [0, 40, 41, 60, 63], [0, 300, 417, 427, 427], 8, 2, 256, type, window=window, rows=[0, 9, 10, 18, 39])
+    run(ctx, window + 1, [3, 20, 145], [5, 22, 190], 2, 2, 256, type, window=window, behind=2, pad=8, rows=[0, 16, 70, 124])
+
+
+@pytest.mark.parametrize("splits", ["1", "2", "5", "1000"])
+@pytest.mark.parametrize("type", [0, 1])
+def test_wide_heads_parts(ctx, monkeypatch, splits, type):
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", "1")
+    monkeypatch.setenv("GGQ_PROMPT_SPLITS", splits)
+    run(ctx, 30, [0, 40, 41, 41, 60], [0, 300, 700, 710, 729], 6, 2, 256, type, behind=3, rows=[0, 18, 39])
+    run(ctx, 31, [2, 90], [0, 260], 4, 1, 256, type, window=100, rows=[0, 50, 87])
+
+
+@pytest.mark.parametrize("splits", ["1", "3"])
+def test_wide_heads_in_groups(ctx, monkeypatch, splits):
+    """More than 256 MB of planes: the kv heads go in groups of six."""
+    monkeypatch.setenv("GGQ_PROMPT_SPLITS", splits)
+    run(ctx, 52, [0, 3], [0, 20011], 8, 8, 256, 0, rows=[0, 2])
+
+
+@pytest.mark.parametrize("type", [0, 1])
+def test_wide_heads_captured(ctx, monkeypatch, type):
+    """Captured once; inputs and offsets change between the replays, and each equals the eager call bit for bit."""
+    import torch
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", "1")
+    gen = _generator(53)
+    lay = Layer(ctx, 1, 1, 32, 8, 2, 256, 4, 4)
+    rows = 300
+    q, k, v, out, off = _prompt_of(lay, rows, gen)
+    if type:
+        k, v = k.half(), v.half()
+    ref = torch.empty_like(out)
+    lay.prompt(q, k, v, ref, off, off, stream(), type)
+    torch.cuda.synchronize()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        lay.prompt(q, k, v, out, off, off, s.cuda_stream, type)
+    for i in range(5):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device="cuda", generator=gen))
+        off.copy_(t(np.array([0, 1 + 7 * i, rows - i], np.int32)))
+        out.zero_()
+        ref.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        lay.prompt(q, k, v, ref, off, off, stream(), type)
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref), i
+        r = 1 + 7 * i
+        w, tol = au.attention(host(q)[r:r + 1], host(k)[r:], host(v)[r:], 0)
+        au.check(host(out)[r:r + 1], w, tol)
