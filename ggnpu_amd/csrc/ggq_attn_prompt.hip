@@ -523,24 +523,14 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     auto open = [&](int it) { info = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(lds + (it & 1) * KB + Head<HD>::info)); };
     auto scores = [&](int it) {
         const h8* kp = (const h8*)(lds + (it & 1) * KB + HB) + lane;
-        // two sums in turn where no other wavefront fills the wait of a product for the one before it
-        // (256-wide heads, 2048 rows: 238 -> 221 us; 128-wide ones do without: 166 -> 170)
-        constexpr int NA = NW == 8 ? 1 : 2;
-        f16v sa[NA] = {};
-        int turn = 0;
-        auto add = [&](h8 x, h8 y) {
-            sa[turn % NA] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, sa[turn % NA], 0, 0, 0);
-            turn++;
-        };
+        st = f16v{};
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const h8 kh = kp[s * 64];
-            add(kh, qh[s]);
-            add(kh, ql[s]);
-            if constexpr (P == 2) add(kp[s * 64 + PL / 16], qh[s]);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[s], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[s], st, 0, 0, 0);
+            if constexpr (P == 2) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kp[s * 64 + PL / 16], qh[s], st, 0, 0, 0);
         }
-        st = sa[0];
-        if constexpr (NA == 2) st += sa[1];
     };
     auto powers = [&](int it) {
         const uint8_t* slot = lds + (it & 1) * KB;
