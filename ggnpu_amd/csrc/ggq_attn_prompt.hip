@@ -523,14 +523,15 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     auto open = [&](int it) { info = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(lds + (it & 1) * KB + Head<HD>::info)); };
     auto scores = [&](int it) {
         const h8* kp = (const h8*)(lds + (it & 1) * KB + HB) + lane;
+        // the small products first: the hi hi ones alone round at the size of the sum (head_dim / 16 of them)
         st = f16v{};
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            const h8 kh = kp[s * 64];
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[s], st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[s], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kp[s * 64], ql[s], st, 0, 0, 0);
             if constexpr (P == 2) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kp[s * 64 + PL / 16], qh[s], st, 0, 0, 0);
         }
+#pragma unroll
+        for (int s = 0; s < KS; s++) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kp[s * 64], qh[s], st, 0, 0, 0);
     };
     auto powers = [&](int it) {
         const uint8_t* slot = lds + (it & 1) * KB;

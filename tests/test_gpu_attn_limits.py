@@ -165,3 +165,26 @@ def test_prompt_large_values_of_little_weight(ctx, hd, type, where):
             want, tol = weighted(q[i, :hd], k[:i + 1], v[:i + 1], hd ** -0.5, 2.0 ** -36 if type else 0.0)
             for h in range(n_head):
                 au.check(got[i, h * hd:(h + 1) * hd], want, tol)
+
+
+@pytest.mark.parametrize("hd,bound", [(64, 3.3e-6), (128, 4.1e-6), (256, 5.5e-6)])
+def test_prompt_scores_add_small_products_first(gpu, monkeypatch, hd, bound):
+    """Scores of 44 whose products all have one sign, told from the weights of two keys.  The products of the fp16 parts
+    are added 16 values a step: with the small ones first, only the hd / 16 steps of hi times hi round at the size of the
+    sum.  Emulated in 64 bits with a rounding to fp32 a step (two, if the step adds in halves), the difference of two scores
+    is then off by 2.3 (2.8), 2.7 (3.6) and 3.5 (4.8) e-6, root mean square, and by 3.7, 4.7 and 6.2 e-6 at the least with
+    hi times hi in between."""
+    monkeypatch.setenv("GGQ_PROMPT_MFMA", "1")
+    rng = np.random.default_rng(55)
+    n, heads = 512, 8
+    c = 44 * hd ** -0.5
+    q = (1 + 0.2 * rng.standard_normal((n, heads * hd))).astype(np.float32)
+    k = (c * (1 + 0.2 * rng.standard_normal((2 * n, heads * hd)))).astype(np.float32)
+    v = np.zeros((2 * n, heads * hd), np.float32)
+    v[0::2] = 1
+    got = attend(gpu, q, k, v, heads, heads, hd, 0, np.arange(n + 1), 2 * np.arange(n + 1)).reshape(n, heads, hd)[..., 0].astype(np.float64)
+    s = (k.reshape(n, 2, heads, hd).astype(np.float64) * q.reshape(n, 1, heads, hd)).sum(-1) * hd ** -0.5
+    d = s[:, 0] - s[:, 1]
+    assert 40 < s.mean() < 48 and np.abs(d).max() < 6
+    err = np.log(got / (1 - got)) - d
+    assert np.sqrt((err ** 2).mean()) <= bound
