@@ -195,3 +195,68 @@ def test_wide_heads_captured(ctx, monkeypatch, type):
         r = 1 + 7 * i
         w, tol = au.attention(host(q)[r:r + 1], host(k)[r:], host(v)[r:], 0)
         au.check(host(out)[r:r + 1], w, tol)
+
+
+def _cache(ctx, n_pages, page_len, n_kv, hd, kt, vt, table, lens, max_len):
+    import ctypes
+
+    import torch
+    size = ctx.lib.ggq_kv_page_bytes(ctypes.byref(gl.KvCache(None, 0, page_len, n_kv, hd, kt, vt)))
+    mem = torch.full((n_pages, size), 0x22, dtype=torch.uint8, device="cuda")
+    tab, ln = t(np.asarray(table, np.int32)), t(np.asarray(lens, np.int32))
+    keep = (mem, tab, ln)
+    return (gl.KvCache(mem.data_ptr(), n_pages, page_len, n_kv, hd, kt, vt),
+            gl.KvSeqs(len(lens), len(table[0]), max_len, tab.data_ptr(), ln.data_ptr()), keep)
+
+
+def test_pages_that_several_sequences_read(ctx):
+    """A common start of two pages and one of its own for each of three sequences; one of them twice in the call."""
+    import torch
+    n_kv, hd, page = 2, 128, 64
+    gen = _generator(54)
+    k, v = (torch.randn((5 * page, n_kv, hd), device="cuda", generator=gen) for _ in range(2))
+    cache, seqs, keep = _cache(ctx, 6, page, n_kv, hd, 8, 4, [[4, 0, 2, 5, 1]], [5 * page], 5 * page)
+    ld = n_kv * hd
+    off = t(np.array([0, 5 * page], np.int32))
+    ctx.check(ctx.lib.ggq_kv_store_dev(ctx.h, cache, seqs, off.data_ptr(), 5 * page, k.data_ptr(), ld, v.data_ptr(), ld, 0, stream()), "store")
+    lens = [150, 130, 192, 150]
+    table, ln = t(np.array([[4, 0, 2], [4, 0, 5], [4, 0, 1], [4, 0, 2]], np.int32)), t(np.array(lens, np.int32))
+    shared = gl.KvSeqs(4, 3, 192, table.data_ptr(), ln.data_ptr())
+    q, out = torch.randn((4, 4, hd), device="cuda", generator=gen), torch.empty((4, 4, hd), device="cuda")
+    q[3] = q[0]
+    ctx.check(ctx.lib.ggq_attention_kv_dev(ctx.h, cache, shared, q.data_ptr(), 4 * hd, 4, 0.0, 0, out.data_ptr(), 4 * hd, stream()), "a")
+    kk, vv = au.kv_quantize(host(k), 8)[0], au.kv_quantize(host(v), 4)[0]
+    got = host(out)
+    for s, last in enumerate((2, 3, 4, 2)):
+        at = np.concatenate([np.arange(2 * page), np.arange(last * page, (last + 1) * page)])[:lens[s]]
+        want, tol = au.attention(host(q)[s:s + 1], kk[at], vv[at], lens[s] - 1)
+        au.check(got[s:s + 1], want, tol)
+    assert np.array_equal(got[0], got[3])
+    k2, v2 = (torch.full((sum(lens), n_kv, hd), 5.0, device="cuda") for _ in range(2))
+    off = t(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    ctx.check(ctx.lib.ggq_kv_load_dev(ctx.h, cache, shared, off.data_ptr(), sum(lens), k2.data_ptr(), ld, v2.data_ptr(), ld, 0, stream()), "l")
+    at = np.concatenate([np.concatenate([np.arange(2 * page), np.arange(x * page, (x + 1) * page)])[:n] for x, n in zip((2, 3, 4, 2), lens)])
+    assert np.array_equal(host(k2), kk[at].astype(np.float32)) and np.array_equal(host(v2), vv[at].astype(np.float32))
+
+
+def test_more_rows_than_positions(ctx):
+    """Rows of a sequence beyond its length have positions below 0: nothing is stored or loaded for them."""
+    import torch
+    n_kv, hd, page = 1, 64, 32
+    gen = _generator(55)
+    k, v = (torch.randn((60, n_kv, hd), device="cuda", generator=gen) for _ in range(2))
+    cache, seqs, keep = _cache(ctx, 4, page, n_kv, hd, 4, 4, [[2, 0], [1, 3]], [10, -3], 64)
+    off = t(np.array([0, 40, 60], np.int32))
+    mem = keep[0]
+    before = host(mem)
+    ctx.check(ctx.lib.ggq_kv_store_dev(ctx.h, cache, seqs, off.data_ptr(), 60, k.data_ptr(), 64, v.data_ptr(), 64, 0, stream()), "store")
+    after = host(mem)
+    assert np.array_equal(after[[0, 1, 3]], before[[0, 1, 3]])
+    K, V = au.kv_unpack(after, n_kv, page, hd, 4, 4)
+    K0, V0 = au.kv_unpack(before, n_kv, page, hd, 4, 4)
+    assert np.array_equal(K[2, :10], au.kv_quantize(host(k)[30:40], 4)[0]) and np.array_equal(K[2, 10:], K0[2, 10:])
+    assert np.array_equal(V[2, :10], au.kv_quantize(host(v)[30:40], 4)[0]) and np.array_equal(V[2, 10:], V0[2, 10:])
+    k2, v2 = (torch.full((60, n_kv, hd), 5.0, device="cuda") for _ in range(2))
+    ctx.check(ctx.lib.ggq_kv_load_dev(ctx.h, cache, seqs, off.data_ptr(), 60, k2.data_ptr(), 64, v2.data_ptr(), 64, 0, stream()), "load")
+    assert (host(k2)[:30] == 5).all() and (host(k2)[40:] == 5).all() and (host(v2)[:30] == 5).all() and (host(v2)[40:] == 5).all()
+    assert np.array_equal(host(k2)[30:40], K[2, :10].astype(np.float32)) and np.array_equal(host(v2)[30:40], V[2, :10].astype(np.float32))
