@@ -6,9 +6,13 @@
 // order in which the matrix cores take them, values transposed.  attn_kernel
 // then computes per unit, with v_mfma_f32_32x32x16_f16,
 //   S^T[position][column] = K Q^T,  O^T[value][column] += V^T P^T
-// as the products hi hi + hi lo + lo hi of fp32 keys and values (two products
-// with fp16 ones, which need no split), so results are as exact as fp32
-// sums.  A column is one (query row, head) pair: the rows of a sequence and the
+// as the products hi lo + lo hi + hi hi of fp32 keys and values (hi lo + hi hi with fp16
+// ones, which need no split).  Queries and weights are cut to hi (11 bits) and lo, keys and
+// values rounded to hi and lo: 22 bits of the largest value of a row each, and lo lo is left
+// out, so a product is off by up to 2^-20 of it where fp32 has 2^-24.  The small products of a score
+// come first, which leaves a rounding a step of 16 hi hi products; against 64 bits the results
+// are off by 2.8e-7 in the mean over 720 drawn calls where elementary fp32 operations are by 5.0e-7.
+//   A column is one (query row, head) pair: the rows of a sequence and the
 // heads that share a kv head are numbered through, 32 columns a wavefront,
 // so any ratio of heads fills the tiles and all wavefronts of a workgroup share
 // each unit in LDS.
@@ -21,14 +25,14 @@
 // workgroup's wavefronts, which share the SIMDs with the first, runs a phase behind
 // it, so that one of two is always at the matrix cores while the other is not.
 //   The maximum moves only when a unit exceeds it by 2^4; weights are kept times
-// 2^11 (at most 2^15), so hi + lo of a small weight keeps 2^-35 of the largest.
+// 2^11 (at most 2^15), so hi + lo of a small weight keeps 2^-36 of the largest.
 // Scores take their position's power of two back; weights take the values', relative to
 // the unit of the row's running sums, which follows the largest product of weight and value
 // that the row has seen: neither a position that it does not see nor one of next to no
 // weight has a say in what it keeps of the others.
 // Bound: the matrix cores, at the clock that their load leaves (8191 rows of 32
-// heads of 128 in fp32: 1.37 ms, 1.2 PFLOP/s of fp16 products, what the
-// library's matmul reaches; a unit 5100 cycles, three fifths of them products).
+// heads of 128 in fp32: 1.38 to 1.48 ms on several cards, 1.1 to 1.2 PFLOP/s of fp16 products, what the
+// library's matmul reaches; a unit about 5100 cycles, three fifths of them products).
 #include <algorithm>
 #include <cstdlib>
 #include <type_traits>
@@ -677,8 +681,10 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
                 sums(it);
                 scores(it + 1);
                 // operands are read AHEAD of their products: a read takes longer than the two products that
-                // the compiler would leave it
-                constexpr int AHEAD = 8, NG = KS + 2 * DB;  // reads; operands (each of P planes, P + 1 products)
+                // the compiler would leave it.  (The order is that of P + 1 products for the P planes of an operand; the
+                // second look at the keys' hi planes is left to the compiler.  us, 2048 rows of 32x8x128, of 16x2x256: no
+                // order 159, 213, this one 149, 198, one that counts the second look 149, 227.)
+                constexpr int AHEAD = 8, NG = KS + 2 * DB;  // reads; operands
                 __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
                 for (int i = 0; i < NG - AHEAD / P; i++) {
@@ -786,19 +792,21 @@ AttnPromptPlan attn_prompt_plan(const ggq_attention_prompt_params& p) {
     AttnPromptPlan pl{};
     // The VALU's one launch up to 2^27 products of rows, heads, keys and values, while a wavefront
     // does not go through the keys too often (us, few -> matrix cores; fp32, heads x kv heads x width):
-    //   19 rows: 32x8x64 7.2 -> 11.6, 16x2x256 10.0 -> 24.9; 128 rows: 32x8x128 18.6 -> 26.6
-    //   256 rows: 32x8x64 23.6 -> 24.6, 32x8x128 (2^28) 43.9 -> 34.2; 40 prompts of 150 rows,
-    //   8x8x64 (2^27.6) 62.7 -> 40.5; 512 rows 4x1x128 23.2 -> 31.0; 1000 rows 2x1x64 32.7 -> 27.1
-    //   one row: 501 keys 32x8x128 21.8 -> 23.5, 2001 keys 68 -> 40
+    //   19 rows: 32x8x64 6.0 -> 11.0, 16x2x256 8.5 -> 23.3; 128 rows: 32x8x128 16.5 -> 24.7
+    //   256 rows: 32x8x64 20.3 -> 22.0, 32x8x128 (2^28) 39.3 -> 30.0; 40 prompts of 150 rows,
+    //   8x8x64 (2^28.8) 94 -> 43; 512 rows 4x1x128 21.0 -> 29.8; 1000 rows 2x1x64 31.1 -> 26.2
+    //   one row: 501 keys 32x8x128 20.5 -> 22.7, 2001 keys 67 -> 37
+    // Lengths are known as a mean only: one long sequence among short ones is taken like them (63 rows of 5
+    // keys with 4 rows of 20000, 32x8x128: 630 -> 1072).
     const char* env = getenv("GGQ_PROMPT_MFMA");
     const double keys = (double)p.n_kv_rows / p.n_seq;
     if (env && *env) pl.few = atoi(env) == 0;
     else pl.few = keys <= 640 && keys * p.n_rows * p.n_head * p.head_dim <= (double)(1 << 27) * 1.01;
     if (pl.few) return pl;
     // few tiles: the positions in parts of four units at least, where that saves a workgroup
-    // more units than the join costs (us with 1, 2, 3, 4 .. parts; * the rule's: 512 rows 32x8x128 49, 44,
-    // 41*; 16x2x256 66, 53, 50, 48*; 5 packed prompts 12x2x128 f16 49, 46*, 57; one row of 4001 keys
-    // 227, 128, .., 46 with 16, 50 with 31*)
+    // more units than the join costs (us with 1, 2, 3, 4 parts; * the rule's: 512 rows 32x8x128 47, 42,
+    // 40*, 39; 16x2x256 66, 52, 48*, 46; 5 packed prompts 12x2x128 f16 52, 48*, 60, 63; one row of 4001 keys
+    // 225, 127, 94, 79, .., 48 with 16, 49 with 31*)
     const int64_t wgs = tiles_of(p) * p.n_kv_head, units = units_of(p) / p.n_seq;
     const int64_t n = std::min<int64_t>(cu_count() / wgs, units / 4);
     pl.splits = n > 1 && units * (n - 1) > 4 * n ? (int)n : 1;

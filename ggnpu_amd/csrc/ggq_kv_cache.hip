@@ -241,8 +241,8 @@ void rows_go(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r, bool 
 
 template <int HD, int KB, int VB> hipError_t rows_launch(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvRows& r,
                                                          bool store, hipStream_t s) {
-    // four rows a thread once that leaves every CU two workgroups: their loads overlap (16 x 4001 rows of 2 heads of
-    // 128 into fp16: 24.3 us with one row, 18.7 with four); below that one row, for the shorter chain
+    // four rows a thread once that leaves every CU two workgroups: their loads overlap (16 x 4001 fp16 rows of 2 heads of
+    // 128 in 8 bits: load 30.2 us with one row, 18.6 with four, store 25.8 and 20.9); below that one row, for the shorter chain
     const bool many = (int64_t)r.n_rows * c.n_kv_head * HD * 2 / (4 * 2048) >= 2 * cu_count();
     if (r.type == GGQ_TYPE_F32) many ? rows_go<HD, KB, VB, 4, float>(c, q, r, store, s) : rows_go<HD, KB, VB, 1, float>(c, q, r, store, s);
     else many ? rows_go<HD, KB, VB, 4, _Float16>(c, q, r, store, s) : rows_go<HD, KB, VB, 1, _Float16>(c, q, r, store, s);
@@ -669,8 +669,8 @@ template <int HD, int KB, int VB, int NT> int64_t resident() {
 
 // One round of workgroups at most, four records in a part at least; and only where
 // the rounds of records that it saves a wavefront are worth the join (in us, one sequence,
-// 8 kv heads of 128 in 4 bits: 500 positions 7.5 with one part, 8.1 with 4; 1000: 10.2,
-// 8.3 with 8; 4000: 26.3, 9.0 with 32; 16 sequences of 1000: 10.5, 11.2 with 2).
+// 8 kv heads of 128 in 4 bits: 500 positions 7.3 with one part, 8.1 with 4; 1000: 9.8,
+// 8.3 with 8; 4000: 25.0, 8.7 with 32; 16 sequences of 1000: 9.9, 10.7 with 2; of 6000: 38, 27).
 template <int HD, int KB, int VB> int attn_splits(const KvAttnArgs& a, int64_t records) {
     const int G = a.n_head / a.c.n_kv_head, NW = G <= 4 ? kv_waves<HD, 1>() : kv_waves<HD, 2>();
     const int64_t wgs = (int64_t)a.q.n_seq * a.c.n_kv_head * ((G + 7) / 8);

@@ -90,11 +90,13 @@ int ggq_sync(ggq_ctx* ctx);
  * also use a buffer per stream (streams from the
  * ninth on share eight, and their calls wait for one another where they meet
  * on one), and other kernels where it cannot be had: the same products, rounded
- * in another order, in several times the time.  A stream's work is complete
+ * in another order, in several times the time (attention: up to 26 times, a
+ * prompt of 8191 rows 18 ms for 1.4, one sequence of 131001 positions 580 us for 22).  A stream's work is complete
  * before the stream is destroyed.  Each capture gets a buffer of its
  * own that stays with its graph: a call outside a capture, on any stream, sets
  * aside what eight captures of the largest such call so far need (two where
- * that is more than 256 MB), ggq_reserve its bytes, at most 8 GiB of a context.
+ * that is more than 256 MB; anew, and for twice as much at least, when a call is
+ * larger than any before), ggq_reserve its bytes, at most 8 GiB of a context.
  * Run a call between captures when there are more of them.  The synchronous
  * host-pointer calls use their own buffers.  No reference counterpart (the
  * reference has no device workspace). */
@@ -382,11 +384,21 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * ascending, within n_rows and n_kv_rows; kv_off NULL: the same as q_off).
  * The last query row sees all of its sequence's keys, each row before it one
  * less: a prompt's next chunk is n query rows against all positions so far.
- * With window > 0 a row sees the last `window` of those only.  A row that
+ * With window > 0 a row sees the last `window` of those only (any value: one
+ * above every length is none).  A row that
  * sees nothing gets zeros; rows outside of all sequences stay as they were.
  * Keys that a row does not see do not count, whatever they hold; a row that
  * sees a key which is not finite, or whose query is not, has no defined
- * result (the others keep theirs).  Rows are
+ * result (the others keep theirs).
+ * Scores, weights and sums are fp32.  Calls of more than about 2^27 products, or
+ * 640 keys a sequence, go through fp16 parts on the matrix cores: a query, a key and a value of F32
+ * rows keep 22 bits of their row's largest value (smaller ones an absolute 2^-31 of
+ * it), a product of scores or sums is off by up to 2^-20 of it, and a weight
+ * keeps an absolute 2^-36 of its row's largest (F32: a weight times its value that, of
+ * the largest such product).  In the mean the results are as far from 64 bits as those of
+ * elementary fp32 operations.
+ * The kernel is chosen by the mean length n_kv_rows / n_seq: a batch of many empty or
+ * short sequences and one long one runs slower than the long one alone would.  Rows are
  * [n_head or n_kv_head][head_dim] values, dense, with row strides ld*; q and
  * out fp32, k and v of `type` (GGQ_TYPE_F32 or GGQ_TYPE_F16, a slab
  * [position][n_kv_head][head_dim] as it is); head_dim 64, 128 or 256; any
