@@ -25,7 +25,8 @@
 // workgroup's wavefronts, which share the SIMDs with the first, runs a phase behind
 // it, so that one of two is always at the matrix cores while the other is not.
 //   The maximum moves only when a unit exceeds it by 2^4; weights are kept times
-// 2^11 (at most 2^15), so hi + lo of a small weight keeps 2^-36 of the largest.
+// 2^11 (at most 2^15), so hi + lo of a small weight keeps 2^-36 of the largest (with values
+// that the planes do not bring closer than 2^8: 2^-28 of the largest product).
 // Scores take their position's power of two back; weights take the values', relative to
 // the unit of the row's running sums, which follows the largest product of weight and value
 // that the row has seen: neither a position that it does not see nor one of next to no

@@ -394,8 +394,8 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * 640 keys a sequence, go through fp16 parts on the matrix cores: a query, a key and a value of F32
  * rows keep 22 bits of their row's largest value (smaller ones an absolute 2^-31 of
  * it), a product of scores or sums is off by up to 2^-20 of it, and a weight
- * keeps an absolute 2^-36 of its row's largest (F32: a weight times its value that, of
- * the largest such product).  In the mean the results are as far from 64 bits as those of
+ * keeps an absolute 2^-36 of its row's largest (F32: a weight times the largest value of
+ * its position 2^-28 of the largest such product, what is below counts as nothing).  In the mean the results are as far from 64 bits as those of
  * elementary fp32 operations.
  * The kernel is chosen by the mean length n_kv_rows / n_seq: a batch of many empty or
  * short sequences and one long one runs slower than the long one alone would.  Rows are
