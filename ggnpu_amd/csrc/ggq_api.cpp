@@ -27,6 +27,7 @@
 #include "ggq_attn.h"
 #include "ggq_formats.h"
 #include "ggq_launch.h"
+#include "ggq_steps.h"
 
 static_assert(ggq::kScratchBytes == GGQ_NOALLOC_SCRATCH_BYTES, "scratch size of the header and the library differ");
 
@@ -1306,6 +1307,119 @@ int ggq_attention_kv_dev(ggq_ctx* c, const ggq_kv_cache* cache, const ggq_kv_seq
     const hipError_t e = ggq::launch_kv_attn(a, splits, ws, s);
     lane_done(c, s);
     return hip_status(c, e, "cache attention");
+    GGQ_END(c)
+}
+
+int ggq_attention_kv_rows_dev(ggq_ctx* c, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off,
+                              int n_rows, const float* q, int64_t ldq, int n_head, float scale, int window, float* out,
+                              int64_t ldo, void* stream) {
+    GGQ_GUARD(c)
+    const int st = check_kv(c, cache, seqs);
+    if (st != GGQ_OK) return st;
+    if (n_head < 1 || n_head > 65535 || n_head % cache->n_kv_head)
+        return set_status(c, GGQ_INVALID_PARAM, "need n_head a multiple of n_kv_head, at most 65535");
+    const int64_t row = (int64_t)n_head * cache->head_dim;
+    if (n_rows < 0 || ldq < row || ldo < row || window < 0 || !std::isfinite(scale))
+        return set_status(c, GGQ_INVALID_PARAM, "need n_rows >= 0, ldq, ldo of a row or more, window >= 0 and a finite scale");
+    if ((int64_t)n_rows * n_head / 4 + seqs->n_seq > INT32_MAX)
+        return set_status(c, GGQ_INVALID_PARAM, "n_rows * n_head is too large");
+    if (n_rows == 0 || seqs->n_seq == 0) return set_status(c, GGQ_OK);
+    if (!q || !out) return set_status(c, GGQ_INVALID_PARAM, "null q/out");
+    if (!aligned16(q) || !aligned16(out) || ldq % 4 || ldo % 4)
+        return set_status(c, GGQ_INVALID_PARAM, "q, out and their rows must be 16-byte aligned");
+    const hipStream_t s = pick_stream(c, stream);
+    const ggq::KvChunkArgs a{*cache, *seqs, row_off, n_rows, q, ldq, n_head, log2_scale(scale, cache->head_dim), window, out, ldo};
+    ggq::KvChunkPlan pl = ggq::kv_chunk_plan(a, true);
+    void* ws = nullptr;
+    if (pl.ws_bytes) {
+        ws = lane_ws(c, s, pl.ws_bytes, nullptr, 0);
+        if (!ws) pl = ggq::kv_chunk_plan(a, false);  // one workgroup takes all positions: slower, no workspace
+    }
+    const hipError_t e = ggq::launch_kv_chunk(a, pl, ws, s);
+    lane_done(c, s);
+    return hip_status(c, e, "cache attention of rows");
+    GGQ_END(c)
+}
+
+int ggq_delta_rule_dev(ggq_ctx* c, const ggq_delta_rule_params* p, void* stream) {
+    GGQ_GUARD(c)
+    if (!p) return set_status(c, GGQ_INVALID_PARAM, "null params");
+    if (p->n_k_head < 1 || p->n_v_head < 1 || p->n_v_head % p->n_k_head || p->n_v_head > 65535)
+        return set_status(c, GGQ_INVALID_PARAM, "need n_v_head a multiple of n_k_head, at most 65535");
+    if (p->k_dim != 64 && p->k_dim != 128 && p->k_dim != 256)
+        return set_status(c, GGQ_INVALID_PARAM, "k_dim must be 64, 128 or 256 (got %d)", p->k_dim);
+    if (p->v_dim < 16 || p->v_dim > 512 || p->v_dim % 16)
+        return set_status(c, GGQ_INVALID_PARAM, "v_dim must be a multiple of 16, at most 512 (got %d)", p->v_dim);
+    const int64_t krow = (int64_t)p->n_k_head * p->k_dim, vrow = (int64_t)p->n_v_head * p->v_dim;
+    if (p->ldq < krow || p->ldk < krow || p->ldv < vrow || p->ldo < vrow || p->ld_gate < p->n_v_head || p->ld_beta < p->n_v_head)
+        return set_status(c, GGQ_INVALID_PARAM, "row strides must hold a row's heads");
+    if (p->flags & ~(GGQ_DELTA_BETA_SIGMOID | GGQ_DELTA_QK_NORM)) return set_status(c, GGQ_INVALID_PARAM, "unknown flags %d", p->flags);
+    if (p->n_seq < 0 || p->n_seq > 65535 || p->n_rows < 0 || p->n_slots < 0 || !std::isfinite(p->scale) || !(p->eps >= 0.0f))
+        return set_status(c, GGQ_INVALID_PARAM, "need n_seq in 0..65535, n_rows and n_slots >= 0, a finite scale and eps >= 0");
+    if (p->n_seq == 0 || p->n_slots == 0) return set_status(c, GGQ_OK);
+    if (!p->state || !p->state_out || (p->n_rows && (!p->q || !p->k || !p->v || !p->gate || !p->beta || !p->out)))
+        return set_status(c, GGQ_INVALID_PARAM, "null q/k/v/gate/beta/state/out");
+    if (p->gate_bias && !p->gate_rate) return set_status(c, GGQ_INVALID_PARAM, "gate_bias without gate_rate");
+    if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || !aligned16(p->state) ||
+        !aligned16(p->state_out) || p->ldq % 4 || p->ldk % 4 || p->ldv % 4 || p->ldo % 4)
+        return set_status(c, GGQ_INVALID_PARAM, "q, k, v, out, their rows and the states must be 16-byte aligned");
+    const hipStream_t s = pick_stream(c, stream);
+    const size_t need = ggq::delta_ws_bytes(*p);
+    void* ws = need ? lane_ws(c, s, need, nullptr, 0) : nullptr;  // (none: row by row)
+    const hipError_t e = ggq::launch_delta(*p, ws, s);
+    lane_done(c, s);
+    return hip_status(c, e, "delta rule");
+    GGQ_END(c)
+}
+
+int ggq_norm_dev(ggq_ctx* c, const ggq_norm_params* p, void* stream) {
+    GGQ_GUARD(c)
+    if (!p) return set_status(c, GGQ_INVALID_PARAM, "null params");
+    const int K = p->n_cols, len = p->norm_len ? p->norm_len : K;
+    if (p->act_mode != GGQ_ACT_F32 && p->act_mode != GGQ_ACT_Q8_ROW && p->act_mode != GGQ_ACT_Q8_BLOCK32)
+        return set_status(c, GGQ_INVALID_PARAM, "bad act_mode %d", p->act_mode);
+    if (p->n_rows < 0 || K < 4 || K > 32768 || K % 4 || (p->act_mode == GGQ_ACT_Q8_BLOCK32 && K % 32))
+        return set_status(c, GGQ_INVALID_PARAM, "n_cols must be a multiple of 4 (32 for Q8_BLOCK32), at most 32768 (got %d)", K);
+    if (len < 4 || len % 4 || K % len) return set_status(c, GGQ_INVALID_PARAM, "norm_len must be a multiple of 4 that divides n_cols (got %d)", len);
+    if (!(p->eps >= 0.0f)) return set_status(c, GGQ_INVALID_PARAM, "eps must be 0 or above");
+    const struct { const void* ptr; int64_t ld; const char* what; } rows[] = {
+        {p->x, p->ldx, "x"}, {p->add, p->ld_add, "add"}, {p->sum, p->ld_sum, "sum"}, {p->gate, p->ld_gate, "gate"}, {p->out, p->ldo, "out"}};
+    for (const auto& r : rows)
+        if (r.ptr && (r.ld < K || r.ld % 4 || !aligned16(r.ptr)))
+            return set_status(c, GGQ_INVALID_PARAM, "%s: 16-byte aligned, with a stride of n_cols or more, a multiple of 4", r.what);
+    if (p->n_rows == 0) return set_status(c, GGQ_OK);
+    if (!p->x || (p->act_mode != GGQ_ACT_F32 && (!p->codes || !p->scales)) || (p->act_mode == GGQ_ACT_F32 && !p->out && !p->sum))
+        return set_status(c, GGQ_INVALID_PARAM, "null x, no output, or codes without codes/scales");
+    if (!aligned16(p->norm_w) || (p->act_mode != GGQ_ACT_F32 && !aligned16(p->codes)))
+        return set_status(c, GGQ_INVALID_PARAM, "norm_w and codes must be 16-byte aligned");
+    if ((p->sum && ((p->sum == p->x && p->ld_sum != p->ldx) || (p->sum == p->add && p->ld_sum != p->ld_add))) ||
+        (p->out && p->out == p->x && p->ldo != p->ldx) || (p->out && p->out == p->sum))
+        return set_status(c, GGQ_INVALID_PARAM, "sum over x or add and out over x take the same stride; out and sum are apart");
+    return hip_status(c, ggq::launch_norm(*p, pick_stream(c, stream)), "norm");
+    GGQ_END(c)
+}
+
+int ggq_sample_dev(ggq_ctx* c, const ggq_sample_params* p, void* stream) {
+    GGQ_GUARD(c)
+    if (!p) return set_status(c, GGQ_INVALID_PARAM, "null params");
+    if (p->n_rows < 0 || p->n_rows > 65535 || p->n_vocab < 1 || p->n_vocab > 1 << 22 || p->ld < p->n_vocab)
+        return set_status(c, GGQ_INVALID_PARAM, "need n_rows in 0..65535, n_vocab in 1..2^22 and ld >= n_vocab (got %d, %d, %lld)",
+                          p->n_rows, p->n_vocab, (long long)p->ld);
+    if (p->n_rows == 0) return set_status(c, GGQ_OK);
+    if (!p->logits || !p->u || !p->token) return set_status(c, GGQ_INVALID_PARAM, "null logits/u/token");
+    const hipStream_t s = pick_stream(c, stream);
+    const size_t need = ggq::sample_ws_bytes(*p);
+    void* ws = lane_ws(c, s, need, nullptr, 0);
+    if (!ws) {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        const bool capturing = hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
+        return set_status(c, capturing ? GGQ_ERROR : GGQ_OUT_OF_MEMORY,
+                          "sampling: %zu bytes of workspace needed%s", need,
+                          capturing ? " while the stream is being captured; call ggq_reserve or run the call once before the capture" : "");
+    }
+    const hipError_t e = ggq::launch_sample(*p, ws, s);
+    lane_done(c, s);
+    return hip_status(c, e, "sampling");
     GGQ_END(c)
 }
 

@@ -28,4 +28,49 @@ __device__ __forceinline__ Two rows16(float v) {
     return Two{__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
 }
 
+// ---- operands from the records of a quantized cache
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// A block's scale from its byte.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+
+union Frag {
+    uint32_t w[4];
+    bf16x8 v;
+};
+
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float s, int b) {
+    bf16x2 r;
+    switch (b) {  // the byte is an immediate
+    case 0: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0); break;
+    case 1: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1); break;
+    case 2: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2); break;
+    default: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3); break;
+    }
+    return __builtin_bit_cast(uint32_t, r);
+}
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t w, float s, int half) {
+    const bf16x2 r = half ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true)
+                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false);
+    return __builtin_bit_cast(uint32_t, r);
+}
+// Values 2i and 2i + 1 of a run of codes.
+template <int BITS> __device__ __forceinline__ uint32_t pair_of(const uint32_t* w, float s, int i) {
+    if constexpr (BITS == 4) return fp4_pair(w[i / 4], s, i % 4);
+    else return fp8_pair(w[i / 2], s, i % 2);
+}
+
+// Over the four groups of 16 lanes.
+__device__ __forceinline__ float rows_max(float v) {
+    const Two x = rows16(v), y = halves(max3(x.a, x.b, x.b));
+    return max3(y.a, y.b, y.b);
+}
+
+__device__ __forceinline__ uint32_t bf16_pack(float a, float b) {  // upper halves
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+}
+
 }  // namespace ggq

@@ -20,8 +20,6 @@ namespace {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
-
 // The address of a position's record and its place there.
 struct Place {
     uint8_t* rec;  // null: there is none
@@ -285,37 +283,7 @@ hipError_t launch_kv_rows(const ggq_kv_cache& c, const ggq_kv_seqs& q, const KvR
 // and V in 4 bits: 566 MB in 103 us, 5.5 TB/s); with 64-wide ones the VALU, whose
 // work on scores does not shrink with the head (131001 positions: 238
 // instructions a record, 71 MB in 21 us and 4 us for the join).
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 namespace {
-
-union Frag {
-    uint32_t w[4];
-    bf16x8 v;
-};
-
-__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float s, int b) {
-    bf16x2 r;
-    switch (b) {  // the byte is an immediate
-    case 0: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0); break;
-    case 1: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1); break;
-    case 2: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2); break;
-    default: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3); break;
-    }
-    return __builtin_bit_cast(uint32_t, r);
-}
-__device__ __forceinline__ uint32_t fp8_pair(uint32_t w, float s, int half) {
-    const bf16x2 r = half ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true)
-                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false);
-    return __builtin_bit_cast(uint32_t, r);
-}
-// Values 2i and 2i + 1 of a run of codes.
-template <int BITS> __device__ __forceinline__ uint32_t pair_of(const uint32_t* w, float s, int i) {
-    if constexpr (BITS == 4) return fp4_pair(w[i / 4], s, i % 4);
-    else return fp8_pair(w[i / 2], s, i % 2);
-}
 
 template <int CTRL> __device__ __forceinline__ float quad_perm(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
@@ -324,12 +292,6 @@ __device__ __forceinline__ float quad_sum(float v) {
     v += quad_perm<0xB1>(v);  // lanes 1 0 3 2
     return v + quad_perm<0x4E>(v);  // lanes 2 3 0 1
 }
-// Over the four groups of 16 lanes.
-__device__ __forceinline__ float rows_max(float v) {
-    const Two x = rows16(v), y = halves(max3(x.a, x.b, x.b));
-    return max3(y.a, y.b, y.b);
-}
-
 // A part of x, its upper 16 bits: three cuts of 8 bits each hold all 24, x0 = x
 // cut, x1 = (x - x0) cut, x2 = x - x0 - x1.  A lane's part is chosen by its masks:
 // what they cut off is subtracted (everything for the column that is zero).
@@ -343,10 +305,6 @@ __device__ __forceinline__ float bf16_part(float x, Cuts c) {
     x -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & c.a);
     return x - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & c.b);
 }
-__device__ __forceinline__ uint32_t bf16_pack(float a, float b) {  // upper halves
-    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
-}
-
 // Wavefronts of a workgroup, by their registers.
 template <int HD, int NT> constexpr int kv_waves() { return HD == 256 ? 4 : 8; }
 

@@ -1,0 +1,458 @@
+// ggq_kv_chunk.hip -- causal attention of several rows of each sequence over the
+// pages of its quantized cache (ggq_attention_kv_rows_dev).
+//
+// As the attention of single tokens (ggq_kv_cache.hip) a wavefront computes per
+// record of 32 positions, on bf16 matrix cores with exact operands,
+//   S^T[position][column] = sum_d K[position][d] Q[d][column]
+//   O^T[d][column]       += sum_position V[position][d] P[position][column]
+// but a column is a (row, head) pair here: the rows of a sequence and the heads that
+// share a kv head are numbered through, 16 a tile, and the three bf16 parts
+// of q and of the weights are three products instead of three columns.  A weight is made
+// once, and no column is empty where the pairs fill the tiles.
+//   A workgroup has 16 CT columns; its wavefronts take the records of its part of the
+// positions in turn and add up in LDS, kv_chunk_join_kernel adds up the parts.
+#include <algorithm>
+#include <cstdlib>
+
+#include "ggq_attn.h"
+#include "ggq_attn_device.h"
+#include "ggq_launch.h"
+#include "ggq_steps.h"
+
+namespace ggq {
+namespace {
+
+// Sequence s has the column tiles of n from off[s] * G / n + s on: a bound that needs no sum over the sequences before.
+__device__ __forceinline__ int tile_of(const KvChunkArgs& a, int s, int G, int n) {
+    return (int)((uint32_t)min(max(a.row_off ? a.row_off[s] : s, 0), a.n_rows) * (uint32_t)G / (uint32_t)n) + s;
+}
+
+// Three bf16 parts of x hold all its 24 bits: x cut, what is left cut, what is left then.
+__device__ __forceinline__ float cut16(float x) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xFFFF0000u);
+}
+__device__ __forceinline__ void parts_of(float a, float b, uint32_t (&w)[3]) {
+    w[0] = bf16_pack(a, b);
+    a -= cut16(a);
+    b -= cut16(b);
+    w[1] = bf16_pack(a, b);
+    a -= cut16(a);
+    b -= cut16(b);
+    w[2] = bf16_pack(a, b);
+}
+
+template <int HD, int CT> constexpr int chunk_waves() { return HD * CT >= 256 ? 4 : 8; }
+
+template <int HD, int KB, int VB, int CT>
+__global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(KvChunkArgs a, int splits, float* part) {
+    constexpr int NW = chunk_waves<HD, CT>(), NC = 16 * CT;
+    constexpr int KW = HD * KB / 64, VW = HD * VB / 64;  // dwords of a lane's K and V codes
+    constexpr int NS = HD / 32;                          // k steps of S^T, blocks of a head
+    constexpr int NO = HD / 16;                          // row tiles of O^T
+    constexpr int VD = HD / 16;                          // values of a lane's V at one position
+    constexpr int64_t RB = kKvTile * HD * (KB + VB) / 8 + 2 * HD;
+    __shared__ float sm[NW][NC], sl[NW][NC], so[NW][NC][HD + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, r = lane & 15;
+    const int kvh = blockIdx.y, split = blockIdx.z, id = blockIdx.x;
+    const int G = a.n_head / a.c.n_kv_head;  // query heads of this kv head
+    const int tpp = a.c.page_len / kKvTile;
+    int seq = 0;
+    for (int i = 1; i < a.q.n_seq; i += NW * 64) {
+        const int j = i + tid;
+        seq += __syncthreads_count(j < a.q.n_seq && tile_of(a, j, G, NC) <= id);
+    }
+    const int r0 = min(max(a.row_off ? a.row_off[seq] : seq, 0), a.n_rows);
+    const int nr = min(max(a.row_off ? a.row_off[seq + 1] : seq + 1, 0), a.n_rows) - r0;
+    const int nf = max(nr, 0) * G, f0 = (id - tile_of(a, seq, G, NC)) * NC;
+    if (f0 < 0 || f0 >= nf) return;
+    const int64_t len = a.q.len[seq], lim = min(min(len, (int64_t)a.q.max_len), (int64_t)a.q.table_len * a.c.page_len);
+    // columns: pair f has row f / G at position len - nr + f / G; it sees positions beg .. end - 1
+    auto end_of = [&](int f) { return len - nr + f / G + 1; };
+    auto see = [&](int f, int& b, int& e) {
+        const int64_t x = end_of(f);
+        e = (int)max(min(x, lim), (int64_t)0);
+        b = a.window > 0 ? (int)max(x - a.window, (int64_t)0) : 0;
+    };
+    int beg[CT], end[CT], fc[CT];
+    bool live[CT];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        const int f = f0 + 16 * n + r;
+        live[n] = f < nf;
+        fc[n] = min(f, nf - 1);
+        see(fc[n], beg[n], end[n]);
+    }
+    // rows ascend with the columns: the first and the last bound what any and what all of them see
+    int lo, all_hi, all_lo, hi;
+    see(f0, lo, all_hi);
+    see(min(f0 + NC, nf) - 1, all_lo, hi);
+    const int t0 = lo / kKvTile, t1 = hi > lo ? (hi + kKvTile - 1) / kKvTile : t0;
+    int per = (t1 - t0 + splits - 1) / splits;
+    if (per > NW) per = (per + NW - 1) / NW * NW;
+    const int first = t0 + split * per, last = min(t1, first + per);
+
+    Frag qf[CT][NS][3];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        const int qi = fc[n] / G, h = fc[n] - qi * G;
+        const float* qp = a.Q + (int64_t)(r0 + qi) * a.ldq + (int64_t)(kvh * G + h) * HD + g * (HD / 4);
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const float4 u = *(const float4*)(qp + 8 * s), v = *(const float4*)(qp + 8 * s + 4);
+            const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t w[3];
+                parts_of(x[2 * i] * a.scale, x[2 * i + 1] * a.scale, w);
+#pragma unroll
+                for (int j = 0; j < 3; j++) qf[n][s][j].w[i] = w[j];
+            }
+        }
+    }
+    f32x4 o[CT][NO];
+    float m[CT], l[CT];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NO; i++) o[n][i] = f32x4{0, 0, 0, 0};
+    }
+
+    struct Rec {
+        uint32_t k[KW], v[VW], ks[NS / 2 + (NS < 2)];
+        uint2 vs;
+        bool there;
+    };
+    const int n_it = last > first + wave ? (last - first - wave + NW - 1) / NW : 0;  // records of this wavefront
+    int pages = -1;  // lane i: page of record i of the current 64
+    auto look = [&](int it) {
+        const int t = first + wave + NW * (it + lane);
+        pages = it + lane < n_it ? a.q.pages[(int64_t)seq * a.q.table_len + t / tpp] : -1;
+        if (pages >= a.c.n_pages) pages = -1;
+    };
+    auto load = [&](int it, Rec& x) {
+        const int page = __builtin_amdgcn_readlane(pages, it & 63);
+        x.there = page >= 0;
+        if (!x.there) return;
+        const int t = first + wave + NW * it;
+        const uint8_t* rec = (const uint8_t*)a.c.pages + (((int64_t)page * a.c.n_kv_head + kvh) * tpp + t % tpp) * RB;
+#pragma unroll
+        for (int i = 0; i < KW; i += 4) {
+            const uint4 v = *(const uint4*)(rec + 256 * i + 16 * lane);
+            x.k[i] = v.x; x.k[i + 1] = v.y; x.k[i + 2] = v.z; x.k[i + 3] = v.w;
+        }
+        rec += kKvTile * HD * KB / 8;
+#pragma unroll
+        for (int i = 0; i < VW; i += 4) {
+            const uint4 v = *(const uint4*)(rec + 256 * i + 16 * lane);
+            x.v[i] = v.x; x.v[i + 1] = v.y; x.v[i + 2] = v.z; x.v[i + 3] = v.w;
+        }
+        rec += kKvTile * HD * VB / 8;
+        // K scales: a lane's quarter of the head lies in block g * NS / 4 (and the next one of 256-wide heads)
+        if constexpr (NS <= 4) x.ks[0] = *(const uint16_t*)(rec + (16 * (g * NS / 4) + r) * 2);
+        else {
+            x.ks[0] = *(const uint16_t*)(rec + (16 * (2 * g) + r) * 2);
+            x.ks[1] = *(const uint16_t*)(rec + (16 * (2 * g + 1) + r) * 2);
+        }
+        x.vs = *(const uint2*)(rec + HD + (4 * (r * VD / 32) + g) * 8);
+    };
+    auto compute = [&](int it, Rec& x) {
+        if (!x.there) return;
+        const int base = (first + wave + NW * it) * kKvTile;
+        const bool partial = base < all_lo || base + kKvTile > all_hi;
+        f32x4 st[2][CT];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int n = 0; n < CT; n++) st[t][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            Frag f[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int blk = NS <= 4 ? 0 : s / 4;  // (256-wide: 64 values of a lane, two blocks)
+                const float sc = scale_of((x.ks[blk] >> (8 * t)) & 255u);
+#pragma unroll
+                for (int i = 0; i < 4; i++) f[t].w[i] = pair_of<KB>(x.k + (t * (HD / 4) + 8 * s) * KB / 32, sc, i);
+            }
+            // (the small parts first: they do not round at the size of the sum)
+#pragma unroll
+            for (int j = 2; j >= 0; j--)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int n = 0; n < CT; n++)
+                        st[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t].v, qf[n][s][j].v, st[t][n], 0, 0, 0);
+        }
+        uint32_t poison = 0;  // positions whose values read back as NaN, which some columns see and some do not
+        if (partial) {
+            // codes of positions that no column sees, or that are NaN: zero, with a finite scale
+            uint32_t keep[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int pos = base + 16 * (j / 4) + 4 * g + j % 4;
+                keep[j] = pos >= lo && pos < hi ? 0xFFFFFFFFu : 0u;
+                uint32_t bad = ((j < 4 ? x.vs.x : x.vs.y) >> (8 * (j & 3)) & 255u) == 255u;
+                if constexpr (VB == 8) {
+#pragma unroll
+                    for (int d = 0; d < VD; d++)
+                        bad |= (x.v[(j * VD + d) / 4] >> (8 * ((j * VD + d) % 4)) & 127u) == 127u;
+                }
+                if (bad && keep[j]) {
+                    poison |= 1u << j;
+                    keep[j] = 0;
+                }
+            }
+            constexpr int BPP = VD * VB / 8;  // bytes of a position
+#pragma unroll
+            for (int d = 0; d < VW; d++) {
+                if constexpr (BPP >= 4) x.v[d] &= keep[d * 4 / BPP];
+                else x.v[d] &= (keep[2 * d] & 0xFFFFu) | (keep[2 * d + 1] & 0xFFFF0000u);
+            }
+            uint32_t lo4 = 0, hi4 = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                lo4 |= (keep[j] ? (x.vs.x >> (8 * j)) & 255u : 127u) << (8 * j);
+                hi4 |= (keep[j + 4] ? (x.vs.y >> (8 * j)) & 255u : 127u) << (8 * j);
+            }
+            x.vs = make_uint2(lo4, hi4);
+            if (__any(poison != 0)) {
+#pragma unroll
+                for (int s = 1; s < 16; s <<= 1) poison |= (uint32_t)__shfl_xor((int)poison, s, 64);
+            }
+        }
+        bool move = false;
+        float top[CT];
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            if (partial) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int pos = base + 16 * (j / 4) + 4 * g + j % 4;
+                    const bool sees = pos >= beg[n] && pos < end[n];
+                    if (!sees) st[j / 4][n][j % 4] = -INFINITY;
+                    else if (poison >> j & 1u) l[n] = __builtin_nanf("");
+                }
+            }
+            const f32x4 x0 = st[0][n], x1 = st[1][n];
+            top[n] = rows_max(max3(max3(x0[0], x0[1], x0[2]), max3(x0[3], x1[0], x1[1]), max3(x1[2], x1[3], x1[3])));
+            move |= top[n] > m[n] + 8.0f;
+        }
+        if (__any(move)) {
+#pragma unroll
+            for (int n = 0; n < CT; n++) {
+                const float mn = max3(m[n], top[n], top[n]);
+                const float al = __builtin_amdgcn_exp2f(m[n] - (mn == -INFINITY ? 0.0f : mn));
+                m[n] = mn;
+                l[n] *= al;
+#pragma unroll
+                for (int i = 0; i < NO; i++) o[n][i] *= al;
+            }
+        }
+        Frag pf[CT][3];
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            const float mm = m[n] == -INFINITY ? 0.0f : m[n];
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                e[j] = __builtin_amdgcn_exp2f(st[j / 4][n][j % 4] - mm);
+                l[n] += e[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t w[3];
+                parts_of(e[2 * j], e[2 * j + 1], w);
+#pragma unroll
+                for (int i = 0; i < 3; i++) pf[n][i].w[j] = w[i];
+            }
+        }
+        // weights times values, two row tiles (values 2 i, 2 i + 1 of a lane's run) at a time
+        float vs[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) vs[j] = scale_of(((j < 4 ? x.vs.x : x.vs.y) >> (8 * (j & 3))) & 255u);
+#pragma unroll
+        for (int i = 0; i < NO / 2; i++) {
+            uint32_t c[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int v = j * VD + 2 * i;  // index in the lane's run of codes, even
+                if constexpr (VB == 4) c[j] = fp4_pair(x.v[v / 8], vs[j], v % 8 / 2);
+                else c[j] = fp8_pair(x.v[v / 4], vs[j], v % 4 / 2);
+            }
+            Frag f[2];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                f[0].w[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x05040100u);
+                f[1].w[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x07060302u);
+            }
+#pragma unroll
+            for (int j = 2; j >= 0; j--)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int n = 0; n < CT; n++)
+                        o[n][2 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[e].v, pf[n][j].v, o[n][2 * i + e], 0, 0, 0);
+        }
+    };
+    Rec cur, nxt;
+    look(0);
+    if (n_it > 0) load(0, cur);
+    for (int it = 0; it < n_it; it++) {
+        if (it + 1 < n_it) {
+            if (((it + 1) & 63) == 0) look(it + 1);
+            load(it + 1, nxt);
+        }
+        compute(it, cur);
+        cur = nxt;
+    }
+
+    // the wavefronts' parts
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        float s = l[n];  // of this group's positions
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        const int c = 16 * n + r;
+        if (g == 0) { sm[wave][c] = m[n]; sl[wave][c] = s; }
+#pragma unroll
+        for (int i = 0; i < NO; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) so[wave][c][(4 * g + e) * VD + i] = o[n][i][e];
+    }
+    __syncthreads();
+    const int nc = min(NC, nf - f0);
+    for (int e = tid; e < nc * HD; e += NW * 64) {
+        const int c = e / HD, d = e % HD;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; w++) mx = fmaxf(mx, sm[w][c]);
+        float ls = 0.0f, os = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float al = sm[w][c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][c] - mx);
+            ls = fmaf(sl[w][c], al, ls);
+            os = fmaf(so[w][c][d], al, os);
+        }
+        const int qi = (f0 + c) / G, head = kvh * G + (f0 + c) - qi * G;
+        if (splits == 1) {
+            // no position at all: zeros (a NaN keeps its way through the sum)
+            a.out[(int64_t)(r0 + qi) * a.ldo + (int64_t)head * HD + d] = ls == 0.0f && mx == -INFINITY ? 0.0f : os / ls;
+        } else {
+            float* po = part + (((int64_t)(r0 + qi) * a.n_head + head) * splits + split) * (HD + 2);
+            po[d] = os;
+            if (d == 0) { po[HD] = mx; po[HD + 1] = ls; }
+        }
+    }
+}
+
+// The parts of one row's head, in their order: a wavefront each, HD / 64 values a lane.
+template <int HD> __global__ __launch_bounds__(256) void kv_chunk_join_kernel(KvChunkArgs a, int splits, const float* part) {
+    constexpr int DPL = HD / 64;
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = (int)(w / a.n_head), head = (int)(w % a.n_head), lane = threadIdx.x & 63;
+    if (row >= a.n_rows) return;
+    bool in = !a.row_off && row < a.q.n_seq;  // a row of some sequence
+    if (a.row_off)
+        for (int i = 0; i < a.q.n_seq && !in; i += 64) {
+            const int j = i + lane;
+            in = __any(j < a.q.n_seq && a.row_off[j] <= row && row < a.row_off[j + 1]);
+        }
+    if (!in) return;
+    const float* q = part + w * splits * (HD + 2);
+    float mx = -INFINITY;
+    for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, q[(int64_t)i * (HD + 2) + HD]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    float ls = 0.0f, os[DPL] = {};
+#pragma unroll 4
+    for (int i = 0; i < splits; i++) {
+        const float* x = q + (int64_t)i * (HD + 2);
+        const float wt = x[HD] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[HD] - mx);
+        ls = fmaf(x[HD + 1], wt, ls);
+#pragma unroll
+        for (int d = 0; d < DPL; d++) os[d] = fmaf(x[lane + 64 * d], wt, os[d]);
+    }
+    float* out = a.out + (int64_t)row * a.ldo + (int64_t)head * HD + lane;
+#pragma unroll
+    for (int d = 0; d < DPL; d++) out[64 * d] = ls == 0.0f && mx == -INFINITY ? 0.0f : os[d] / ls;
+}
+
+constexpr int kMaxSplits = 256;
+
+// Workgroups that the chip holds at once.
+template <int HD, int KB, int VB, int CT> int64_t resident() {
+    static const int64_t n = [] {
+        int r = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&r, (const void*)kv_chunk_kernel<HD, KB, VB, CT>, chunk_waves<HD, CT>() * 64, 0) != hipSuccess || r < 1)
+            r = 1;
+        return (int64_t)r * cu_count();
+    }();
+    return n;
+}
+
+int64_t tiles_of(const KvChunkArgs& a, int nc) { return (int64_t)a.n_rows * (a.n_head / a.c.n_kv_head) / nc + a.q.n_seq; }
+
+// One round of workgroups at most, four records in a part at least, where that saves more than the join costs.
+template <int HD, int KB, int VB, int CT> int splits_of(const KvChunkArgs& a, int64_t records) {
+    constexpr int NW = chunk_waves<HD, CT>();
+    const int64_t wgs = tiles_of(a, 16 * CT) * a.c.n_kv_head;
+    const int64_t n = std::min<int64_t>(resident<HD, KB, VB, CT>() / wgs, (records + 3) / 4);
+    return n > 1 && records * (n - 1) > 3 * NW * n ? (int)std::min<int64_t>(n, kMaxSplits) : 1;
+}
+
+template <int HD, int KB, int VB> int splits_go(const KvChunkArgs& a, int ct, int64_t records) {
+    if constexpr (HD < 256)
+        if (ct == 2) return splits_of<HD, KB, VB, 2>(a, records);
+    return splits_of<HD, KB, VB, 1>(a, records);
+}
+
+template <int HD, int KB, int VB> hipError_t chunk_go(const KvChunkArgs& a, const KvChunkPlan& pl, float* ws, hipStream_t s) {
+    const dim3 grid((unsigned)tiles_of(a, 16 * pl.kind), (unsigned)a.c.n_kv_head, (unsigned)pl.splits);
+    bool done = false;
+    if constexpr (HD < 256)
+        if (pl.kind == 2) {
+            kv_chunk_kernel<HD, KB, VB, 2><<<grid, chunk_waves<HD, 2>() * 64, 0, s>>>(a, pl.splits, ws);
+            done = true;
+        }
+    if (!done) kv_chunk_kernel<HD, KB, VB, 1><<<grid, chunk_waves<HD, 1>() * 64, 0, s>>>(a, pl.splits, ws);
+    if (pl.splits > 1) kv_chunk_join_kernel<HD><<<dim3((unsigned)(((int64_t)a.n_rows * a.n_head + 3) / 4)), 256, 0, s>>>(a, pl.splits, ws);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+#define GGQ_BY_CACHE(HD_, F, ...)                                                                              \
+    (c.k_type == GGQ_KV_MXFP4 ? (c.v_type == GGQ_KV_MXFP4 ? F<HD_, 4, 4>(__VA_ARGS__) : F<HD_, 4, 8>(__VA_ARGS__)) \
+                              : (c.v_type == GGQ_KV_MXFP4 ? F<HD_, 8, 4>(__VA_ARGS__) : F<HD_, 8, 8>(__VA_ARGS__)))
+
+KvChunkPlan kv_chunk_plan(const KvChunkArgs& a, bool workspace) {
+    const ggq_kv_cache& c = a.c;
+    KvChunkPlan pl{1, 1, 0};
+    // two tiles a wavefront where a sequence's pairs fill more than one
+    const int64_t pairs = (int64_t)a.n_rows * (a.n_head / c.n_kv_head);
+    if (c.head_dim < 256 && pairs > 16 * (int64_t)a.q.n_seq) pl.kind = 2;
+    if (!workspace) return pl;
+    int64_t span = std::min<int64_t>(a.q.max_len, (int64_t)a.q.table_len * c.page_len);
+    if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + a.n_rows / a.q.n_seq + kKvTile);
+    const int64_t records = (span + kKvTile - 1) / kKvTile;
+    if (const char* e = getenv("GGQ_KV_SPLITS"); e && atoi(e) > 0)
+        pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(atoi(e), kMaxSplits), records));
+    else if (c.head_dim == 64) pl.splits = GGQ_BY_CACHE(64, splits_go, a, pl.kind, records);
+    else if (c.head_dim == 128) pl.splits = GGQ_BY_CACHE(128, splits_go, a, pl.kind, records);
+    else pl.splits = GGQ_BY_CACHE(256, splits_go, a, pl.kind, records);
+    if (pl.splits > 1) pl.ws_bytes = sizeof(float) * (size_t)a.n_rows * a.n_head * pl.splits * (c.head_dim + 2);
+    return pl;
+}
+
+hipError_t launch_kv_chunk(const KvChunkArgs& a, const KvChunkPlan& pl, void* ws, hipStream_t s) {
+    const ggq_kv_cache& c = a.c;
+    if (c.head_dim == 64) return GGQ_BY_CACHE(64, chunk_go, a, pl, (float*)ws, s);
+    if (c.head_dim == 128) return GGQ_BY_CACHE(128, chunk_go, a, pl, (float*)ws, s);
+    return GGQ_BY_CACHE(256, chunk_go, a, pl, (float*)ws, s);
+}
+#undef GGQ_BY_CACHE
+
+}  // namespace ggq

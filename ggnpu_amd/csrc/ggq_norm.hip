@@ -1,0 +1,198 @@
+// ggq_norm.hip -- what stands between two layers' matmuls: the residual's
+// addition, RMSNorm of rows or of their heads, a SiLU gate, and the int8 codes
+// that the next matmul reads (ggq_norm_dev).
+//
+// A workgroup holds one row in registers, R runs of four values a thread, so
+// each input is read once and nothing is written that the caller did not ask
+// for.  Values are made in 64 bits from the fp32 sum on and rounded once: the
+// order of the square sum then does not show in the codes, whose borders an fp32
+// last bit would move values across.  gfx950 has fp64 FMAs at the rate of
+// single fp32 ones, and a row is a few of them a value.
+// Bound: HBM (measured figures at norm_launch below).
+#include <algorithm>
+
+#include "ggq_device.h"
+#include "ggq_steps.h"
+
+namespace ggq {
+namespace {
+
+struct NormArgs {
+    ggq_norm_params p;
+    int len;    // values that are normalised together
+    int lanes;  // a group's lanes where it is a power of two of up to a wavefront's (reduced by shuffles), else 0
+};
+
+template <int TPB, typename T, typename F> __device__ __forceinline__ T wg_reduce(T v, T* red, F f) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
+    if constexpr (TPB > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < TPB / 64; i++) v = f(v, red[i]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t codes_of(const float4& y, float inv) {
+    return (uint32_t)(uint8_t)to_i8(__fmul_rn(y.x, inv)) | (uint32_t)(uint8_t)to_i8(__fmul_rn(y.y, inv)) << 8 |
+           (uint32_t)(uint8_t)to_i8(__fmul_rn(y.z, inv)) << 16 | (uint32_t)(uint8_t)to_i8(__fmul_rn(y.w, inv)) << 24;
+}
+__device__ __forceinline__ float step_of(float amax) { return amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f; }
+__device__ __forceinline__ double silu64(float z) { return (double)z / (1.0 + exp(-(double)z)); }
+
+template <int TPB, int R>
+__global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
+    __shared__ double red[TPB / 64];
+    __shared__ float redf[TPB / 64];
+    extern __shared__ double parts[];  // a square sum a run, where groups are neither the row nor a power of two of lanes
+    const ggq_norm_params& p = a.p;
+    const int64_t m = blockIdx.x;
+    const int tid = threadIdx.x, K = p.n_cols;
+    const float* xr = p.x + m * p.ldx;
+    float4 v[R], g[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int k = 4 * (tid + TPB * i);
+        v[i] = k < K ? *(const float4*)(xr + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    if (p.add) {
+        const float* ar = p.add + m * p.ld_add;
+        float4 b[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int k = 4 * (tid + TPB * i);
+            b[i] = k < K ? *(const float4*)(ar + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) v[i] = make_float4(v[i].x + b[i].x, v[i].y + b[i].y, v[i].z + b[i].z, v[i].w + b[i].w);
+    }
+    if (p.gate) {
+        const float* gr = p.gate + m * p.ld_gate;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int k = 4 * (tid + TPB * i);
+            g[i] = k < K ? *(const float4*)(gr + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+    if (p.sum) {
+        float* sr = p.sum + m * p.ld_sum;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int k = 4 * (tid + TPB * i);
+            if (k < K) *(float4*)(sr + k) = v[i];
+        }
+    }
+    // each run's factor
+    double f[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const double x = v[i].x, y = v[i].y, z = v[i].z, w = v[i].w;
+        f[i] = fma(w, w, fma(z, z, fma(y, y, x * x)));
+    }
+    const double n = (double)a.len, eps = (double)p.eps;
+    if (a.len == K) {
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < R; i++) ss += f[i];
+        ss = wg_reduce<TPB>(ss, red, [](double s, double t) { return s + t; });
+        const double r = 1.0 / sqrt(ss / n + eps);
+#pragma unroll
+        for (int i = 0; i < R; i++) f[i] = r;
+    } else if (a.lanes) {
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            for (int o = 1; o < a.lanes; o <<= 1) f[i] += __shfl_xor(f[i], o, 64);
+            f[i] = 1.0 / sqrt(f[i] / n + eps);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (tid + TPB * i < K / 4) parts[tid + TPB * i] = f[i];
+        __syncthreads();
+        const int runs = a.len / 4;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int k = tid + TPB * i;
+            if (k >= K / 4) break;
+            double ss = 0.0;
+            for (int j = k / runs * runs, e = j + runs; j < e; j++) ss += parts[j];
+            f[i] = 1.0 / sqrt(ss / n + eps);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int k = 4 * (tid + TPB * i);
+        if (k >= K) break;
+        double y[4] = {(double)v[i].x * f[i], (double)v[i].y * f[i], (double)v[i].z * f[i], (double)v[i].w * f[i]};
+        if (p.norm_w) {
+            const float4 w = *(const float4*)(p.norm_w + k % a.len);
+            y[0] *= (double)w.x; y[1] *= (double)w.y; y[2] *= (double)w.z; y[3] *= (double)w.w;
+        }
+        if (p.gate) {
+            y[0] *= silu64(g[i].x); y[1] *= silu64(g[i].y); y[2] *= silu64(g[i].z); y[3] *= silu64(g[i].w);
+        }
+        v[i] = make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
+    }
+    if (p.out) {
+        float* o = p.out + m * p.ldo;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int k = 4 * (tid + TPB * i);
+            if (k < K) *(float4*)(o + k) = v[i];
+        }
+    }
+    if (p.act_mode == GGQ_ACT_F32) return;
+    float top[R], amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        top[i] = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+        amax = fmaxf(amax, top[i]);
+    }
+    uint32_t* q = (uint32_t*)(p.codes + m * K);
+    if (p.act_mode == GGQ_ACT_Q8_ROW) {
+        amax = wg_reduce<TPB>(amax, redf, [](float s, float t) { return fmaxf(s, t); });
+        const float sc = step_of(amax), inv = __fdiv_rn(1.0f, sc);
+        if (tid == 0) p.scales[m] = sc;
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (tid + TPB * i < K / 4) q[tid + TPB * i] = codes_of(v[i], inv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            float t = top[i];
+            t = fmaxf(t, __shfl_xor(t, 1, 64));
+            t = fmaxf(t, __shfl_xor(t, 2, 64));
+            t = fmaxf(t, __shfl_xor(t, 4, 64));
+            const int k = tid + TPB * i;
+            const float sc = step_of(t);
+            if (k >= K / 4) continue;
+            if ((tid & 7) == 0) p.scales[m * (K / 32) + k / 8] = sc;
+            q[k] = codes_of(v[i], __fdiv_rn(1.0f, sc));
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_norm(const ggq_norm_params& p, hipStream_t s) {
+    NormArgs a{p, p.norm_len ? p.norm_len : p.n_cols, 0};
+    const int lanes = a.len / 4;
+    if (lanes <= 64 && !(lanes & (lanes - 1))) a.lanes = lanes;
+    const size_t lds = a.len == p.n_cols || a.lanes ? 0 : sizeof(double) * (size_t)(p.n_cols / 4);
+#define L(TPB_, R_) norm_kernel<TPB_, R_><<<dim3((unsigned)p.n_rows), TPB_, lds, s>>>(a)
+    if (p.n_cols <= 256) L(64, 1);
+    else if (p.n_cols <= 512) L(64, 2);
+    else if (p.n_cols <= 1024) L(64, 4);
+    else if (p.n_cols <= 2048) L(256, 2);
+    else if (p.n_cols <= 4096) L(256, 4);
+    else if (p.n_cols <= 8192) L(512, 4);
+    else if (p.n_cols <= 16384) L(1024, 4);
+    else L(1024, 8);
+#undef L
+    return hipGetLastError();
+}
+
+}  // namespace ggq

@@ -44,6 +44,8 @@ class RopeLayout(enum.IntEnum):
 
 # element types of rows (GGML ids)
 TYPE_F32, TYPE_F16 = 0, 1
+# flags of ggq_delta_rule_params
+DELTA_BETA_SIGMOID, DELTA_QK_NORM = 1, 2
 
 
 class Producer(enum.IntEnum):
@@ -159,6 +161,34 @@ class AttnPromptParams(ctypes.Structure):
                 ("window", ctypes.c_int)]
 
 
+class DeltaRuleParams(ctypes.Structure):
+    """ggq_delta_rule_params (include/ggq.h)."""
+    _fields_ = [("n_k_head", ctypes.c_int), ("n_v_head", ctypes.c_int), ("k_dim", ctypes.c_int), ("v_dim", ctypes.c_int),
+                ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("k", ctypes.c_void_p), ("ldk", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("ldv", ctypes.c_int64), ("gate", ctypes.c_void_p), ("ld_gate", ctypes.c_int64),
+                ("beta", ctypes.c_void_p), ("ld_beta", ctypes.c_int64), ("gate_rate", ctypes.c_void_p),
+                ("gate_bias", ctypes.c_void_p), ("flags", ctypes.c_int), ("eps", ctypes.c_float), ("scale", ctypes.c_float),
+                ("state", ctypes.c_void_p), ("state_out", ctypes.c_void_p), ("n_slots", ctypes.c_int),
+                ("slot", ctypes.c_void_p), ("n_seq", ctypes.c_int), ("n_rows", ctypes.c_int), ("row_off", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64)]
+
+
+class NormParams(ctypes.Structure):
+    """ggq_norm_params (include/ggq.h)."""
+    _fields_ = [("n_rows", ctypes.c_int), ("n_cols", ctypes.c_int), ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+                ("add", ctypes.c_void_p), ("ld_add", ctypes.c_int64), ("sum", ctypes.c_void_p), ("ld_sum", ctypes.c_int64),
+                ("norm_w", ctypes.c_void_p), ("norm_len", ctypes.c_int), ("eps", ctypes.c_float),
+                ("gate", ctypes.c_void_p), ("ld_gate", ctypes.c_int64), ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64),
+                ("act_mode", ctypes.c_int), ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
+class SampleParams(ctypes.Structure):
+    """ggq_sample_params (include/ggq.h)."""
+    _fields_ = [("n_rows", ctypes.c_int), ("n_vocab", ctypes.c_int), ("logits", ctypes.c_void_p), ("ld", ctypes.c_int64),
+                ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p), ("u", ctypes.c_void_p), ("token", ctypes.c_void_p), ("prob", ctypes.c_void_p)]
+
+
 class MulMatParams(ctypes.Structure):
     """MulMatParams (include/ggnpu/backend.h:21-35)."""
     _fields_ = [
@@ -204,6 +234,11 @@ SIGNATURES = {
     "ggq_kv_load_dev": (_I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(KvSeqs), _P, _I, _P, _I64, _P, _I64, _I, _P]),
     "ggq_attention_kv_dev": (_I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(KvSeqs), _P, _I64, _I, ctypes.c_float, _I,
                                   _P, _I64, _P]),
+    "ggq_attention_kv_rows_dev": (_I, [_P, ctypes.POINTER(KvCache), ctypes.POINTER(KvSeqs), _P, _I, _P, _I64, _I,
+                                       ctypes.c_float, _I, _P, _I64, _P]),
+    "ggq_delta_rule_dev": (_I, [_P, ctypes.POINTER(DeltaRuleParams), _P]),
+    "ggq_norm_dev": (_I, [_P, ctypes.POINTER(NormParams), _P]),
+    "ggq_sample_dev": (_I, [_P, ctypes.POINTER(SampleParams), _P]),
     "ggq_attention_prompt_dev": (_I, [_P, ctypes.POINTER(AttnPromptParams), _P]),
     "ggq_mul_mat_q8_batch_dev": (_I, [_P, _P, _I, _U32, _I64, _P, _P, _I, _P]),
     "ggq_dequant_dev": (_I, [_P, _P, _U32, _I64, _P, _P]),

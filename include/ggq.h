@@ -378,6 +378,23 @@ int ggq_kv_load_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* 
 int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const float* q, int64_t ldq,
                          int n_head, float scale, int window, float* out, int64_t ldo, void* stream);
 
+/* The same for several rows of each sequence (a prompt's next part, proposed
+ * tokens to be checked, prompts and single tokens in one call): rows
+ * row_off[s] .. row_off[s+1]-1 of q and out (device, [n_seq + 1], ascending,
+ * within n_rows; NULL: row s for sequence s) are the last ones of sequence s,
+ * as a store call with the same offsets has put them into the cache.  The last
+ * row sits at position len[s] - 1, each row before it one earlier; a row sees
+ * its own position and those before it, with window > 0 the last `window` of
+ * those.  Rows in front of position 0 see nothing and get zeros, and so does
+ * a row whose positions have no page; rows of no sequence stay as they were.
+ * Positions that a row does not see, or that have no page, do not count,
+ * whatever they hold; a row that sees a key or value that reads back as NaN has no
+ * defined result (the others keep theirs).  Products are exact in fp32
+ * terms, as above.  q and out 16-byte aligned, ldq and ldo multiples of 4. */
+int ggq_attention_kv_rows_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off,
+                              int n_rows, const float* q, int64_t ldq, int n_head, float scale, int window, float* out,
+                              int64_t ldo, void* stream);
+
 /* Causal attention of whole prompts (prefill), packed one behind the other:
  * rows q_off[s] .. q_off[s+1]-1 of q and out and rows kv_off[s] ..
  * kv_off[s+1]-1 of k and v belong to sequence s (device, [n_seq + 1] each,
@@ -425,6 +442,138 @@ typedef struct {
     int window;  /* 0: none */
 } ggq_attention_prompt_params;
 int ggq_attention_prompt_dev(ggq_ctx* ctx, const ggq_attention_prompt_params* params, void* stream);
+
+/* Gated delta rule, the token mixer of linear attention layers (qwen35 and
+ * qwen35moe have one in three of four layers): each head keeps a state S of
+ * k_dim x v_dim numbers instead of a cache.  Per row t of a sequence:
+ *   S = exp(g_t) S;  S = S + b_t k_t (v_t - S^T k_t)^T;  out_t = scale * S^T q_t
+ * with g_t (the decay's logarithm, normally <= 0; -infinity forgets
+ * everything) and b_t of the row's head.  Value head h reads the q and k of
+ * head h / (n_v_head / n_k_head).  gate and beta are g and b as they are, or
+ *   gate_rate set:          g = gate_rate[h] * softplus(gate + gate_bias[h])
+ *                           (gate_bias NULL: 0; a GGUF file's ssm_a and ssm_dt.bias)
+ *   GGQ_DELTA_BETA_SIGMOID  b = 1 / (1 + exp(-beta))
+ *   GGQ_DELTA_QK_NORM       q and k are divided by sqrt(sum(x^2) + eps) first
+ * Sequences are packed: rows row_off[s] .. row_off[s+1]-1 (device, [n_seq +
+ * 1], ascending, within n_rows; NULL: row s is sequence s's only one).  Sequence
+ * s starts from state[slot[s]] and leaves state_out[slot[s]] (device, [n_slots]
+ * [n_v_head][v_dim][k_dim] fp32; slot NULL: s); state_out may be state itself.
+ * A slot belongs to one sequence of a call at most.  A sequence whose slot lies
+ * outside [0, n_slots) is passed over: its rows of out stay as they were.  One
+ * without rows has its state copied.  Slots of no sequence and rows of no
+ * sequence stay as they were.
+ * All sums and states are fp32.  Sequences of up to about 24 rows in the mean
+ * go row by row, longer ones in parts of 16 rows, for which the rows' values are
+ * solved together (the same result, rounded in another order); without workspace
+ * for that (a buffer per stream, as for the matmuls) they go row by row.
+ * Rows are dense heads: q and k [n_k_head][k_dim], v and out
+ * [n_v_head][v_dim], gate and beta [n_v_head], with row strides ld*.  k_dim
+ * 64, 128 or 256, v_dim a multiple of 16 up to 512; all pointers but gate,
+ * beta, gate_rate, gate_bias, slot and row_off 16-byte aligned, ldq, ldk, ldv and ldo
+ * multiples of 4. */
+#define GGQ_DELTA_BETA_SIGMOID 1
+#define GGQ_DELTA_QK_NORM 2
+typedef struct {
+    int n_k_head, n_v_head, k_dim, v_dim;
+    const float* q;
+    int64_t ldq;
+    const float* k;
+    int64_t ldk;
+    const float* v;
+    int64_t ldv;
+    const float* gate;
+    int64_t ld_gate;
+    const float* beta;
+    int64_t ld_beta;
+    const float* gate_rate; /* [n_v_head] or NULL */
+    const float* gate_bias; /* [n_v_head] or NULL */
+    int flags;
+    float eps;
+    float scale; /* 0: 1 / sqrt(k_dim) */
+    const float* state;
+    float* state_out;
+    int n_slots;
+    const int32_t* slot; /* [n_seq] or NULL */
+    int n_seq;
+    int n_rows;
+    const int32_t* row_off; /* [n_seq + 1] or NULL */
+    float* out;
+    int64_t ldo;
+} ggq_delta_rule_params;
+int ggq_delta_rule_dev(ggq_ctx* ctx, const ggq_delta_rule_params* params, void* stream);
+
+/* What stands between two layers' matmuls, in one launch: the residual's
+ * addition, RMSNorm, and the next matmul's input as fp32 rows, as int8
+ * codes, or both.  Per row:
+ *   s = x + add                          (add NULL: x); to `sum` where that is set
+ *   y = s / sqrt(mean(s^2) + eps) * norm_w  over groups of norm_len values (0: the
+ *                                        row; a head's values for the norm of heads)
+ *   y = y * silu(gate)                   where gate is set (the gated norm behind
+ *                                        linear attention), silu(z) = z / (1 + exp(-z))
+ * s is rounded to fp32 once, y is made from it in 64 bits and rounded once.
+ * out receives y; codes and scales what ggq_quantize_act_dev makes of y in
+ * act_mode GGQ_ACT_Q8_ROW or GGQ_ACT_Q8_BLOCK32 (GGQ_ACT_F32: none), for
+ * ggq_mul_mat_q8_dev and ggq_mul_mat_q8_batch_dev.  sum may be x or add
+ * itself, and out may be x, with the same stride; other overlaps are not allowed.
+ * n_cols a multiple of 4 (of 32 for Q8_BLOCK32), at most 32768; norm_len a
+ * multiple of 4 that divides n_cols; pointers 16-byte aligned (scales 4), strides multiples of 4,
+ * codes dense.  ggq_produce_quantize_act_dev is the form without residual,
+ * heads, gate and fp32 rows, in fp32 steps. */
+typedef struct {
+    int n_rows, n_cols;
+    const float* x;
+    int64_t ldx;
+    const float* add; /* or NULL */
+    int64_t ld_add;
+    float* sum; /* or NULL */
+    int64_t ld_sum;
+    const float* norm_w; /* [norm_len] or NULL (= 1) */
+    int norm_len;
+    float eps;
+    const float* gate; /* or NULL */
+    int64_t ld_gate;
+    float* out; /* or NULL */
+    int64_t ldo;
+    int act_mode;
+    int8_t* codes;
+    float* scales;
+} ggq_norm_params;
+int ggq_norm_dev(ggq_ctx* ctx, const ggq_norm_params* params, void* stream);
+
+/* One token of each row of logits, drawn by a given random number: the form
+ * of ggq_logits_argmax_dev for temperatures above 0.  Row m has temperature T,
+ * top_k, top_p and min_p (device, [n_rows] each; NULL: 1, off, off, off) and
+ * a random number u in [0, 1).  A token's weight is w = exp((logit - largest) / T).
+ * Tokens are in order of their logits, the lower index first among equals,
+ * and what is kept of them is a head of that order:
+ *   top_k > 0   the first top_k
+ *   top_p < 1   of those, the fewest whose weights sum to top_p of all of those or more
+ *   min_p > 0   those with w >= min_p
+ * and always the first one.  token[m] is the first kept one, in order of the
+ * indices, with which the running sum of the kept weights exceeds u times their
+ * sum (the last one with a weight if rounding lets none); prob[m] (NULL: not
+ * wanted) its share of the sum.  T = 0 (or below, or NaN) takes the first token,
+ * prob 1.  NaN and -infinity have no weight; where nothing is above -infinity the
+ * token is 0 and prob 0.  A logit of +infinity has weight 1 and all finite ones none.
+ * A NaN in top_p or min_p means off, in u 0.
+ * Weights are within 2^-33, their sums within 2^-30 of 64 bits': a token changes only
+ * when u falls that close to the border between two.  A weight below 2^-60 of the largest counts as
+ * that of its order alone: it is kept or not, but not drawn (u = 0 takes the first token that is).
+ * Row stride ld >= n_vocab (any alignment of 4 bytes); n_vocab up to 2^22, n_rows up to 65535. */
+typedef struct {
+    int n_rows;
+    int n_vocab;
+    const float* logits;
+    int64_t ld;
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* u;
+    int32_t* token;
+    float* prob;
+} ggq_sample_params;
+int ggq_sample_dev(ggq_ctx* ctx, const ggq_sample_params* params, void* stream);
 
 /* C = sa[m] * sum_k qa[m][k] * w[n][k]: the GGQ_ACT_Q8_ROW matmul on
  * activations already quantized by ggq_quantize_act_dev (row mode; qa dense
