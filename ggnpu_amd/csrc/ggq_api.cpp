@@ -1353,6 +1353,7 @@ int ggq_delta_rule_dev(ggq_ctx* c, const ggq_delta_rule_params* p, void* stream)
     const int64_t krow = (int64_t)p->n_k_head * p->k_dim, vrow = (int64_t)p->n_v_head * p->v_dim;
     if (p->ldq < krow || p->ldk < krow || p->ldv < vrow || p->ldo < vrow || p->ld_gate < p->n_v_head || p->ld_beta < p->n_v_head)
         return set_status(c, GGQ_INVALID_PARAM, "row strides must hold a row's heads");
+    if (std::max({p->ldq, p->ldk, p->ldv, p->ldo}) > 1 << 24) return set_status(c, GGQ_INVALID_PARAM, "row strides above 2^24 values");
     if (p->flags & ~(GGQ_DELTA_BETA_SIGMOID | GGQ_DELTA_QK_NORM)) return set_status(c, GGQ_INVALID_PARAM, "unknown flags %d", p->flags);
     if (p->n_seq < 0 || p->n_seq > 65535 || p->n_rows < 0 || p->n_slots < 0 || !std::isfinite(p->scale) || !(p->eps >= 0.0f))
         return set_status(c, GGQ_INVALID_PARAM, "need n_seq in 0..65535, n_rows and n_slots >= 0, a finite scale and eps >= 0");

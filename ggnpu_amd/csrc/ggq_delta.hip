@@ -44,7 +44,7 @@ struct DeltaArgs {
 constexpr int kRows = 16;  // rows of a part
 // A part's record of one value head, in floats: T diag(b) and A [16][16], then factors of its rows: of K S, of Q S,
 // of U on its way into the state; the state's own.
-constexpr int kT = 0, kA = 256, kKc = 512, kQc = 528, kKs = 544, kDec = 560, kRecord = 576;
+constexpr int kT = 0, kA = 256, kKc = 512, kQc = 528, kKs = 544, kDec = 560, kRecord = 576;  // (kDec: 16 times)
 
 // Sequence s has the parts from off / 16 + s on: a bound that needs no sum over the sequences before.
 struct Seq {
@@ -185,12 +185,10 @@ struct Log {
 __device__ __forceinline__ float exp_of(Log a, Log b) { return expf((a.hi - b.hi) + (a.lo - b.lo)); }
 
 template <int KD>
-__global__ __launch_bounds__(256) void delta_parts_kernel(DeltaArgs a, int n_parts) {
+__global__ __launch_bounds__(256) void delta_parts_kernel(DeltaArgs a) {
     constexpr int NT = KD / 16;
-    __shared__ float s_kk[4][16][17], s_qk[4][16][17];
-    __shared__ __attribute__((aligned(16))) float s_m[4][4][16][20];
-    __shared__ float s_row[4][4][16][4];  // of a head's rows: b, hi, lo
-    __shared__ float s_r[4][16][2];       // of the rows: factors of k and q
+    // M, then its inverse, of four heads; of their rows: step, sum of logarithms, factor of q
+    __shared__ __attribute__((aligned(16))) float s_m[4][4][16][20], s_row[4][4][16][4];
     const ggq_delta_rule_params& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
     const int id = blockIdx.x;
@@ -211,6 +209,15 @@ __global__ __launch_bounds__(256) void delta_parts_kernel(DeltaArgs a, int n_par
     for (int t = 0; t < NT; t++) k[t] = *(const float4*)(kp + 16 * t);
 #pragma unroll
     for (int t = 0; t < NT; t++) q[t] = *(const float4*)(qp + 16 * t);
+    // of the first four heads, a head a group of lanes
+    const int G = p.n_v_head / p.n_k_head;
+    float ld = 0.0f, b = 0.0f;
+    auto gates = [&](int h0) {
+        const int h = hk * G + min(h0 + g, G - 1);
+        ld = r < n ? decay_of(p, row, h) : 0.0f;
+        b = r < n ? step_of(p, row, h) : 0.0f;
+    };
+    gates(0);
     f32x4 kk{0, 0, 0, 0}, qk{0, 0, 0, 0};
     float sk = 0.0f, sq2 = 0.0f;
 #pragma unroll
@@ -234,18 +241,10 @@ __global__ __launch_bounds__(256) void delta_parts_kernel(DeltaArgs a, int n_par
         rq = a.scale / sqrtf(sq2 + p.eps);
     }
     if (r >= n) rk = rq = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        s_kk[wave][4 * g + e][r] = kk[e];
-        s_qk[wave][4 * g + e][r] = qk[e];
-    }
-    if (g == 0) { s_r[wave][r][0] = rk; s_r[wave][r][1] = rq; }
-    const int G = p.n_v_head / p.n_k_head;
     for (int h0 = 0; h0 < G; h0 += 4) {
-        const int h = hk * G + min(h0 + g, G - 1);
-        float ld = r < n ? decay_of(p, row, h) : 0.0f;
-        ld = fminf(fmaxf(ld, -1000.0f), 1000.0f) + (ld - ld == 0.0f || ld == INFINITY || ld == -INFINITY ? 0.0f : ld);  // (NaN stays)
-        const float b = r < n ? step_of(p, row, h) : 0.0f;
+        if (h0) gates(h0);
+        // (NaN stays)
+        ld = fminf(fmaxf(ld, -1000.0f), 1000.0f) + (ld - ld == 0.0f || ld == INFINITY || ld == -INFINITY ? 0.0f : ld);
         Log L;
         L.hi = __builtin_rintf(ld * 256.0f) * (1.0f / 256.0f);
         L.lo = ld - L.hi;
@@ -255,130 +254,245 @@ __global__ __launch_bounds__(256) void delta_parts_kernel(DeltaArgs a, int n_par
             if (r >= o) { L.hi += x; L.lo += y; }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        s_row[wave][g][r][0] = b;
-        s_row[wave][g][r][1] = L.hi;
-        s_row[wave][g][r][2] = L.lo;
+        *(float4*)s_row[wave][g][r] = make_float4(b * rk, L.hi, L.lo, rq);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        // this lane's column r of M and A
-        float* rec = a.parts + ((int64_t)id * p.n_v_head + h) * kRecord;
-        const bool mine = h0 + g < G;
+        // M and A of each head: rows 4 g + e of column r in this lane
+        const int nh = min(4, G - h0);
+        for (int x = 0; x < nh; x++) {
+            float* rec = a.parts + ((int64_t)id * p.n_v_head + hk * G + h0 + x) * kRecord;
+            const float4 cr = *(const float4*)s_row[wave][x][r];
+            const Log lr{cr.y, cr.z};
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float* x = s_row[wave][g][i];
-            const float e = i >= r ? exp_of(Log{x[1], x[2]}, L) : 0.0f;
-            s_m[wave][g][i][r] = i > r ? x[0] * s_r[wave][i][0] * e * rk * s_kk[wave][i][r] : 0.0f;
-            if (mine) rec[kA + 16 * i + r] = i >= r ? s_r[wave][i][1] * e * rk * s_qk[wave][i][r] : 0.0f;
+            for (int e = 0; e < 4; e++) {
+                const int i = 4 * g + e;
+                const float4 ci = *(const float4*)s_row[wave][x][i];
+                const float d = i >= r ? exp_of(Log{ci.y, ci.z}, lr) * rk : 0.0f;
+                s_m[wave][x][i][r] = i > r ? ci.x * d * kk[e] : 0.0f;
+                rec[kA + 16 * i + r] = i >= r ? ci.w * d * qk[e] : 0.0f;
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        // column r of (1 + M)^-1, from the top
+        // column r of (1 + M)^-1 of head g, from the top
+        const int mine = min(g, nh - 1);
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             float v = i == r ? 1.0f : 0.0f;
 #pragma unroll
-            for (int m = 0; m < i; m++) v = fmaf(-s_m[wave][g][i][m], x[m], v);
+            for (int m = 0; m < i; m += 4) {
+                const float4 w = *(const float4*)&s_m[wave][mine][i][m];
+                v = fmaf(-w.x, x[m], v);
+                if (m + 1 < i) v = fmaf(-w.y, x[m + 1], v);
+                if (m + 2 < i) v = fmaf(-w.z, x[m + 2], v);
+                if (m + 3 < i) v = fmaf(-w.w, x[m + 3], v);
+            }
             x[i] = v;
         }
-        if (!mine) continue;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (g < nh) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) rec[kT + 16 * i + r] = x[i] * b;
-        const Log end{s_row[wave][g][15][1], s_row[wave][g][15][2]};
-        const float c = expf(L.hi + L.lo);
-        rec[kKc + r] = c * rk;
-        rec[kQc + r] = c * rq;
-        rec[kKs + r] = exp_of(end, L) * rk;
-        if (r == 0) rec[kDec] = expf(end.hi + end.lo);
+            for (int i = 0; i < 16; i++) s_m[wave][g][i][r] = x[i] * b;
+            float* rec = a.parts + ((int64_t)id * p.n_v_head + hk * G + h0 + g) * kRecord;
+            const float4 last = *(const float4*)s_row[wave][g][15];
+            const Log end{last.y, last.z};
+            const float c = expf(L.hi + L.lo);
+            rec[kKc + r] = c * rk;
+            rec[kQc + r] = c * rq;
+            rec[kKs + r] = exp_of(end, L) * rk;
+            rec[kDec + r] = expf(end.hi + end.lo);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int x = 0; x < nh; x++) {
+            float* rec = a.parts + ((int64_t)id * p.n_v_head + hk * G + h0 + x) * kRecord;
+            *(float4*)(rec + kT + 4 * lane) = *(const float4*)&s_m[wave][x][lane >> 2][4 * (lane & 3)];
+        }
     }
 }
 
+// 64 lanes' 16 bytes at src + each lane's offset into LDS at lds + 16 lane.  The caller waits on the vector memory
+// counter.  (m0 is reserved: the compiler sets it right before its own uses.)
+__device__ __forceinline__ void dma16(const void* src, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(src) : "memory");
+}
+
+// A part in LDS: K, Q (16-byte runs of row i exclusive-ored with i, which keeps both ways of reading them off each
+// other's banks), V's 16 columns, the record (and what lies behind it, so that all loads are alike).  `slots` parts are
+// under way.
+template <int KD> struct Ring {
+    static constexpr int kq = kRows * KD * 4, v = 2 * kq, rec = v + 1024, bytes = rec + 3072;
+    static constexpr int slots = KD == 64 ? 8 : KD == 128 ? 6 : 3;
+    static constexpr int loads = KD / 32 + 1;  // of a wavefront, a part
+};
+
+// Wavefronts 0 to 3 have a quarter of k each; 4 to 7, which share their SIMDs, load the parts to come and write the
+// results of those that are done, while the others wait for products.
 template <int KD>
-__global__ __launch_bounds__(256) void delta_scan_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
     constexpr int NT = KD / 64;  // tiles of 16 numbers of k of a wavefront
+    constexpr int RPR = KD / 4;  // 16-byte runs of a row
+    typedef Ring<KD> R;
+    static_assert(R::slots * R::bytes < 128 * 1024, "LDS that global_load_lds addresses");
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[R::slots * R::bytes];
     __shared__ __attribute__((aligned(16))) f32x4 s_ks[2][4][64], s_o[2][4][64];
     const ggq_delta_rule_params& p = a.p;
     const int h = blockIdx.x, seq = blockIdx.z, v0 = blockIdx.y * 16;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
+    const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave8 & 3;
     const int slot = slot_of(p, seq);
     if (slot < 0) return;
     const Seq sq = seq_of(p, seq);
-    const int hk = h / (p.n_v_head / p.n_k_head), k0 = wave * NT * 16;
-    const int64_t at = (((int64_t)slot * p.n_v_head + h) * p.v_dim + v0 + r) * KD + k0 + 4 * g;
+    const int hk = h / (p.n_v_head / p.n_k_head);
+    const int parts = (sq.n + kRows - 1) / kRows, last_row = sq.n - 1;
+    auto after = [](int in) { return in + 1 == R::slots ? 0 : in + 1; };
+
+    if (wave8 >= 4) {
+        if (!parts) return;
+        const float *kp = p.k + sq.row * p.ldk + (int64_t)hk * KD, *qp = p.q + sq.row * p.ldq + (int64_t)hk * KD;
+        const float* vp = p.v + sq.row * p.ldv + (int64_t)h * p.v_dim + v0;
+        float* op = p.out + sq.row * p.ldo + (int64_t)h * p.v_dim + v0;
+        // (one of them loads V, the others the record)
+        const float* rec0 = a.parts + (sq.part * p.n_v_head + h) * kRecord + (wave - 1) * 256;
+        // loads of part i into slot `in` (behind the last part: that one again, so that their number stays).  A lane's offsets
+        // from a part's first row: of whole parts, and of the last one, whose rows end with the sequence's
+        constexpr int NL = KD / 64;
+        const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
+        uint32_t ko[2][NL], qo[2][NL], ro[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            const int most = w ? last_row - (parts - 1) * kRows : kRows - 1;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int x = (wave * NL + j) * 64 + lane, row = x / RPR, run = x % RPR ^ (row & 15);
+                ko[w][j] = 4u * ((uint32_t)min(row, most) * (uint32_t)p.ldk + 4u * run);  // (strides of up to 2^24)
+                qo[w][j] = 4u * ((uint32_t)min(row, most) * (uint32_t)p.ldq + 4u * run);
+            }
+            ro[w] = wave ? 16u * lane : 4u * ((uint32_t)min(lane >> 2, most) * (uint32_t)p.ldv + 4u * (lane & 3));
+        }
+        const int64_t rest_step = wave ? (int64_t)p.n_v_head * kRecord : (int64_t)kRows * p.ldv;
+        const float* rest0 = wave ? rec0 : vp;
+        auto fetch = [&](int i, int in) {
+            const uint32_t to = lds_at + (uint32_t)in * R::bytes;
+            const int pt = min(i, parts - 1);
+            const bool end = pt == parts - 1;
+            const float *kb = kp + (int64_t)pt * kRows * p.ldk, *qb = qp + (int64_t)pt * kRows * p.ldq;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                dma16(kb, end ? ko[1][j] : ko[0][j], to + (uint32_t)(wave * NL + j) * 1024u);
+                dma16(qb, end ? qo[1][j] : qo[0][j], to + R::kq + (uint32_t)(wave * NL + j) * 1024u);
+            }
+            dma16(rest0 + (int64_t)pt * rest_step, end ? ro[1] : ro[0], to + R::v + (uint32_t)wave * 1024u);
+        };
+        auto put = [&](int i) {  // the wavefronts' parts of O, 4 rows a wavefront
+            const int row = i * kRows + 4 * wave + g;
+            const float* o = (const float*)s_o[i & 1] + (wave * 16 + r) * 4 + g;
+            const float v = (o[0] + o[256]) + (o[512] + o[768]);
+            if (row <= last_row) op[row * p.ldo + r] = v;
+        };
+        // (the counter also counts this wavefront's stores: a smaller number outstanding than loads only waits longer)
+        for (int i = 0; i < R::slots - 1; i++) fetch(i, i);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((R::slots - 2) * R::loads) : "memory");
+        int before = R::slots - 1;
+        for (int i = 0; i < parts; i++) {
+            fetch(i + R::slots - 1, before);  // over the part before i, which nobody reads any more
+            before = after(before);
+            if (i > 1) put(i - 2);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((R::slots - 2) * R::loads) : "memory");
+        }
+        // (no load may come into LDS that is another workgroup's by then)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (parts > 1) put(parts - 2);
+        put(parts - 1);
+        return;
+    }
+
+    const int tile0 = wave * NT;
+    const int64_t at = (((int64_t)slot * p.n_v_head + h) * p.v_dim + v0 + r) * KD + 16 * tile0 + 4 * g;
     f32x4 s[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) s[t] = *(const f32x4*)(p.state + at + 16 * t);
-    const float *kp = p.k + sq.row * p.ldk + (int64_t)hk * KD + k0, *qp = p.q + sq.row * p.ldq + (int64_t)hk * KD + k0;
-    const float* vp = p.v + sq.row * p.ldv + (int64_t)h * p.v_dim + v0 + r;
-    float* op = p.out + sq.row * p.ldo + (int64_t)h * p.v_dim + v0;
-    const float* rec0 = a.parts + (sq.part * p.n_v_head + h) * kRecord;
-    const int parts = (sq.n + kRows - 1) / kRows;
     struct In {
-        f32x4 k[NT], q[NT], kt[NT], v, t, kc, qc, ks;
-        float a, dec;
+        f32x4 k[NT], q[NT];
     };
-    auto load = [&](int i, In& x) {
-        const int last = sq.n - 1, n0 = i * kRows;
-        const int row = min(n0 + r, last);
-        const float* rec = rec0 + (int64_t)i * p.n_v_head * kRecord;
+    auto rows_in = [&](int in, In& x) {
+        const uint8_t* from = ring + in * R::bytes;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            x.k[t] = *(const f32x4*)(kp + row * p.ldk + 16 * t + 4 * g);
-            x.q[t] = *(const f32x4*)(qp + row * p.ldq + 16 * t + 4 * g);
+            const int at_run = (r * RPR + ((4 * (tile0 + t) + g) ^ r)) * 16;
+            x.k[t] = *(const f32x4*)(from + at_run);
+            x.q[t] = *(const f32x4*)(from + R::kq + at_run);
         }
+    };
+    // One part.  Issue is in order, so what waits stands in the shadow of products: this part's other operands beside
+    // K S, the sums' way through LDS beside Q S.
+    auto step = [&](int i, int in, const In& cur, In& nxt) {
+        const uint8_t* from = ring + in * R::bytes;
+        const float *rec = (const float*)(from + R::rec), *vin = (const float*)(from + R::v);
+        f32x4 ks[2] = {}, qs[2] = {};
+        auto q_s = [&](int first, int last) {
+#pragma unroll
+            for (int x = first; x < last; x++)
+                qs[x & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.q[x % NT][x / NT], s[x % NT][x / NT], qs[x & 1], 0, 0, 0);
+        };
+#pragma unroll
+        for (int x = 0; x < 4 * NT; x++)
+            ks[x & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.k[x % NT][x / NT], s[x % NT][x / NT], ks[x & 1], 0, 0, 0);
+        f32x4 v, kt[NT];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int y = min(n0 + 4 * g + e, last);
+            v[e] = vin[(4 * g + e) * 16 + r];
 #pragma unroll
-            for (int t = 0; t < NT; t++) x.kt[t][e] = kp[y * p.ldk + 16 * t + r];
-            x.v[e] = vp[y * p.ldv];
+            for (int t = 0; t < NT; t++)
+                kt[t][e] = ((const float*)from)[((4 * g + e) * RPR + ((4 * (tile0 + t) + (r >> 2)) ^ (4 * g + e))) * 4 + (r & 3)];
         }
-        x.t = *(const f32x4*)(rec + kT + 16 * r + 4 * g);
-        x.a = rec[kA + 16 * r + 4 * g + wave];
-        x.kc = *(const f32x4*)(rec + kKc + 4 * g);
-        x.qc = *(const f32x4*)(rec + kQc + 4 * g);
-        x.ks = *(const f32x4*)(rec + kKs + 4 * g);
-        x.dec = rec[kDec];
-    };
-    auto put = [&](int i) {  // the wavefronts' parts of O, 4 rows a wavefront
-        const int row = i * kRows + 4 * wave + g;
-        const float* o = (const float*)s_o[i & 1] + (wave * 16 + r) * 4 + g;
-        const float v = (o[0] + o[256]) + (o[512] + o[768]);
-        if (row < sq.n) op[row * p.ldo + r] = v;
-    };
-    In cur, nxt;
-    if (parts) load(0, cur);
-    for (int i = 0; i < parts; i++) {
-        if (i + 1 < parts) load(i + 1, nxt);
-        f32x4 ks{0, 0, 0, 0}, qs{0, 0, 0, 0};
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) ks = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.k[t][e], s[t][e], ks, 0, 0, 0);
-        s_ks[i & 1][wave][lane] = ks;
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) qs = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.q[t][e], s[t][e], qs, 0, 0, 0);
-        __syncthreads();
-        if (i) put(i - 1);
+        const f32x4 tr = *(const f32x4*)(rec + kT + 16 * r + 4 * g), kc = *(const f32x4*)(rec + kKc + 4 * g);
+        const f32x4 qc = *(const f32x4*)(rec + kQc + 4 * g), kf = *(const f32x4*)(rec + kKs + 4 * g);
+        const float ar = rec[kA + 16 * r + 4 * g + wave], dec = rec[kDec];
+        __builtin_amdgcn_sched_barrier(0);
+        q_s(0, NT);
+        __builtin_amdgcn_sched_barrier(0);
+        s_ks[i & 1][wave][lane] = ks[0] + ks[1];
+        __builtin_amdgcn_sched_barrier(0);
+        q_s(NT, 2 * NT);
+        __builtin_amdgcn_sched_barrier(0);
+        // the next part's loads have come and the sums are in LDS
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const f32x4* x = &s_ks[i & 1][0][lane];
-        ks = (x[0] + x[64]) + (x[128] + x[192]);
-        const f32x4 rest = cur.v - cur.kc * ks;
+        const f32x4 x0 = x[0], x1 = x[64], x2 = x[128], x3 = x[192];
+        rows_in(after(in), nxt);  // (behind the last part: that one again)
+        __builtin_amdgcn_sched_barrier(0);
+        q_s(2 * NT, 4 * NT);
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x4 rest = v - kc * ((x0 + x1) + (x2 + x3));
         f32x4 u{0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 4; e++) u = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.t[e], rest[e], u, 0, 0, 0);
-        const float ue = wave == 0 ? u[0] : wave == 1 ? u[1] : wave == 2 ? u[2] : u[3];
-        s_o[i & 1][wave][lane] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.a, ue, qs * cur.qc, 0, 0, 0);
-        u *= cur.ks;
+        for (int e = 0; e < 4; e++) u = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[e], rest[e], u, 0, 0, 0);
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            s[t] *= cur.dec;
+        for (int t = 0; t < NT; t++) s[t] *= dec;
+        const f32x4 of = (qs[0] + qs[1]) * qc;
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x4 w = u * kf;
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.kt[t][e], u[e], s[t], 0, 0, 0);
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kt[t][e], w[e], s[t], 0, 0, 0);
+        const int wv = tid >> 6;
+        const float ue = wv == 0 ? u[0] : wv == 1 ? u[1] : wv == 2 ? u[2] : u[3];
+        s_o[i & 1][wave][lane] = __builtin_amdgcn_mfma_f32_16x16x4f32(ar, ue, of, 0, 0, 0);
+    };
+    if (parts) {
+        __syncthreads();
+        In x, y;
+        rows_in(0, x);
+        int in = 0;
+        for (int i = 0; i < parts; i += 2) {
+            step(i, in, x, y);
+            in = after(in);
+            if (i + 1 == parts) break;
+            step(i + 1, in, y, x);
+            in = after(in);
         }
-        cur = nxt;
+        __syncthreads();
     }
-    __syncthreads();
-    if (parts) put(parts - 1);
 #pragma unroll
     for (int t = 0; t < NT; t++) *(f32x4*)(p.state_out + at + 16 * t) = s[t];
 }
@@ -388,9 +502,9 @@ int64_t parts_of(const ggq_delta_rule_params& p) { return (int64_t)p.n_rows / kR
 template <int KD> hipError_t delta_launch(const DeltaArgs& a, bool parts, hipStream_t s) {
     const ggq_delta_rule_params& p = a.p;
     if (parts) {
-        delta_parts_kernel<KD><<<dim3((unsigned)parts_of(p), (unsigned)((p.n_k_head + 3) / 4)), 256, 0, s>>>(a, (int)parts_of(p));
+        delta_parts_kernel<KD><<<dim3((unsigned)parts_of(p), (unsigned)((p.n_k_head + 3) / 4)), 256, 0, s>>>(a);
         // (heads first: the slices of one head share its rows in one XCD's L2 where there is a multiple of 8 heads)
-        delta_scan_kernel<KD><<<dim3((unsigned)p.n_v_head, (unsigned)(p.v_dim / 16), (unsigned)p.n_seq), 256, 0, s>>>(a);
+        delta_scan_kernel<KD><<<dim3((unsigned)p.n_v_head, (unsigned)(p.v_dim / 16), (unsigned)p.n_seq), 512, 0, s>>>(a);
         return hipGetLastError();
     }
     constexpr int C = KD == 256 ? 2 : 4;
@@ -408,7 +522,7 @@ size_t delta_ws_bytes(const ggq_delta_rule_params& p) {
     if (!p.row_off) return 0;
     const char* env = getenv("GGQ_DELTA_PARTS");
     if (env && *env ? atoi(env) == 0 : p.n_rows <= 24 * (int64_t)p.n_seq) return 0;
-    return sizeof(float) * kRecord * (size_t)parts_of(p) * p.n_v_head;
+    return sizeof(float) * (kRecord * (size_t)parts_of(p) * p.n_v_head + 256);  // (the last record's loads go 192 floats further)
 }
 
 hipError_t launch_delta(const ggq_delta_rule_params& p, void* ws, hipStream_t s) {

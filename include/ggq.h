@@ -470,7 +470,7 @@ int ggq_attention_prompt_dev(ggq_ctx* ctx, const ggq_attention_prompt_params* pa
  * [n_v_head][v_dim], gate and beta [n_v_head], with row strides ld*.  k_dim
  * 64, 128 or 256, v_dim a multiple of 16 up to 512; all pointers but gate,
  * beta, gate_rate, gate_bias, slot and row_off 16-byte aligned, ldq, ldk, ldv and ldo
- * multiples of 4. */
+ * multiples of 4, at most 2^24. */
 #define GGQ_DELTA_BETA_SIGMOID 1
 #define GGQ_DELTA_QK_NORM 2
 typedef struct {
