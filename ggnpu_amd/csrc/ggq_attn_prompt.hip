@@ -41,6 +41,7 @@
 #include "ggq_attn.h"
 #include "ggq_attn_device.h"
 #include "ggq_launch.h"
+#include "ggq_steps.h"
 
 namespace ggq {
 namespace {
@@ -70,7 +71,25 @@ template <> struct Head<256> {
 template <int HD> constexpr int64_t unit_bytes(int planes) { return (int64_t)planes * 2 * kUnit * HD * 2 + Head<HD>::bytes; }
 // Exponents between that of an all-zero row of values and its unit's (an int16_t with the sign changed).
 constexpr int kZero = 4096;
-enum { BAD_V = 1 << 20, NO_V = 1 << 21, OWN_K = 1 << 22, OWN_V = 1 << 23 };
+enum { BAD_V = 1 << 20, NO_V = 1 << 21, OWN_K = 1 << 22, OWN_V = 1 << 23, NO_PAGE = 1 << 24 };
+
+// Where keys and values come from: rows of float or _Float16, or the records of a quantized cache, whose codes
+// have at most 4 significant bits and need one plane, under powers of two as fp32 rows (exact but for values 2^36 below the
+// largest of their unit).
+template <int KB, int VB> struct Codes {};
+typedef Codes<0, 0> AnyCodes;  // (the attention itself does not need to know)
+template <typename T> struct Source {
+    static constexpr bool cache = true, powers = true;
+    static constexpr int planes = 1;
+};
+template <> struct Source<float> {
+    static constexpr bool cache = false, powers = true;
+    static constexpr int planes = 2;
+};
+template <> struct Source<_Float16> {
+    static constexpr bool cache = false, powers = false;
+    static constexpr int planes = 1;
+};
 
 // Sequence s has the units from off[s] / 32 + s on (and as many column tiles of
 // n from off[s] * G / n + s): a bound that needs no sum over the sequences before.
@@ -82,6 +101,9 @@ struct PromptArgs {
     float* part;
     int G, tiles, splits;
     int kv0, kvn;  // the kv heads of this launch, whose planes there is room for
+    KvChunkArgs kv;   // keys and values of a cache:
+    int units;        // room for as many units of each sequence
+    int64_t record;   // bytes of a record
 };
 
 // A sequence's rows of an offset array, held inside [0, n].
@@ -95,6 +117,24 @@ __device__ __forceinline__ Span span_of(const int32_t* off, int s, int64_t most)
 // The first position that a row with `below` positions at or before its own sees (below < 1: none are).  A window
 // may be anything up to INT32_MAX: nothing is subtracted from a negative number.
 __device__ __forceinline__ int first_of(int below, int window) { return window ? max(max(below, 0) - window, 0) : 0; }
+// A sequence of a cache: its length, the positions there may be pages for, the first unit that its rows see.
+struct Cached {
+    int len, lim, first;
+};
+__device__ __forceinline__ Cached cached_of(const PromptArgs& a, int s, int rows) {
+    Cached c;
+    c.len = max(a.kv.q.len[s], 0);
+    c.lim = (int)min(min((int64_t)c.len, (int64_t)a.kv.q.max_len), (int64_t)a.kv.q.table_len * a.kv.c.page_len);
+    c.first = first_of(c.len - rows + 1, a.p.window) / kUnit;
+    return c;
+}
+// The record of a unit (null: there is none).
+__device__ __forceinline__ const uint8_t* record_of(const PromptArgs& a, int s, int kvh, int u) {
+    const int tpp = a.kv.c.page_len / kUnit;
+    const int32_t page = a.kv.q.pages[(int64_t)s * a.kv.q.table_len + u / tpp];
+    if (page < 0 || page >= a.kv.c.n_pages) return nullptr;
+    return (const uint8_t*)a.kv.c.pages + (((int64_t)page * a.kv.c.n_kv_head + kvh) * tpp + u % tpp) * a.record;
+}
 __device__ __forceinline__ const int32_t* kv_off_of(const ggq_attention_prompt_params& p) { return p.kv_off ? p.kv_off : p.q_off; }
 
 __device__ __forceinline__ uint32_t mag_bits(float v) {  // 0 for what is not finite
@@ -247,39 +287,112 @@ __global__ __launch_bounds__(256) void attn_few_kernel(PromptArgs a) {
     }
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// N codes from their bytes, as fp32.
+template <int BITS, int N> __device__ __forceinline__ void decode(const uint8_t* at, float s, float* x) {
+    constexpr int W = N * BITS / 32 > 0 ? N * BITS / 32 : 1;
+    uint32_t w[W];
+    if constexpr (N * BITS == 16) w[0] = *(const uint16_t*)at;
+    else if constexpr (N * BITS == 32) w[0] = *(const uint32_t*)at;
+    else if constexpr (N * BITS == 64) {
+        const uint2 v = *(const uint2*)at;
+        w[0] = v.x; w[1] = v.y;
+    } else {
+        const uint4 v = *(const uint4*)at;
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        f32x2 v;
+        if constexpr (BITS == 4) {
+            switch (i % 8 / 2) {  // the byte is an immediate
+            case 0: v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i / 8], s, 0); break;
+            case 1: v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i / 8], s, 1); break;
+            case 2: v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i / 8], s, 2); break;
+            default: v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i / 8], s, 3); break;
+            }
+        } else {
+            v = i % 4 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i / 4], s, true) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i / 4], s, false);
+        }
+        x[i] = v[0];
+        x[i + 1] = v[1];
+    }
+}
+// A thread's HD / 8 values of its position from a record (include/ggq.h has the places).
+template <int HD, int KB, int VB> __device__ __forceinline__ void codes_in(const uint8_t* rec, int pos, int d0, float* k, float* v) {
+    constexpr int V = HD / 8, VD = HD / 16;
+    const uint8_t *vc = rec + kUnit * HD * KB / 8, *ks = vc + kUnit * HD * VB / 8, *vs = ks + HD;
+    const int blk = d0 / 32;
+    const float sk = scale_of(ks[(16 * blk + pos % 16) * 2 + pos / 16]);
+    const float sv = scale_of(vs[(4 * blk + pos % 16 / 4) * 8 + 4 * (pos / 16) + pos % 4]);
+    constexpr int KN = V * KB > 128 ? 128 / KB : V;  // codes of one load
+#pragma unroll
+    for (int i = 0; i < V; i += KN) {
+        const int b = (pos / 16 * (HD / 4) + (d0 + i) % (HD / 4)) * KB / 8;
+        decode<KB, KN>(rec + 1024 * (b / 16) + 16 * (16 * (d0 / (HD / 4)) + pos % 16) + b % 16, sk, k + i);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int b = (4 * (pos / 16) + pos % 4) * VD * VB / 8;
+        decode<VB, VD>(vc + 1024 * (b / 16) + 16 * (16 * (pos % 16 / 4) + d0 / VD + i) + b % 16, sv, v + i * VD);
+    }
+}
+template <typename T> struct Bits;
+template <int KB, int VB> struct Bits<Codes<KB, VB>> {
+    static constexpr int k = KB, v = VB;
+};
+
 template <int HD, typename T>
 __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
-    constexpr int P = sizeof(T) == 4 ? 2 : 1, V = HD / 8;  // planes, values of a thread
-    constexpr int PL = kUnit * HD;                         // values of a plane
+    constexpr int P = Source<T>::planes, V = HD / 8;  // planes, values of a thread
+    constexpr bool W = Source<T>::powers;
+    constexpr int PL = kUnit * HD;                    // values of a plane
     __shared__ float sv[kUnit][HD + 1];
     __shared__ uint32_t red[4][3];
     const int tid = threadIdx.x, kvh = a.kv0 + blockIdx.y;
-    const int32_t* off = kv_off_of(a.p);
     const int64_t id = blockIdx.x;
-    int seq = 0;
-    for (int i = 1; i < a.p.n_seq; i += 256) {
-        const int j = i + tid;
-        seq += __syncthreads_count(j < a.p.n_seq && bound_of(max(off[j], 0), kUnit, j) <= id);
-    }
-    const Span sp = span_of(off, seq, a.p.n_kv_rows);
-    const int64_t u = id - bound_of(sp.a, kUnit, seq);
-    if (u < 0 || u * kUnit >= sp.n) return;
     const int pos = tid / 8, d0 = tid % 8 * V;
-    const bool in = u * kUnit + pos < sp.n;
-    const int64_t row = sp.a + min(u * kUnit + pos, sp.n - 1);
-    struct alignas(16) Run { T x[16 / sizeof(T)]; };
-    constexpr int PR = 16 / sizeof(T), NR = V / PR;
-    const Run* kr = (const Run*)((const T*)a.p.k + row * a.p.ldk + (int64_t)kvh * HD + d0);
-    const Run* vr = (const Run*)((const T*)a.p.v + row * a.p.ldv + (int64_t)kvh * HD + d0);
-    Run kin[NR], vin[NR];
-#pragma unroll
-    for (int i = 0; i < NR; i++) { kin[i] = kr[i]; vin[i] = vr[i]; }
+    bool in;
     float k[V], v[V];
     uint32_t mk = 0, mv = 0, bad = 0;
+    if constexpr (Source<T>::cache) {
+        const int seq = (int)(id / a.units);
+        const Cached c = cached_of(a, seq, (int)span_of(a.p.q_off, seq, a.p.n_rows).n);
+        const int u = c.first + (int)(id % a.units);
+        if ((int64_t)u * kUnit >= c.lim) return;
+        const uint8_t* rec = record_of(a, seq, kvh, u);
+        if (!rec) bad = NO_PAGE;
+        in = rec && u * kUnit + pos < c.lim;
+        if (in) codes_in<HD, Bits<T>::k, Bits<T>::v>(rec, pos, d0, k, v);
+    } else {
+        const int32_t* off = kv_off_of(a.p);
+        int seq = 0;
+        for (int i = 1; i < a.p.n_seq; i += 256) {
+            const int j = i + tid;
+            seq += __syncthreads_count(j < a.p.n_seq && bound_of(max(off[j], 0), kUnit, j) <= id);
+        }
+        const Span sp = span_of(off, seq, a.p.n_kv_rows);
+        const int64_t u = id - bound_of(sp.a, kUnit, seq);
+        if (u < 0 || u * kUnit >= sp.n) return;
+        in = u * kUnit + pos < sp.n;
+        const int64_t row = sp.a + min(u * kUnit + pos, sp.n - 1);
+        struct alignas(16) Run { T x[16 / sizeof(T)]; };
+        constexpr int PR = 16 / sizeof(T), NR = V / PR;
+        const Run* kr = (const Run*)((const T*)a.p.k + row * a.p.ldk + (int64_t)kvh * HD + d0);
+        const Run* vr = (const Run*)((const T*)a.p.v + row * a.p.ldv + (int64_t)kvh * HD + d0);
+        Run kin[NR], vin[NR];
+#pragma unroll
+        for (int i = 0; i < NR; i++) { kin[i] = kr[i]; vin[i] = vr[i]; }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            k[i] = (float)kin[i / PR].x[i % PR];
+            v[i] = (float)vin[i / PR].x[i % PR];
+        }
+    }
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        k[i] = in ? (float)kin[i / PR].x[i % PR] : 0.0f;
-        v[i] = in ? (float)vin[i / PR].x[i % PR] : 0.0f;
+        k[i] = in ? k[i] : 0.0f;
+        v[i] = in ? v[i] : 0.0f;
         mk = max(mk, mag_bits(k[i]));
         mv = max(mv, mag_bits(v[i]));
         if (!finite(v[i])) {
@@ -311,13 +424,13 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
     uv = max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1]));
     bad = red[0][2] | red[1][2] | red[2][2] | red[3][2];
     // fp16 values stay as they are
-    const int ku = P == 2 ? up_to_2_15(uk) : 0, vu = P == 2 ? up_to_2_15(uv) : 0;
-    int ke = P == 2 && mk ? up_to_2_15(mk) : ku, ve = P == 2 && mv ? up_to_2_15(mv) : vu;
+    const int ku = W ? up_to_2_15(uk) : 0, vu = W ? up_to_2_15(uv) : 0;
+    int ke = W && mk ? up_to_2_15(mk) : ku, ve = W && mv ? up_to_2_15(mv) : vu;
     if (ke <= ku + 8) ke = ku;
     if (ve <= vu + 8) ve = vu;
     // values that are all zero have any exponent: one that stands for no value (of a unit with others: hidden ones
     // must not lend it theirs)
-    if (P == 2 && in && !mv && uv) ve = vu + kZero;
+    if (W && in && !mv && uv) ve = vu + kZero;
     const int own_k = __syncthreads_or(ke != ku), own_v = __syncthreads_or(ve != vu);
     typedef typename Head<HD>::num num;
     uint8_t* out = a.planes + (id * a.kvn + (kvh - a.kv0)) * unit_bytes<HD>(P);
@@ -334,7 +447,7 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
         h8 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float x = P == 2 ? ldexpf(k[i + j], ke) : k[i + j];
+            const float x = W ? ldexpf(k[i + j], ke) : k[i + j];
             hi[j] = (_Float16)x;
             lo[j] = (_Float16)(x - (float)hi[j]);  // (NaN for an infinity)
         }
@@ -344,7 +457,7 @@ __global__ __launch_bounds__(256) void planes_kernel(PromptArgs a) {
         if constexpr (P == 2) *(h8*)(at + PL) = lo;
     }
 #pragma unroll
-    for (int i = 0; i < V; i++) sv[pos][d0 + i] = P == 2 ? ldexpf(v[i], ve) : v[i];
+    for (int i = 0; i < V; i++) sv[pos][d0 + i] = W ? ldexpf(v[i], ve) : v[i];
     __syncthreads();
     _Float16* vp = kp + P * PL;
     for (int e = tid; e < HD * 4; e += 256) {  // (value, step of 16 positions, half)
@@ -396,9 +509,23 @@ __device__ __forceinline__ void phase_end(bool loads) {
     else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// Whether position x of a record has a value that reads back as NaN.
+template <int HD> __device__ bool nan_value(const ggq_kv_cache& c, const uint8_t* rec, int x) {
+    const int VB = c.v_type, VD = HD / 16;
+    const uint8_t *vc = rec + kUnit * HD * c.k_type / 8, *vs = vc + kUnit * HD * VB / 8 + HD;
+    for (int blk = 0; blk < HD / 32; blk++)
+        if (vs[(4 * blk + x % 16 / 4) * 8 + 4 * (x / 16) + x % 4] == 255) return true;
+    for (int e = 0; VB == 8 && e < HD; e++) {
+        const int b = (4 * (x / 16) + x % 4) * VD + e % VD;
+        if ((vc[1024 * (b / 16) + 16 * (16 * (x % 16 / 4) + e / VD) + b % 16] & 127) == 127) return true;
+    }
+    return false;
+}
+
 template <int HD, typename T>
 __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a) {
-    constexpr int P = sizeof(T) == 4 ? 2 : 1, NW = waves_of<HD>(), PL = kUnit * HD * 2;  // PL: bytes of a plane
+    constexpr bool W = Source<T>::powers;
+    constexpr int P = Source<T>::planes, NW = waves_of<HD>(), PL = kUnit * HD * 2;  // PL: bytes of a plane
     constexpr int64_t UB = unit_bytes<HD>(P);
     typedef typename Head<HD>::num num;
     constexpr int HB = Head<HD>::bytes, KB = HB + P * PL, VB = P * PL;          // LDS bytes of a unit's header and keys, of its values
@@ -419,11 +546,16 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         const int j = i + tid;
         seq += __syncthreads_count(j < p.n_seq && (int)((uint32_t)max(min(p.q_off[j], p.n_rows), 0) * G / NC) + j <= id);
     }
-    const Span qs = span_of(p.q_off, seq, p.n_rows), ks = span_of(kv_off_of(p), seq, p.n_kv_rows);
+    const Span qs = span_of(p.q_off, seq, p.n_rows);
+    Span ks{0, 0};
+    Cached kc{0, 0, 0};
+    if constexpr (Source<T>::cache) kc = cached_of(a, seq, (int)qs.n);
+    else ks = span_of(kv_off_of(p), seq, p.n_kv_rows);
     // (n_rows * G fits 31 bits: the caller sees to it)
     const int nf = (int)qs.n * G, f0 = (id - ((int)((uint32_t)qs.a * G / NC) + seq)) * NC;
     if (f0 < 0 || f0 >= nf) return;
-    const int n_keys = (int)ks.n, shift = n_keys - (int)qs.n + 1;  // row i sees positions below shift + i
+    // row i sees positions below shift + i, of those that there are
+    const int n_keys = Source<T>::cache ? kc.lim : (int)ks.n, shift = (Source<T>::cache ? kc.len : (int)ks.n) - (int)qs.n + 1;
     const int i0 = (int)((uint32_t)f0 / G), i1 = (int)((uint32_t)(min(nf, f0 + NC) - 1) / G);
     const int wg_end = min(max(shift + i1, 0), n_keys);
     const int wg_beg = first_of(shift + i0, p.window);
@@ -435,7 +567,8 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     // there is, the nearest unit: the same number of loads each time).  Two of the four wavefronts
     // that load take the keys, two the values, LD KB in a row each.
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    const uint8_t* units = a.planes + ((bound_of(ks.a, kUnit, seq) + u0) * a.kvn + kvi) * UB;
+    const int64_t unit0 = Source<T>::cache ? (int64_t)seq * a.units - kc.first : bound_of(ks.a, kUnit, seq);
+    const uint8_t* units = a.planes + ((unit0 + u0) * a.kvn + kvi) * UB;
     const int64_t stride = a.kvn * UB;
     const int share = wave & 3;
     const bool of_k = share < 2;
@@ -524,7 +657,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             for (int j = 0; j < 4; j++) x[i + j] = v.x[j];
         }
     };
-    int dv[P == 2 ? 16 : 1];
+    int dv[W ? 16 : 1];
     auto open = [&](int it) { info = __builtin_amdgcn_readfirstlane(*(const uint32_t*)(lds + (it & 1) * KB + Head<HD>::info)); };
     auto scores = [&](int it) {
         const h8* kp = (const h8*)(lds + (it & 1) * KB + HB) + lane;
@@ -541,7 +674,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     auto powers = [&](int it) {
         const uint8_t* slot = lds + (it & 1) * KB;
         // (the slot is loaded over before the weights of the wavefronts behind)
-        if constexpr (P == 2) {
+        if constexpr (W) {
             if (info & OWN_K) {  // (scores in one step: the unit's exponent may be that of hidden keys, far from the seen ones')
                 const int ku = (int)(info & 1023u) - 512;
                 int dk[16];
@@ -555,19 +688,19 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
     h8 ph[2], pl[2];
     auto weights = [&](int it) {
         const int base = (u0 + it) * kUnit;
-        const bool masked = masks(it);
+        const bool masked = masks(it) || (Source<T>::cache && (info & NO_PAGE));
         const int ku = (int)(info & 1023u) - 512, vu = (int)(info >> 10 & 1023u) - 512;
         bad |= info;
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int at = base + 8 * (i / 4) + 4 * h + i % 4;
-                if (at >= end || at < beg) st[i] = -INFINITY;
+                if (at >= end || at < beg || (Source<T>::cache && (info & NO_PAGE))) st[i] = -INFINITY;
             }
         }
         // to powers of two, where powers() has not (an exponent beyond fp32's range gives a score of 0 or an infinite one
         // either way)
-        const float cs = P == 2 && (info & OWN_K) ? 1.0f : ldexpf(1.0f, max(-126, min(127, -(qe + ku))));
+        const float cs = W && (info & OWN_K) ? 1.0f : ldexpf(1.0f, max(-126, min(127, -(qe + ku))));
         float top = max3(st[0], st[1], st[2]);
 #pragma unroll
         for (int i = 3; i < 15; i += 2) top = max3(top, st[i], st[i + 1]);
@@ -576,7 +709,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         if (__any(top > m + 4.0f)) {
             const float mn = max3(m, top, top);
             const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
-            if (P == 2 && m > -INFINITY) least = min(least + (int)fminf(mn - m, 4096.0f), kNone);  // (so much do the sums shrink)
+            if (W && m > -INFINITY) least = min(least + (int)fminf(mn - m, 4096.0f), kNone);  // (so much do the sums shrink)
             m = mn;
             l *= al;
 #pragma unroll
@@ -584,7 +717,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         }
         // the weights' power of two besides 2^(11 - m)
         int c = 0;
-        if constexpr (P == 2) {
+        if constexpr (W) {
             // In the sums' unit a position's weight times value is 2^(s - m + ve - its exponent): `heavy` is the largest
             // s - m - (exponent - vu) that the column sees, `roof` the ve up to which its weight stays within 2^15.
             float heavy = top - m;
@@ -622,8 +755,8 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
             e[i] = __builtin_amdgcn_exp2f(fmaf(st[i], cs, -ref));
             sum[i & 1] += e[i];
         }
-        l += P == 2 ? ldexpf(sum[0] + sum[1], -c) : sum[0] + sum[1];
-        if constexpr (P == 2) {
+        l += W ? ldexpf(sum[0] + sum[1], -c) : sum[0] + sum[1];
+        if constexpr (W) {
             if (info & OWN_V) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) e[i] = ldexpf(e[i], dv[i] + (ve - vu));
@@ -707,8 +840,19 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         // infinities and NaN among the values are zero in the planes: here they come, to the rows that see them
         for (int u = u0; u < u1; u++) {
             if (!(*(const uint32_t*)(units + (u - u0) * stride + Head<HD>::info) & BAD_V)) continue;
+            if constexpr (Source<T>::cache) {  // (a NaN, whose row has no defined result)
+                const uint8_t* rec = record_of(a, seq, kvh, u);
+                if (!rec) continue;
+                for (int x = max(u * kUnit, beg) - u * kUnit; x < min((u + 1) * kUnit, end) - u * kUnit; x++)
+                    if (nan_value<HD>(a.kv.c, rec, x)) {
+#pragma unroll
+                        for (int d = 0; d < DB; d++) o[d] += __builtin_nanf("");
+                    }
+                continue;
+            } else
             for (int at = max(u * kUnit, beg); at < min((u + 1) * kUnit, end); at++) {
-                const T* vr = (const T*)p.v + (ks.a + at) * p.ldv + (int64_t)kvh * HD + 4 * h;
+                typedef typename std::conditional<Source<T>::cache, float, T>::type E;
+                const E* vr = (const E*)p.v + (ks.a + at) * p.ldv + (int64_t)kvh * HD + 4 * h;
 #pragma unroll
                 for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -720,7 +864,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         }
     }
     const float inv = 1.0f / l;
-    const bool none = end <= beg;
+    const bool none = end <= beg || (Source<T>::cache && m == -INFINITY && l == 0.0f);  // (nothing but positions without a page)
     float* part = a.part + (((qs.a + qi) * p.n_head + head) * a.splits + split) * (HD + 4);
     const bool whole = a.splits == 1, empty = whole ? none : m == -INFINITY && l == 0.0f;
     // the row's result, or this part's weighted mean with its maximum and its sum
@@ -842,6 +986,87 @@ hipError_t launch_attn_prompt(const ggq_attention_prompt_params& p, const AttnPr
     else { BY_T(256) }
 #undef BY_T
 #undef L
+    return hipGetLastError();
+}
+
+// ---- keys and values of a cache
+namespace {
+template <int HD> int64_t kv_unit_bytes() { return unit_bytes<HD>(1); }
+// Units of a sequence that its rows may see.
+int kv_units_of(const KvChunkArgs& a) {
+    const int64_t span = std::min<int64_t>(a.q.max_len, (int64_t)a.q.table_len * a.c.page_len);
+    int64_t n = (span + kUnit - 1) / kUnit;
+    if (a.window > 0) n = std::min<int64_t>(n, ((int64_t)a.window + a.n_rows + kUnit - 1) / kUnit + 1);
+    return (int)std::max<int64_t>(n, 1);
+}
+ggq_attention_prompt_params prompt_of(const KvChunkArgs& a) {
+    ggq_attention_prompt_params p{};
+    p.n_head = a.n_head;
+    p.n_kv_head = a.c.n_kv_head;
+    p.head_dim = a.c.head_dim;
+    p.q = a.Q;
+    p.ldq = a.ldq;
+    p.out = a.out;
+    p.ldo = a.ldo;
+    p.n_rows = a.n_rows;
+    p.n_seq = a.q.n_seq;
+    p.q_off = a.row_off;
+    p.scale = a.scale;
+    p.window = a.window;
+    return p;
+}
+size_t kv_head_bytes(const KvChunkArgs& a) {
+    const int hd = a.c.head_dim;
+    return (size_t)kv_units_of(a) * a.q.n_seq * (hd == 64 ? kv_unit_bytes<64>() : hd == 128 ? kv_unit_bytes<128>() : kv_unit_bytes<256>());
+}
+int kv_heads_at_once(const KvChunkArgs& a) {
+    return (int)std::max<size_t>(1, std::min<size_t>((size_t)a.c.n_kv_head, (size_t(256) << 20) / kv_head_bytes(a)));
+}
+size_t kv_planes_bytes(const KvChunkArgs& a) { return (kv_head_bytes(a) * kv_heads_at_once(a) + 255) / 256 * 256; }
+
+template <int HD, int KB, int VB> void kv_planes_go(const PromptArgs& a, hipStream_t s) {
+    planes_kernel<HD, Codes<KB, VB>><<<dim3((unsigned)((int64_t)a.units * a.p.n_seq), (unsigned)a.kvn), 256, 0, s>>>(a);
+}
+template <int HD> void kv_go(PromptArgs& a, int at_once, hipStream_t s) {
+    const ggq_kv_cache& c = a.kv.c;
+    for (a.kv0 = 0; a.kv0 < c.n_kv_head; a.kv0 += at_once) {
+        a.kvn = std::min(at_once, c.n_kv_head - a.kv0);
+        if (c.k_type == GGQ_KV_MXFP4) c.v_type == GGQ_KV_MXFP4 ? kv_planes_go<HD, 4, 4>(a, s) : kv_planes_go<HD, 4, 8>(a, s);
+        else c.v_type == GGQ_KV_MXFP4 ? kv_planes_go<HD, 8, 4>(a, s) : kv_planes_go<HD, 8, 8>(a, s);
+        attn_kernel<HD, AnyCodes><<<dim3((unsigned)(a.tiles * (int64_t)a.kvn), (unsigned)a.splits), waves_of<HD>() * 64, 0, s>>>(a);
+    }
+    if (a.splits > 1) attn_join_kernel<HD><<<dim3((unsigned)(((int64_t)a.p.n_rows * a.p.n_head + 3) / 4)), 256, 0, s>>>(a);
+}
+}  // namespace
+
+AttnPromptPlan attn_kv_planes_plan(const KvChunkArgs& a) {
+    AttnPromptPlan pl{};
+    const ggq_attention_prompt_params p = prompt_of(a);
+    const int64_t wgs = tiles_of(p) * p.n_kv_head, units = kv_units_of(a);
+    const int64_t n = std::min<int64_t>(cu_count() / wgs, units / 4);
+    pl.splits = n > 1 && units * (n - 1) > 4 * n ? (int)n : 1;
+    if (const char* e = getenv("GGQ_PROMPT_SPLITS"); e && atoi(e) > 0)
+        pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(atoi(e), 256), units));
+    pl.ws_bytes = kv_planes_bytes(a);
+    if (pl.splits > 1) pl.ws_bytes += sizeof(float) * (size_t)p.n_rows * p.n_head * pl.splits * (p.head_dim + 4);
+    return pl;
+}
+
+hipError_t launch_attn_kv_planes(const KvChunkArgs& k, const AttnPromptPlan& pl, void* ws, hipStream_t s) {
+    PromptArgs a{};
+    a.p = prompt_of(k);
+    a.kv = k;
+    a.units = kv_units_of(k);
+    a.record = kv_record_bytes(k.c);
+    a.planes = (uint8_t*)ws;
+    a.part = (float*)((char*)ws + kv_planes_bytes(k));
+    a.G = k.n_head / k.c.n_kv_head;
+    a.splits = pl.splits;
+    a.tiles = (int)tiles_of(a.p);
+    const int at_once = kv_heads_at_once(k);
+    if (k.c.head_dim == 64) kv_go<64>(a, at_once, s);
+    else if (k.c.head_dim == 128) kv_go<128>(a, at_once, s);
+    else kv_go<256>(a, at_once, s);
     return hipGetLastError();
 }
 

@@ -410,10 +410,10 @@ template <int HD, int KB, int VB> int splits_go(const KvChunkArgs& a, int ct, in
 }
 
 template <int HD, int KB, int VB> hipError_t chunk_go(const KvChunkArgs& a, const KvChunkPlan& pl, float* ws, hipStream_t s) {
-    const dim3 grid((unsigned)tiles_of(a, 16 * pl.kind), (unsigned)a.c.n_kv_head, (unsigned)pl.splits);
+    const dim3 grid((unsigned)tiles_of(a, 16 * pl.tiles), (unsigned)a.c.n_kv_head, (unsigned)pl.splits);
     bool done = false;
     if constexpr (HD < 256)
-        if (pl.kind == 2) {
+        if (pl.tiles == 2) {
             kv_chunk_kernel<HD, KB, VB, 2><<<grid, chunk_waves<HD, 2>() * 64, 0, s>>>(a, pl.splits, ws);
             done = true;
         }
@@ -430,24 +430,32 @@ template <int HD, int KB, int VB> hipError_t chunk_go(const KvChunkArgs& a, cons
 
 KvChunkPlan kv_chunk_plan(const KvChunkArgs& a, bool workspace) {
     const ggq_kv_cache& c = a.c;
-    KvChunkPlan pl{1, 1, 0};
+    KvChunkPlan pl{1, {}, 1, 0};
     // two tiles a wavefront where a sequence's pairs fill more than one
     const int64_t pairs = (int64_t)a.n_rows * (a.n_head / c.n_kv_head);
-    if (c.head_dim < 256 && pairs > 16 * (int64_t)a.q.n_seq) pl.kind = 2;
+    if (c.head_dim < 256 && pairs > 16 * (int64_t)a.q.n_seq) pl.tiles = 2;
     if (!workspace) return pl;
+    const char* env = getenv("GGQ_KV_PLANES");
+    if (a.row_off && (env && *env ? atoi(env) != 0 : pairs >= 256 * (int64_t)a.q.n_seq)) {
+        pl.tiles = 0;
+        pl.planes = attn_kv_planes_plan(a);
+        pl.ws_bytes = pl.planes.ws_bytes;
+        return pl;
+    }
     int64_t span = std::min<int64_t>(a.q.max_len, (int64_t)a.q.table_len * c.page_len);
     if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + a.n_rows / a.q.n_seq + kKvTile);
     const int64_t records = (span + kKvTile - 1) / kKvTile;
     if (const char* e = getenv("GGQ_KV_SPLITS"); e && atoi(e) > 0)
         pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(atoi(e), kMaxSplits), records));
-    else if (c.head_dim == 64) pl.splits = GGQ_BY_CACHE(64, splits_go, a, pl.kind, records);
-    else if (c.head_dim == 128) pl.splits = GGQ_BY_CACHE(128, splits_go, a, pl.kind, records);
-    else pl.splits = GGQ_BY_CACHE(256, splits_go, a, pl.kind, records);
+    else if (c.head_dim == 64) pl.splits = GGQ_BY_CACHE(64, splits_go, a, pl.tiles, records);
+    else if (c.head_dim == 128) pl.splits = GGQ_BY_CACHE(128, splits_go, a, pl.tiles, records);
+    else pl.splits = GGQ_BY_CACHE(256, splits_go, a, pl.tiles, records);
     if (pl.splits > 1) pl.ws_bytes = sizeof(float) * (size_t)a.n_rows * a.n_head * pl.splits * (c.head_dim + 2);
     return pl;
 }
 
 hipError_t launch_kv_chunk(const KvChunkArgs& a, const KvChunkPlan& pl, void* ws, hipStream_t s) {
+    if (!pl.tiles) return launch_attn_kv_planes(a, pl.planes, ws, s);
     const ggq_kv_cache& c = a.c;
     if (c.head_dim == 64) return GGQ_BY_CACHE(64, chunk_go, a, pl, (float*)ws, s);
     if (c.head_dim == 128) return GGQ_BY_CACHE(128, chunk_go, a, pl, (float*)ws, s);

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "../../include/ggq.h"
+#include "ggq_attn.h"
 
 namespace ggq {
 
@@ -36,10 +37,15 @@ struct KvChunkArgs {
     int64_t ldo;
 };
 struct KvChunkPlan {
-    int splits, kind;
+    int tiles;              // column tiles of a wavefront; 0: by planes of operands, as prompts
+    AttnPromptPlan planes;
+    int splits;
     size_t ws_bytes;
 };
 KvChunkPlan kv_chunk_plan(const KvChunkArgs& a, bool workspace);
 hipError_t launch_kv_chunk(const KvChunkArgs& a, const KvChunkPlan& pl, void* ws, hipStream_t s);
+// (ggq_attn_prompt.hip)
+AttnPromptPlan attn_kv_planes_plan(const KvChunkArgs& a);
+hipError_t launch_attn_kv_planes(const KvChunkArgs& a, const AttnPromptPlan& pl, void* ws, hipStream_t s);
 
 }  // namespace ggq
