@@ -1042,7 +1042,9 @@ template <int HD> void kv_go(PromptArgs& a, int at_once, hipStream_t s) {
 AttnPromptPlan attn_kv_planes_plan(const KvChunkArgs& a) {
     AttnPromptPlan pl{};
     const ggq_attention_prompt_params p = prompt_of(a);
-    const int64_t wgs = tiles_of(p) * p.n_kv_head, units = kv_units_of(a);
+    // (workgroups with work: of sequences of the mean length)
+    const int64_t nc = (p.head_dim == 256 ? 4 : 8) * 32, pairs = ((int64_t)p.n_rows + p.n_seq - 1) / p.n_seq * (p.n_head / p.n_kv_head);
+    const int64_t wgs = std::max<int64_t>(1, (pairs + nc - 1) / nc) * p.n_seq * p.n_kv_head, units = kv_units_of(a);
     const int64_t n = std::min<int64_t>(cu_count() / wgs, units / 4);
     pl.splits = n > 1 && units * (n - 1) > 4 * n ? (int)n : 1;
     if (const char* e = getenv("GGQ_PROMPT_SPLITS"); e && atoi(e) > 0)

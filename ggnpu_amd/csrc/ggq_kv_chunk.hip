@@ -22,9 +22,10 @@
 namespace ggq {
 namespace {
 
-// Sequence s has the column tiles of n from off[s] * G / n + s on: a bound that needs no sum over the sequences before.
-__device__ __forceinline__ int tile_of(const KvChunkArgs& a, int s, int G, int n) {
-    return (int)((uint32_t)min(max(a.row_off ? a.row_off[s] : s, 0), a.n_rows) * (uint32_t)G / (uint32_t)n) + s;
+// Column tiles of n of a sequence's rows off0 .. off1 - 1.
+__device__ __forceinline__ int tiles_in(int off0, int off1, int n_rows, int G, int n) {
+    const int rows = min(max(off1, 0), n_rows) - min(max(off0, 0), n_rows);
+    return (int)(((uint32_t)max(rows, 0) * (uint32_t)G + (uint32_t)n - 1) / (uint32_t)n);
 }
 
 // Three bf16 parts of x hold all its 24 bits: x cut, what is left cut, what is left then.
@@ -41,32 +42,75 @@ __device__ __forceinline__ void parts_of(float a, float b, uint32_t (&w)[3]) {
     w[2] = bf16_pack(a, b);
 }
 
-template <int HD, int CT> constexpr int chunk_waves() { return HD * CT >= 256 ? 4 : 8; }
+template <int HD, int CT> constexpr int chunk_waves() { return 4; }
+// Wavefronts of a SIMD, by their registers.
+template <int HD, int CT> constexpr int chunk_side() { return HD * CT <= 128 ? 4 : 2; }
 
 template <int HD, int KB, int VB, int CT>
-__global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(KvChunkArgs a, int splits, float* part) {
+__global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>())) void kv_chunk_kernel(KvChunkArgs a, int splits, float* part) {
     constexpr int NW = chunk_waves<HD, CT>(), NC = 16 * CT;
     constexpr int KW = HD * KB / 64, VW = HD * VB / 64;  // dwords of a lane's K and V codes
     constexpr int NS = HD / 32;                          // k steps of S^T, blocks of a head
     constexpr int NO = HD / 16;                          // row tiles of O^T
     constexpr int VD = HD / 16;                          // values of a lane's V at one position
     constexpr int64_t RB = kKvTile * HD * (KB + VB) / 8 + 2 * HD;
-    __shared__ float sm[NW][NC], sl[NW][NC], so[NW][NC][HD + 1];
+    __shared__ float sm[NW][NC], sl[NW][NC];
+    // the parts of q, and in the end the wavefronts' sums
+    constexpr int SQ = CT * NS * 3 * 64 * 16, SO = NW * NC * (HD + 1) * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[SQ > SO ? SQ : SO];
+    auto sq = (bf16x8(*)[NS][3][64])lds;
+    auto so = (float(*)[NC][HD + 1])lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r = lane & 15;
     const int kvh = blockIdx.y, split = blockIdx.z, id = blockIdx.x;
     const int G = a.n_head / a.c.n_kv_head;  // query heads of this kv head
     const int tpp = a.c.page_len / kKvTile;
-    int seq = 0;
-    for (int i = 1; i < a.q.n_seq; i += NW * 64) {
+    // The tile's sequence: tiles are numbered through, by a running sum over the offsets.  (Numbers behind the last tile are
+    // the last workgroups: they do not hold up others.)
+    __shared__ int32_t s_sum[NW], s_find[5];
+    if (tid == 0) s_find[0] = -1;
+    int before = 0;
+    for (int i = 0; i < a.q.n_seq; i += NW * 64) {
         const int j = i + tid;
-        seq += __syncthreads_count(j < a.q.n_seq && tile_of(a, j, G, NC) <= id);
+        int off0 = 0, off1 = 0, len = 0;
+        if (j < a.q.n_seq) {
+            off0 = a.row_off ? a.row_off[j] : j;
+            off1 = a.row_off ? a.row_off[j + 1] : j + 1;
+            len = a.q.len[j];
+        }
+        const int mine = tiles_in(off0, off1, a.n_rows, G, NC);
+        int run = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(run, o, 64);
+            if (lane >= o) run += t;
+        }
+        __syncthreads();
+        if (lane == 63) s_sum[wave] = run;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            if (w < wave) run += s_sum[w];
+            all += s_sum[w];
+        }
+        run += before;
+        if (id >= run - mine && id < run) {
+            s_find[1] = id - (run - mine);
+            s_find[2] = min(max(off0, 0), a.n_rows);
+            s_find[3] = min(max(off1, 0), a.n_rows);
+            s_find[4] = len;
+            s_find[0] = j;
+        }
+        before += all;
+        __syncthreads();
+        if (s_find[0] >= 0) break;
     }
-    const int r0 = min(max(a.row_off ? a.row_off[seq] : seq, 0), a.n_rows);
-    const int nr = min(max(a.row_off ? a.row_off[seq + 1] : seq + 1, 0), a.n_rows) - r0;
-    const int nf = max(nr, 0) * G, f0 = (id - tile_of(a, seq, G, NC)) * NC;
-    if (f0 < 0 || f0 >= nf) return;
-    const int64_t len = a.q.len[seq], lim = min(min(len, (int64_t)a.q.max_len), (int64_t)a.q.table_len * a.c.page_len);
+    const int seq = __builtin_amdgcn_readfirstlane(s_find[0]);
+    if (seq < 0) return;
+    const int r0 = __builtin_amdgcn_readfirstlane(s_find[2]), nr = __builtin_amdgcn_readfirstlane(s_find[3]) - r0;
+    const int nf = nr * G, f0 = __builtin_amdgcn_readfirstlane(s_find[1]) * NC;
+    const int64_t len = __builtin_amdgcn_readfirstlane(s_find[4]), lim = min(min(len, (int64_t)a.q.max_len), (int64_t)a.q.table_len * a.c.page_len);
     // columns: pair f has row f / G at position len - nr + f / G; it sees positions beg .. end - 1
     auto end_of = [&](int f) { return len - nr + f / G + 1; };
     auto see = [&](int f, int& b, int& e) {
@@ -74,14 +118,11 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(
         e = (int)max(min(x, lim), (int64_t)0);
         b = a.window > 0 ? (int)max(x - a.window, (int64_t)0) : 0;
     };
-    int beg[CT], end[CT], fc[CT];
-    bool live[CT];
+    int beg[CT], end[CT];
 #pragma unroll
     for (int n = 0; n < CT; n++) {
         const int f = f0 + 16 * n + r;
-        live[n] = f < nf;
-        fc[n] = min(f, nf - 1);
-        see(fc[n], beg[n], end[n]);
+        see(min(f, nf - 1), beg[n], end[n]);
     }
     // rows ascend with the columns: the first and the last bound what any and what all of them see
     int lo, all_hi, all_lo, hi;
@@ -92,24 +133,6 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(
     if (per > NW) per = (per + NW - 1) / NW * NW;
     const int first = t0 + split * per, last = min(t1, first + per);
 
-    Frag qf[CT][NS][3];
-#pragma unroll
-    for (int n = 0; n < CT; n++) {
-        const int qi = fc[n] / G, h = fc[n] - qi * G;
-        const float* qp = a.Q + (int64_t)(r0 + qi) * a.ldq + (int64_t)(kvh * G + h) * HD + g * (HD / 4);
-#pragma unroll
-        for (int s = 0; s < NS; s++) {
-            const float4 u = *(const float4*)(qp + 8 * s), v = *(const float4*)(qp + 8 * s + 4);
-            const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t w[3];
-                parts_of(x[2 * i] * a.scale, x[2 * i + 1] * a.scale, w);
-#pragma unroll
-                for (int j = 0; j < 3; j++) qf[n][s][j].w[i] = w[j];
-            }
-        }
-    }
     f32x4 o[CT][NO];
     float m[CT], l[CT];
 #pragma unroll
@@ -181,10 +204,11 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(
 #pragma unroll
             for (int j = 2; j >= 0; j--)
 #pragma unroll
-                for (int t = 0; t < 2; t++)
+                for (int n = 0; n < CT; n++) {
+                    const bf16x8 q = sq[n][s][j][lane];
 #pragma unroll
-                    for (int n = 0; n < CT; n++)
-                        st[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t].v, qf[n][s][j].v, st[t][n], 0, 0, 0);
+                    for (int t = 0; t < 2; t++) st[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t].v, q, st[t][n], 0, 0, 0);
+                }
         }
         uint32_t poison = 0;  // positions whose values read back as NaN, which some columns see and some do not
         if (partial) {
@@ -300,6 +324,24 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(
     Rec cur, nxt;
     look(0);
     if (n_it > 0) load(0, cur);
+    // the columns' parts in the order of the operands, for all wavefronts
+    for (int x = tid; x < CT * NS * 64; x += NW * 64) {
+        const int n = x / (NS * 64), s = x / 64 % NS, fq = min(f0 + 16 * n + (x & 15), nf - 1), qi = fq / G, h = fq - qi * G;
+        const float* qp = a.Q + (int64_t)(r0 + qi) * a.ldq + (int64_t)(kvh * G + h) * HD + (x >> 4 & 3) * (HD / 4) + 8 * s;
+        const float4 u = *(const float4*)qp, v = *(const float4*)(qp + 4);
+        const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        Frag f[3];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t w[3];
+            parts_of(y[2 * i] * a.scale, y[2 * i + 1] * a.scale, w);
+#pragma unroll
+            for (int j = 0; j < 3; j++) f[j].w[i] = w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 3; j++) sq[n][s][j][x & 63] = f[j].v;
+    }
+    __syncthreads();
     for (int it = 0; it < n_it; it++) {
         if (it + 1 < n_it) {
             if (((it + 1) & 63) == 0) look(it + 1);
@@ -310,6 +352,7 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(
     }
 
     // the wavefronts' parts
+    __syncthreads();
 #pragma unroll
     for (int n = 0; n < CT; n++) {
         float s = l[n];  // of this group's positions
@@ -348,39 +391,50 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64)) void kv_chunk_kernel(
     }
 }
 
-// The parts of one row's head, in their order: a wavefront each, HD / 64 values a lane.
+// The parts of one row's head: their weights first, then a thread a value and group of parts, eight loads in
+// flight, in an order that does not depend on timing.
+constexpr int kMaxSplits = 256;
 template <int HD> __global__ __launch_bounds__(256) void kv_chunk_join_kernel(KvChunkArgs a, int splits, const float* part) {
-    constexpr int DPL = HD / 64;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = (int)(w / a.n_head), head = (int)(w % a.n_head), lane = threadIdx.x & 63;
-    if (row >= a.n_rows) return;
+    constexpr int NG = 256 / HD, B = 8;
+    __shared__ float w[kMaxSplits], red[8], go[NG][HD];
+    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, d = tid % HD, grp = tid / HD;
+    const float* po = part + ((int64_t)row * a.n_head + head) * splits * (HD + 2);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (tid < splits) ml = *(const float2*)(po + (int64_t)tid * (HD + 2) + HD);
     bool in = !a.row_off && row < a.q.n_seq;  // a row of some sequence
     if (a.row_off)
-        for (int i = 0; i < a.q.n_seq && !in; i += 64) {
-            const int j = i + lane;
-            in = __any(j < a.q.n_seq && a.row_off[j] <= row && row < a.row_off[j + 1]);
-        }
-    if (!in) return;
-    const float* q = part + w * splits * (HD + 2);
-    float mx = -INFINITY;
-    for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, q[(int64_t)i * (HD + 2) + HD]);
+        for (int j = tid; j < a.q.n_seq; j += 256) in |= a.row_off[j] <= row && row < a.row_off[j + 1];
+    if (!__syncthreads_or(in)) return;
+    float mx = ml.x;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    float ls = 0.0f, os[DPL] = {};
-#pragma unroll 4
-    for (int i = 0; i < splits; i++) {
-        const float* x = q + (int64_t)i * (HD + 2);
-        const float wt = x[HD] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[HD] - mx);
-        ls = fmaf(x[HD + 1], wt, ls);
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float wt = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+    if (tid < splits) w[tid] = wt;
+    float ls = wt * ml.y;
 #pragma unroll
-        for (int d = 0; d < DPL; d++) os[d] = fmaf(x[lane + 64 * d], wt, os[d]);
+    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o, 64);
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = ls;
+    __syncthreads();
+    float os = 0.0f;
+    for (int i = grp; i < splits; i += NG * B) {
+        float v[B];
+#pragma unroll
+        for (int b = 0; b < B; b++) v[b] = i + b * NG < splits ? po[(int64_t)(i + b * NG) * (HD + 2) + d] : 0.0f;
+#pragma unroll
+        for (int b = 0; b < B; b++)
+            if (i + b * NG < splits) os = fmaf(v[b], w[i + b * NG], os);
     }
-    float* out = a.out + (int64_t)row * a.ldo + (int64_t)head * HD + lane;
+    go[grp][d] = os;
+    __syncthreads();
+    if (grp) return;
+    ls = (red[4] + red[5]) + (red[6] + red[7]);
 #pragma unroll
-    for (int d = 0; d < DPL; d++) out[64 * d] = ls == 0.0f && mx == -INFINITY ? 0.0f : os[d] / ls;
+    for (int i = 1; i < NG; i++) os += go[i][d];
+    a.out[(int64_t)row * a.ldo + (int64_t)head * HD + d] = ls == 0.0f && mx == -INFINITY ? 0.0f : os / ls;
 }
-
-constexpr int kMaxSplits = 256;
 
 // Workgroups that the chip holds at once.
 template <int HD, int KB, int VB, int CT> int64_t resident() {
@@ -396,9 +450,11 @@ template <int HD, int KB, int VB, int CT> int64_t resident() {
 int64_t tiles_of(const KvChunkArgs& a, int nc) { return (int64_t)a.n_rows * (a.n_head / a.c.n_kv_head) / nc + a.q.n_seq; }
 
 // One round of workgroups at most, four records in a part at least, where that saves more than the join costs.
+// (Workgroups with work: those of sequences of the mean length.)
 template <int HD, int KB, int VB, int CT> int splits_of(const KvChunkArgs& a, int64_t records) {
     constexpr int NW = chunk_waves<HD, CT>();
-    const int64_t wgs = tiles_of(a, 16 * CT) * a.c.n_kv_head;
+    const int64_t pairs = ((int64_t)a.n_rows + a.q.n_seq - 1) / a.q.n_seq * (a.n_head / a.c.n_kv_head);
+    const int64_t wgs = std::max<int64_t>(1, (pairs + 16 * CT - 1) / (16 * CT)) * a.q.n_seq * a.c.n_kv_head;
     const int64_t n = std::min<int64_t>(resident<HD, KB, VB, CT>() / wgs, (records + 3) / 4);
     return n > 1 && records * (n - 1) > 3 * NW * n ? (int)std::min<int64_t>(n, kMaxSplits) : 1;
 }
@@ -418,7 +474,7 @@ template <int HD, int KB, int VB> hipError_t chunk_go(const KvChunkArgs& a, cons
             done = true;
         }
     if (!done) kv_chunk_kernel<HD, KB, VB, 1><<<grid, chunk_waves<HD, 1>() * 64, 0, s>>>(a, pl.splits, ws);
-    if (pl.splits > 1) kv_chunk_join_kernel<HD><<<dim3((unsigned)(((int64_t)a.n_rows * a.n_head + 3) / 4)), 256, 0, s>>>(a, pl.splits, ws);
+    if (pl.splits > 1) kv_chunk_join_kernel<HD><<<dim3((unsigned)a.n_rows, (unsigned)a.n_head), 256, 0, s>>>(a, pl.splits, ws);
     return hipGetLastError();
 }
 
@@ -435,16 +491,26 @@ KvChunkPlan kv_chunk_plan(const KvChunkArgs& a, bool workspace) {
     const int64_t pairs = (int64_t)a.n_rows * (a.n_head / c.n_kv_head);
     if (c.head_dim < 256 && pairs > 16 * (int64_t)a.q.n_seq) pl.tiles = 2;
     if (!workspace) return pl;
-    const char* env = getenv("GGQ_KV_PLANES");
-    if (a.row_off && (env && *env ? atoi(env) != 0 : pairs >= 256 * (int64_t)a.q.n_seq)) {
-        pl.tiles = 0;
-        pl.planes = attn_kv_planes_plan(a);
-        pl.ws_bytes = pl.planes.ws_bytes;
-        return pl;
-    }
     int64_t span = std::min<int64_t>(a.q.max_len, (int64_t)a.q.table_len * c.page_len);
     if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + a.n_rows / a.q.n_seq + kKvTile);
     const int64_t records = (span + kKvTile - 1) / kKvTile;
+    // Planes of operands (codes decoded once, two fp16 products where this kernel has three) from so many pairs a sequence
+    // on that they pay for the planes, in calls that are more than their launches (us, tiles -> planes; rows against positions):
+    //   32x8x128: 256 x 7000 122 -> 98, 64 58 -> 63; 512 x 700 42 -> 51, 1024 94 -> 79; 8 sequences 256 x 2000 149 -> 143
+    //   32x8x64: 512 x 4000 86 -> 78, 1024 130 -> 137, 1500 190 -> 245, 2048 281 -> 272
+    //   16x2x256: 256 x 4000 71 -> 77, 384 104 -> 91, 1024 230 -> 193
+    const int64_t mean = ((int64_t)a.n_rows + a.q.n_seq - 1) / a.q.n_seq * (a.n_head / c.n_kv_head);
+    const int64_t least = c.head_dim == 64 ? 8192 : c.head_dim == 128 ? 1024 : 3072;
+    const char* env = getenv("GGQ_KV_PLANES");
+    if (a.row_off && (env && *env ? atoi(env) != 0 : mean >= least && mean * a.q.n_seq * c.n_kv_head * records >= 1000000)) {
+        const AttnPromptPlan planes = attn_kv_planes_plan(a);
+        if (planes.ws_bytes <= (size_t(1) << 30)) {
+            pl.tiles = 0;
+            pl.planes = planes;
+            pl.ws_bytes = planes.ws_bytes;
+            return pl;
+        }
+    }
     if (const char* e = getenv("GGQ_KV_SPLITS"); e && atoi(e) > 0)
         pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(atoi(e), kMaxSplits), records));
     else if (c.head_dim == 64) pl.splits = GGQ_BY_CACHE(64, splits_go, a, pl.tiles, records);
