@@ -36,9 +36,10 @@ template <int TPB, typename T, typename F> __device__ __forceinline__ T wg_reduc
     return v;
 }
 
+// (a row's values may all be so small that the reciprocal of its step is infinite: zeros stay zeros there)
+__device__ __forceinline__ uint32_t code_of(float y, float inv) { return (uint32_t)(uint8_t)to_i8(y == 0.0f ? 0.0f : __fmul_rn(y, inv)); }
 __device__ __forceinline__ uint32_t codes_of(const float4& y, float inv) {
-    return (uint32_t)(uint8_t)to_i8(__fmul_rn(y.x, inv)) | (uint32_t)(uint8_t)to_i8(__fmul_rn(y.y, inv)) << 8 |
-           (uint32_t)(uint8_t)to_i8(__fmul_rn(y.z, inv)) << 16 | (uint32_t)(uint8_t)to_i8(__fmul_rn(y.w, inv)) << 24;
+    return code_of(y.x, inv) | code_of(y.y, inv) << 8 | code_of(y.z, inv) << 16 | code_of(y.w, inv) << 24;
 }
 __device__ __forceinline__ float step_of(float amax) { return amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f; }
 __device__ __forceinline__ double silu64(float z) { return (double)z / (1.0 + exp(-(double)z)); }

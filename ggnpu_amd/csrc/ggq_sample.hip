@@ -80,6 +80,11 @@ template <typename T> __device__ __forceinline__ T scan_add(T v) { return scan_b
 template <typename T> __device__ __forceinline__ T wave_sum(T v) { return lane_of(scan_add(v), 63); }
 template <typename T> __device__ __forceinline__ T wave_max(T v) { return lane_of(scan_by(v, [](T a, T b) { return max(a, b); }), 63); }
 
+// Whether a logit can have a weight: above -infinity.  (On its bits: this compiler's ballot of v > -INFINITY lets NaN through.)
+__device__ __forceinline__ bool there(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    return (u & 0x7FFFFFFFu) <= 0x7F800000u && u != 0xFF800000u;
+}
 // Keys in order of the values (no NaN).
 __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v == 0.0f ? 0.0f : v);
@@ -173,14 +178,14 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a) 
     uint32_t top = 0, at = 0xFFFFFFFFu, n = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const bool in = v[i] > -INFINITY;
+        const bool in = there(v[i]);
         n += (uint32_t)__popcll(__ballot(in));
         top = max(top, in ? key_of(v[i]) : 0u);
     }
     top = wave_max(top);
 #pragma unroll
     for (int i = V - 1; i >= 0; i--) {
-        const u64 is = __ballot(v[i] > -INFINITY && key_of(v[i]) == top);
+        const u64 is = __ballot(there(v[i]) && key_of(v[i]) == top);
         if (is) at = (uint32_t)(base + kBinThreads * i + (tid & ~63)) + (uint32_t)__ffsll(is) - 1;
     }
     if (lane == 0) { red[tid >> 6][0] = top; red[tid >> 6][1] = at; red[tid >> 6][2] = n; }
@@ -208,8 +213,8 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a) 
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const double z = (double)v[i] * c, fl = floor_of(v[i], c);
-            const double w = v[i] > -INFINITY ? __builtin_bit_cast(double, bins[below(first, fl)]) : 0.0;
-            m = fma(v[i] == INFINITY || !(v[i] > -INFINITY) ? 1.0 : factor_of(z - fl), w, m);
+            const double w = there(v[i]) ? __builtin_bit_cast(double, bins[below(first, fl)]) : 0.0;
+            m = fma(v[i] == INFINITY || !there(v[i]) ? 1.0 : factor_of(z - fl), w, m);
         }
         m = wave_sum(m);
         if (lane == 0) sums[tid >> 6] = m;
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a) 
 #pragma unroll
     for (int i = 0; i < V; i++) {
         spot[i] = 0xFFFFFFFFu;
-        if (!(v[i] > -INFINITY)) continue;
+        if (!there(v[i])) continue;
         const Bin b = bin_of(v[i], c);
         const int j = below(first, b.top);
         const u64 old = atomicAdd(&bins[j], (u64(1) << kCount) + (j == kRest ? 0 : b.factor));
@@ -764,7 +769,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
         w[i] = 0.0;
-        if (l[i] > -INFINITY) {
+        if (there(l[i])) {
             const Bin b = bin_of(l[i], c);
             const int j = below(first, b.top);
             if (j < kRest && (j < border.bin || (j == border.bin && place_of(key_of(l[i]), (uint32_t)(base + i)) >= border.place)))

@@ -513,7 +513,8 @@ int ggq_delta_rule_dev(ggq_ctx* ctx, const ggq_delta_rule_params* params, void* 
  * s is rounded to fp32 once, y is made from it in 64 bits and rounded once.
  * out receives y; codes and scales what ggq_quantize_act_dev makes of y in
  * act_mode GGQ_ACT_Q8_ROW or GGQ_ACT_Q8_BLOCK32 (GGQ_ACT_F32: none), for
- * ggq_mul_mat_q8_dev and ggq_mul_mat_q8_batch_dev.  sum may be x or add
+ * ggq_mul_mat_q8_dev and ggq_mul_mat_q8_batch_dev (zeros stay zeros also where all
+ * values are below 3.7e-37).  sum may be x or add
  * itself, and out may be x, with the same stride; other overlaps are not allowed.
  * n_cols a multiple of 4 (of 32 for Q8_BLOCK32), at most 32768; norm_len a
  * multiple of 4 that divides n_cols; pointers 16-byte aligned (scales 4), strides multiples of 4,
