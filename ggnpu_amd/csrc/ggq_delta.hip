@@ -26,6 +26,7 @@
 // state goes from product to product in its registers.
 #include <algorithm>
 #include <cstdlib>
+#include <type_traits>
 
 #include "ggq_device.h"
 #include "ggq_steps.h"
@@ -343,9 +344,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
     const Seq sq = seq_of(p, seq);
     const int hk = h / (p.n_v_head / p.n_k_head);
     const int parts = (sq.n + kRows - 1) / kRows, last_row = sq.n - 1;
-    auto after = [](int in) { return in + 1 == R::slots ? 0 : in + 1; };
-
     if (wave8 >= 4) {
+        auto after = [](int in) { return in + 1 == R::slots ? 0 : in + 1; };
         if (!parts) return;
         const float *kp = p.k + sq.row * p.ldk + (int64_t)hk * KD, *qp = p.q + sq.row * p.ldq + (int64_t)hk * KD;
         const float* vp = p.v + sq.row * p.ldv + (int64_t)h * p.v_dim + v0;
@@ -410,87 +410,96 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
     f32x4 s[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) s[t] = *(const f32x4*)(p.state + at + 16 * t);
-    struct In {
-        f32x4 k[NT], q[NT];
-    };
-    auto rows_in = [&](int in, In& x) {
-        const uint8_t* from = ring + in * R::bytes;
+    // Where this lane reads in a slot: a row's 16-byte runs, K's numbers transposed, the record, V
+    const uint8_t *row_at[NT], *col_at[NT][4], *rec_r = ring + R::rec + 64 * r + 16 * g, *rec_g = ring + R::rec + 16 * g;
+    const uint8_t *a_at = ring + R::rec + 4 * (kA + 16 * r + 4 * g + wave), *v_at = ring + R::v + 4 * (64 * g + r);
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int at_run = (r * RPR + ((4 * (tile0 + t) + g) ^ r)) * 16;
-            x.k[t] = *(const f32x4*)(from + at_run);
-            x.q[t] = *(const f32x4*)(from + R::kq + at_run);
-        }
-    };
-    // One part.  Issue is in order, so what waits stands in the shadow of products: this part's other operands beside
-    // K S, the sums' way through LDS beside Q S.
-    auto step = [&](int i, int in, const In& cur, In& nxt) {
-        const uint8_t* from = ring + in * R::bytes;
-        const float *rec = (const float*)(from + R::rec), *vin = (const float*)(from + R::v);
-        f32x4 ks[2] = {}, qs[2] = {};
+    for (int t = 0; t < NT; t++) {
+        row_at[t] = ring + (r * RPR + ((4 * (tile0 + t) + g) ^ r)) * 16;
+#pragma unroll
+        for (int e = 0; e < 4; e++) col_at[t][e] = ring + (((4 * g + e) * RPR + ((4 * (tile0 + t) + (r >> 2)) ^ (4 * g + e))) * 4 + (r & 3)) * 4;
+    }
+    f32x4 k[NT], q[NT];
+    // One part.  Issue is in order, and an fp32 product keeps its own wavefront's other arithmetic out (an instruction
+    // behind a product costs the product's end and 4 cycles each): so products stand in rows, arithmetic in a few groups, and
+    // what waits (this part's other operands, the sums' way through LDS) in the shadow of products.  The slots of the ring
+    // are unrolled: their addresses are constants.
+    auto step = [&](auto turn) {
+        constexpr int in = decltype(turn)::value % R::slots, odd = decltype(turn)::value & 1;
+        constexpr int here = in * R::bytes, next = (in + 1) % R::slots * R::bytes;
+        f32x4 ks[2] = {}, qs[2] = {}, v, kt[NT];
         auto q_s = [&](int first, int last) {
 #pragma unroll
             for (int x = first; x < last; x++)
-                qs[x & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.q[x % NT][x / NT], s[x % NT][x / NT], qs[x & 1], 0, 0, 0);
+                qs[x & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[x % NT][x / NT], s[x % NT][x / NT], qs[x & 1], 0, 0, 0);
         };
 #pragma unroll
         for (int x = 0; x < 4 * NT; x++)
-            ks[x & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.k[x % NT][x / NT], s[x % NT][x / NT], ks[x & 1], 0, 0, 0);
-        f32x4 v, kt[NT];
+            ks[x & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[x % NT][x / NT], s[x % NT][x / NT], ks[x & 1], 0, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[e] = vin[(4 * g + e) * 16 + r];
+        for (int e = 0; e < 4; e++) v[e] = *(const float*)(v_at + here + 64 * e);
+        const f32x4 kc = *(const f32x4*)(rec_g + here + 4 * kKc), tr = *(const f32x4*)(rec_r + here + 4 * kT);
+        const f32x4 kf = *(const f32x4*)(rec_g + here + 4 * kKs), qc = *(const f32x4*)(rec_g + here + 4 * kQc);
+        const float dec = *(const float*)(ring + R::rec + here + 4 * kDec), ar = *(const float*)(a_at + here);
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                kt[t][e] = ((const float*)from)[((4 * g + e) * RPR + ((4 * (tile0 + t) + (r >> 2)) ^ (4 * g + e))) * 4 + (r & 3)];
-        }
-        const f32x4 tr = *(const f32x4*)(rec + kT + 16 * r + 4 * g), kc = *(const f32x4*)(rec + kKc + 4 * g);
-        const f32x4 qc = *(const f32x4*)(rec + kQc + 4 * g), kf = *(const f32x4*)(rec + kKs + 4 * g);
-        const float ar = rec[kA + 16 * r + 4 * g + wave], dec = rec[kDec];
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) kt[t][e] = *(const float*)(col_at[t][e] + here);
         __builtin_amdgcn_sched_barrier(0);
         q_s(0, NT);
         __builtin_amdgcn_sched_barrier(0);
-        s_ks[i & 1][wave][lane] = ks[0] + ks[1];
+        const f32x4 x0 = ks[0] + ks[1];
+        s_ks[odd][wave][lane] = x0;
         __builtin_amdgcn_sched_barrier(0);
         q_s(NT, 2 * NT);
         __builtin_amdgcn_sched_barrier(0);
         // the next part's loads have come and the sums are in LDS
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const f32x4* x = &s_ks[i & 1][0][lane];
-        const f32x4 x0 = x[0], x1 = x[64], x2 = x[128], x3 = x[192];
-        rows_in(after(in), nxt);  // (behind the last part: that one again)
+        // (pairs, so that all wavefronts have the same sums)
+        const f32x4 x1 = s_ks[odd][wave ^ 1][lane], x2 = s_ks[odd][wave ^ 2][lane], x3 = s_ks[odd][wave ^ 3][lane];
         __builtin_amdgcn_sched_barrier(0);
         q_s(2 * NT, 4 * NT);
         __builtin_amdgcn_sched_barrier(0);
-        const f32x4 rest = v - kc * ((x0 + x1) + (x2 + x3));
-        f32x4 u{0, 0, 0, 0};
+        f32x4 rest, of = (qs[0] + qs[1]) * qc, u{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; e++) rest[e] = fmaf(-kc[e], (x0[e] + x1[e]) + (x2[e] + x3[e]), v[e]);
+#pragma unroll
+        for (int t = 0; t < NT; t++) s[t] *= dec;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < 4; e++) u = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[e], rest[e], u, 0, 0, 0);
 #pragma unroll
-        for (int t = 0; t < NT; t++) s[t] *= dec;
-        const f32x4 of = (qs[0] + qs[1]) * qc;
-        __builtin_amdgcn_sched_barrier(0);
+        for (int t = 0; t < NT; t++) {  // (behind the last part: that one again)
+            k[t] = *(const f32x4*)(row_at[t] + next);
+            q[t] = *(const f32x4*)(row_at[t] + next + R::kq);
+        }
         const f32x4 w = u * kf;
+        const float ue = wave & 2 ? (wave & 1 ? u[3] : u[2]) : wave & 1 ? u[1] : u[0];
+        __builtin_amdgcn_sched_barrier(0);
+        of = __builtin_amdgcn_mfma_f32_16x16x4f32(ar, ue, of, 0, 0, 0);
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
             for (int t = 0; t < NT; t++) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kt[t][e], w[e], s[t], 0, 0, 0);
-        const int wv = tid >> 6;
-        const float ue = wv == 0 ? u[0] : wv == 1 ? u[1] : wv == 2 ? u[2] : u[3];
-        s_o[i & 1][wave][lane] = __builtin_amdgcn_mfma_f32_16x16x4f32(ar, ue, of, 0, 0, 0);
+        s_o[odd][wave][lane] = of;
+        __builtin_amdgcn_sched_barrier(0);
     };
     if (parts) {
         __syncthreads();
-        In x, y;
-        rows_in(0, x);
-        int in = 0;
-        for (int i = 0; i < parts; i += 2) {
-            step(i, in, x, y);
-            in = after(in);
-            if (i + 1 == parts) break;
-            step(i + 1, in, y, x);
-            in = after(in);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            k[t] = *(const f32x4*)row_at[t];
+            q[t] = *(const f32x4*)(row_at[t] + R::kq);
         }
+        int left = parts;
+        // (as many steps as bring the slots and the two of s_ks back to the first)
+        auto steps = [&](auto self, auto turn) -> void {
+            step(turn);
+            left--;
+            if constexpr (decltype(turn)::value + 1 < R::slots * (1 + R::slots % 2))
+                if (left) self(self, std::integral_constant<int, decltype(turn)::value + 1>());
+        };
+        while (left) steps(steps, std::integral_constant<int, 0>());
         __syncthreads();
     }
 #pragma unroll
