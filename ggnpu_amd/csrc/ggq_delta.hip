@@ -25,6 +25,7 @@
 // wants of that lane (step e of a product takes k = 4 g + e from lane group g), so the
 // state goes from product to product in its registers.
 #include <algorithm>
+#include <climits>
 #include <cstdlib>
 #include <type_traits>
 
@@ -35,11 +36,14 @@ namespace ggq {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64;
 
 struct DeltaArgs {
     ggq_delta_rule_params p;
     float scale;
     float* parts;  // records of the parts
+    // Sequences of up to `few` rows go row by row, the others in parts (-1: all in parts; INT_MAX: none).
+    int few;
 };
 
 constexpr int kRows = 16;  // rows of a part
@@ -96,6 +100,7 @@ __global__ __launch_bounds__(256) void delta_rows_kernel(DeltaArgs a) {
     const int slot = slot_of(p, seq);
     if (slot < 0) return;
     const Seq sq = seq_of(p, seq);
+    if (sq.n > a.few) return;
     const int hk = h / (p.n_v_head / p.n_k_head), d0 = blockIdx.y * 16 * C + grp;
     const int64_t at = ((int64_t)slot * p.n_v_head + h) * p.v_dim;
     float4 s[C][N];
@@ -201,7 +206,7 @@ __global__ __launch_bounds__(256) void delta_parts_kernel(DeltaArgs a) {
     const Seq sq = seq_of(p, seq);
     const int64_t first = (id - sq.part) * kRows;
     const int hk = blockIdx.y * 4 + wave;
-    if (first < 0 || first >= sq.n || hk >= p.n_k_head || slot_of(p, seq) < 0) return;  // (no barrier from here on)
+    if (first < 0 || first >= sq.n || sq.n <= a.few || hk >= p.n_k_head || slot_of(p, seq) < 0) return;  // (no barrier from here on)
     const int n = (int)min((int64_t)kRows, sq.n - first);
     const int64_t row0 = sq.row + first, row = row0 + min(r, n - 1);
     const float *kp = p.k + row * p.ldk + (int64_t)hk * KD + 4 * g, *qp = p.q + row * p.ldq + (int64_t)hk * KD + 4 * g;
@@ -335,18 +340,15 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
     static_assert(R::slots * R::bytes < 128 * 1024, "LDS that global_load_lds addresses");
     __shared__ __attribute__((aligned(1024))) uint8_t ring[R::slots * R::bytes];
     __shared__ __attribute__((aligned(16))) f32x4 s_ks[2][4][64], s_o[2][4][64];
+    __shared__ int s_list[512], s_many[8];
     const ggq_delta_rule_params& p = a.p;
-    const int h = blockIdx.x, seq = blockIdx.z, v0 = blockIdx.y * 16;
+    const int h = blockIdx.x, v0 = blockIdx.y * 16;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
     const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave8 & 3;
-    const int slot = slot_of(p, seq);
-    if (slot < 0) return;
-    const Seq sq = seq_of(p, seq);
     const int hk = h / (p.n_v_head / p.n_k_head);
-    const int parts = (sq.n + kRows - 1) / kRows, last_row = sq.n - 1;
-    if (wave8 >= 4) {
+    auto load_and_write = [&](const Seq& sq, int parts) {
         auto after = [](int in) { return in + 1 == R::slots ? 0 : in + 1; };
-        if (!parts) return;
+        const int last_row = sq.n - 1;
         const float *kp = p.k + sq.row * p.ldk + (int64_t)hk * KD, *qp = p.q + sq.row * p.ldq + (int64_t)hk * KD;
         const float* vp = p.v + sq.row * p.ldv + (int64_t)h * p.v_dim + v0;
         float* op = p.out + sq.row * p.ldo + (int64_t)h * p.v_dim + v0;
@@ -402,14 +404,10 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (parts > 1) put(parts - 2);
         put(parts - 1);
-        return;
-    }
+    };
 
     const int tile0 = wave * NT;
-    const int64_t at = (((int64_t)slot * p.n_v_head + h) * p.v_dim + v0 + r) * KD + 16 * tile0 + 4 * g;
     f32x4 s[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) s[t] = *(const f32x4*)(p.state + at + 16 * t);
     // Where this lane reads in a slot: a row's 16-byte runs, K's numbers transposed, the record, V
     const uint8_t *row_at[NT], *col_at[NT][4], *rec_r = ring + R::rec + 64 * r + 16 * g, *rec_g = ring + R::rec + 16 * g;
     const uint8_t *a_at = ring + R::rec + 4 * (kA + 16 * r + 4 * g + wave), *v_at = ring + R::v + 4 * (64 * g + r);
@@ -484,61 +482,116 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
         s_o[odd][wave][lane] = of;
         __builtin_amdgcn_sched_barrier(0);
     };
-    if (parts) {
-        __syncthreads();
+    auto compute = [&](int slot, int parts) {
+        const int64_t at = (((int64_t)slot * p.n_v_head + h) * p.v_dim + v0 + r) * KD + 16 * tile0 + 4 * g;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            k[t] = *(const f32x4*)row_at[t];
-            q[t] = *(const f32x4*)(row_at[t] + R::kq);
+        for (int t = 0; t < NT; t++) s[t] = *(const f32x4*)(p.state + at + 16 * t);
+        if (parts) {
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                k[t] = *(const f32x4*)row_at[t];
+                q[t] = *(const f32x4*)(row_at[t] + R::kq);
+            }
+            int left = parts;
+            // (as many steps as bring the slots and the two of s_ks back to the first)
+            auto steps = [&](auto self, auto turn) -> void {
+                step(turn);
+                left--;
+                if constexpr (decltype(turn)::value + 1 < R::slots * (1 + R::slots % 2))
+                    if (left) self(self, std::integral_constant<int, decltype(turn)::value + 1>());
+            };
+            while (left) steps(steps, std::integral_constant<int, 0>());
+            __syncthreads();
         }
-        int left = parts;
-        // (as many steps as bring the slots and the two of s_ks back to the first)
-        auto steps = [&](auto self, auto turn) -> void {
-            step(turn);
-            left--;
-            if constexpr (decltype(turn)::value + 1 < R::slots * (1 + R::slots % 2))
-                if (left) self(self, std::integral_constant<int, decltype(turn)::value + 1>());
-        };
-        while (left) steps(steps, std::integral_constant<int, 0>());
+#pragma unroll
+        for (int t = 0; t < NT; t++) *(f32x4*)(p.state_out + at + 16 * t) = s[t];
+    };
+    auto sequence = [&](int seq) {  // (of all threads)
+        const int slot = slot_of(p, seq);
+        const Seq sq = seq_of(p, seq);
+        const int parts = (sq.n + kRows - 1) / kRows;
+        if (slot < 0) return;
+        if (wave8 < 4) compute(slot, parts);
+        else if (parts) load_and_write(sq, parts);
+    };
+    if (a.few < 0) return sequence(blockIdx.z);
+    // Each gridDim.z-th one of the longer sequences.
+    int before = 0;
+    for (int from = 0; from < p.n_seq; from += 512) {
+        const int j = from + tid;
+        const bool is = j < p.n_seq && seq_of(p, j).n > a.few;
+        const u64 b = __ballot(is);
+        if (lane == 0) s_many[wave8] = __popcll(b);
+        __syncthreads();
+        int at = 0, many = 0;
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            at += w < wave8 ? s_many[w] : 0;
+            many += s_many[w];
+        }
+        if (is) s_list[at + __popcll(b & ((1ull << lane) - 1))] = j;
+        __syncthreads();
+        for (int i = 0; i < many; i++)
+            if ((before + i) % (int)gridDim.z == (int)blockIdx.z) sequence(__builtin_amdgcn_readfirstlane(s_list[i]));
+        before += many;
         __syncthreads();
     }
-#pragma unroll
-    for (int t = 0; t < NT; t++) *(f32x4*)(p.state_out + at + 16 * t) = s[t];
 }
 
 int64_t parts_of(const ggq_delta_rule_params& p) { return (int64_t)p.n_rows / kRows + p.n_seq; }
 
-template <int KD> hipError_t delta_launch(const DeltaArgs& a, bool parts, hipStream_t s) {
+// How many rows a sequence that goes row by row has at most (DeltaArgs::few).  A row's step takes 0.9 us where the chip
+// is not full, and 10 us are gone before the first part is through: one sequence of 32 heads of 128 x 128 with 8 rows takes 11.1 us
+// row by row and 11.4 in parts, with 16 rows 18.8 and 12.0.  Many sequences fill the chip better row by row (16 of 16 rows 50 and
+// 61 us, of 24 rows 68 and 70; 64 of 16 rows 176 and 225, of 32 rows 342 and 287).  The lengths are on the device: unless all are
+// bound to be short or are long in the mean, both forms are launched and each takes its own sequences.  That costs 5 to 8 us
+// where all are short (64 of 4 rows 73 us, row by row 65) and bounds what one long one costs (64 single tokens and 1024
+// rows: 114 us, row by row 1835, in parts 308).
+int few_rows(const ggq_delta_rule_params& p) {
+    if (!p.row_off) return INT_MAX;
+    const char* env = getenv("GGQ_DELTA_PARTS");
+    const bool many = (int64_t)p.n_seq * p.n_v_head * (p.v_dim / 16) > 1024;
+    const int few = many ? kRows : kRows / 2;
+    if (env && *env) return atoi(env) == 0 ? INT_MAX : atoi(env) == 1 ? -1 : few;
+    if (p.n_rows - p.n_seq < (p.n_seq == 1 ? few : kRows)) return INT_MAX;  // (sequences without rows aside, none is longer)
+    return p.n_rows > (many ? 64 : few) * (int64_t)p.n_seq ? -1 : few;
+}
+
+template <int KD> hipError_t delta_launch(const DeltaArgs& a, hipStream_t s) {
     const ggq_delta_rule_params& p = a.p;
-    if (parts) {
-        delta_parts_kernel<KD><<<dim3((unsigned)parts_of(p), (unsigned)((p.n_k_head + 3) / 4)), 256, 0, s>>>(a);
-        // (heads first: the slices of one head share its rows in one XCD's L2 where there is a multiple of 8 heads)
-        delta_scan_kernel<KD><<<dim3((unsigned)p.n_v_head, (unsigned)(p.v_dim / 16), (unsigned)p.n_seq), 512, 0, s>>>(a);
-        return hipGetLastError();
+    if (a.few >= 0) {
+        constexpr int C = KD == 256 ? 2 : 4;
+        const int64_t wide = (int64_t)p.n_seq * p.n_v_head * ((p.v_dim + 16 * C - 1) / (16 * C));
+        if (wide >= 2 * cu_count())
+            delta_rows_kernel<KD, C><<<dim3((unsigned)p.n_v_head, (unsigned)((p.v_dim + 16 * C - 1) / (16 * C)), (unsigned)p.n_seq), 256, 0, s>>>(a);
+        else
+            delta_rows_kernel<KD, 1><<<dim3((unsigned)p.n_v_head, (unsigned)(p.v_dim / 16), (unsigned)p.n_seq), 256, 0, s>>>(a);
     }
-    constexpr int C = KD == 256 ? 2 : 4;
-    const int64_t wide = (int64_t)p.n_seq * p.n_v_head * ((p.v_dim + 16 * C - 1) / (16 * C));
-    if (wide >= 2 * cu_count())
-        delta_rows_kernel<KD, C><<<dim3((unsigned)p.n_v_head, (unsigned)((p.v_dim + 16 * C - 1) / (16 * C)), (unsigned)p.n_seq), 256, 0, s>>>(a);
-    else
-        delta_rows_kernel<KD, 1><<<dim3((unsigned)p.n_v_head, (unsigned)(p.v_dim / 16), (unsigned)p.n_seq), 256, 0, s>>>(a);
+    if (a.few < INT_MAX) {
+        delta_parts_kernel<KD><<<dim3((unsigned)parts_of(p), (unsigned)((p.n_k_head + 3) / 4)), 256, 0, s>>>(a);
+        // (no more workgroups than sequences can be long, nor than two a CU: one that finds nothing to do takes its LDS first)
+        int64_t z = p.n_seq;
+        if (a.few >= 0)
+            z = std::max<int64_t>(1, std::min({z, (int64_t)p.n_rows / (a.few + 1), 2 * (int64_t)cu_count() / (p.n_v_head * (p.v_dim / 16))}));
+        // (heads first: the slices of one head share its rows in one XCD's L2 where there is a multiple of 8 heads)
+        delta_scan_kernel<KD><<<dim3((unsigned)p.n_v_head, (unsigned)(p.v_dim / 16), (unsigned)z), 512, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t delta_ws_bytes(const ggq_delta_rule_params& p) {
-    if (!p.row_off) return 0;
-    const char* env = getenv("GGQ_DELTA_PARTS");
-    if (env && *env ? atoi(env) == 0 : p.n_rows <= 24 * (int64_t)p.n_seq) return 0;
+    if (few_rows(p) == INT_MAX) return 0;
     return sizeof(float) * (kRecord * (size_t)parts_of(p) * p.n_v_head + 256);  // (the last record's loads go 192 floats further)
 }
 
 hipError_t launch_delta(const ggq_delta_rule_params& p, void* ws, hipStream_t s) {
-    DeltaArgs a{p, p.scale == 0.0f ? (float)(1.0 / sqrt((double)p.k_dim)) : p.scale, (float*)ws};
-    if (p.k_dim == 64) return delta_launch<64>(a, ws != nullptr, s);
-    if (p.k_dim == 128) return delta_launch<128>(a, ws != nullptr, s);
-    return delta_launch<256>(a, ws != nullptr, s);
+    DeltaArgs a{p, p.scale == 0.0f ? (float)(1.0 / sqrt((double)p.k_dim)) : p.scale, (float*)ws, ws ? few_rows(p) : INT_MAX};
+    if (p.k_dim == 64) return delta_launch<64>(a, s);
+    if (p.k_dim == 128) return delta_launch<128>(a, s);
+    return delta_launch<256>(a, s);
 }
 
 }  // namespace ggq

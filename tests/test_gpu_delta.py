@@ -180,6 +180,32 @@ def test_forms_agree(ctx, monkeypatch):
     assert np.array_equal(r[1][0], r[2][0]) and not np.array_equal(r[0][0], r[1][0])
 
 
+@pytest.mark.parametrize("env", ["", "2"])
+@pytest.mark.parametrize("lens,vh", [([1] * 9 + [90] + [3, 16, 17, 0, 33, 8, 9], 2), ([1] * 40 + [200], 2), ([4] * 30, 4), ([1, 30, 1], 32), ([0] * 5, 2),
+                                     ([70] + [1] * 70, 32), ([17] * 12 + [1] * 30, 32)])
+def test_short_and_long_sequences_in_one_call(ctx, monkeypatch, env, lens, vh):
+    """Short ones go row by row and long ones in parts, each once; forced and by the rule."""
+    monkeypatch.setenv("GGQ_DELTA_PARTS", env)
+    c = Case(len(lens) + vh, lens, 2, vh, 64, 32, raw=True, before=2, behind=3)
+    a = c.call(ctx)
+    c.check(*a)
+    b = c.call(ctx, in_place=True)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1][c.slot], b[1][c.slot])
+
+
+def test_long_sequences_among_many(ctx, monkeypatch):
+    """More sequences than are looked through in one turn, the long ones in several turns, one with a slot that does not exist."""
+    monkeypatch.setenv("GGQ_DELTA_PARTS", "2")
+    lens = [1] * 1300
+    for i in (0, 5, 511, 512, 700, 1024, 1299):
+        lens[i] = 20 + i % 7
+    c = Case(21, lens, 1, 1, 64, 16)
+    c.slot[700] = -1
+    o, so = c.call(ctx)
+    c.check(o, so, seqs=[0, 1, 5, 510, 511, 512, 513, 1023, 1024, 1025, 1298, 1299])
+    assert (o[c.off[700]:c.off[701]] == 7).all()
+
+
 def test_decays_of_all_sizes(ctx, form):
     """Nothing forgotten, everything forgotten (also by -infinity), and long runs after large decays: differences of sums keep their bits."""
     c = Case(8, [60], 1, 4, 64, 32)
