@@ -1321,8 +1321,9 @@ int ggq_attention_kv_rows_dev(ggq_ctx* c, const ggq_kv_cache* cache, const ggq_k
     const int64_t row = (int64_t)n_head * cache->head_dim;
     if (n_rows < 0 || ldq < row || ldo < row || window < 0 || !std::isfinite(scale))
         return set_status(c, GGQ_INVALID_PARAM, "need n_rows >= 0, ldq, ldo of a row or more, window >= 0 and a finite scale");
-    if ((int64_t)n_rows * n_head / 4 + seqs->n_seq > INT32_MAX)
-        return set_status(c, GGQ_INVALID_PARAM, "n_rows * n_head is too large");
+    // (a grid has fewer than 2^32 threads a dimension)
+    if ((int64_t)n_rows * (n_head / cache->n_kv_head) / 16 + seqs->n_seq >= 1 << 24)
+        return set_status(c, GGQ_INVALID_PARAM, "n_rows * n_head / n_kv_head is too large");
     if (n_rows == 0 || seqs->n_seq == 0) return set_status(c, GGQ_OK);
     if (!q || !out) return set_status(c, GGQ_INVALID_PARAM, "null q/out");
     if (!aligned16(q) || !aligned16(out) || ldq % 4 || ldo % 4)
@@ -1355,8 +1356,8 @@ int ggq_delta_rule_dev(ggq_ctx* c, const ggq_delta_rule_params* p, void* stream)
         return set_status(c, GGQ_INVALID_PARAM, "row strides must hold a row's heads");
     if (std::max({p->ldq, p->ldk, p->ldv, p->ldo}) > 1 << 24) return set_status(c, GGQ_INVALID_PARAM, "row strides above 2^24 values");
     if (p->flags & ~(GGQ_DELTA_BETA_SIGMOID | GGQ_DELTA_QK_NORM)) return set_status(c, GGQ_INVALID_PARAM, "unknown flags %d", p->flags);
-    if (p->n_seq < 0 || p->n_seq > 65535 || p->n_rows < 0 || p->n_slots < 0 || !std::isfinite(p->scale) || !(p->eps >= 0.0f))
-        return set_status(c, GGQ_INVALID_PARAM, "need n_seq in 0..65535, n_rows and n_slots >= 0, a finite scale and eps >= 0");
+    if (p->n_seq < 0 || p->n_seq > 65535 || p->n_rows < 0 || p->n_rows > 1 << 27 || p->n_slots < 0 || !std::isfinite(p->scale) || !(p->eps >= 0.0f))
+        return set_status(c, GGQ_INVALID_PARAM, "need n_seq in 0..65535, n_rows in 0..2^27, n_slots >= 0, a finite scale and eps >= 0");
     if (p->n_seq == 0 || p->n_slots == 0) return set_status(c, GGQ_OK);
     if (!p->state || !p->state_out || (p->n_rows && (!p->q || !p->k || !p->v || !p->gate || !p->beta || !p->out)))
         return set_status(c, GGQ_INVALID_PARAM, "null q/k/v/gate/beta/state/out");

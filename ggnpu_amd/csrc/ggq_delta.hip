@@ -325,7 +325,7 @@ __device__ __forceinline__ void dma16(const void* src, uint32_t offset, uint32_t
 // other's banks), V's 16 columns, the record (and what lies behind it, so that all loads are alike).  `slots` parts are
 // under way.
 template <int KD> struct Ring {
-    static constexpr int kq = kRows * KD * 4, v = 2 * kq, rec = v + 1024, bytes = rec + 3072;
+    static constexpr int kq = kRows * KD * 4, v = 2 * kq, rec = v + 1024, bytes = rec + 3 * 1024;
     static constexpr int slots = KD == 64 ? 8 : KD == 128 ? 6 : 3;
     static constexpr int loads = KD / 32 + 1;  // of a wavefront, a part
 };

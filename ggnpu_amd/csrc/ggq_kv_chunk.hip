@@ -500,7 +500,7 @@ KvChunkPlan kv_chunk_plan(const KvChunkArgs& a, bool workspace) {
     //   32x8x64: 512 x 4000 86 -> 78, 1024 130 -> 137, 1500 190 -> 245, 2048 281 -> 272
     //   16x2x256: 256 x 4000 71 -> 77, 384 104 -> 91, 1024 230 -> 193
     const int64_t mean = ((int64_t)a.n_rows + a.q.n_seq - 1) / a.q.n_seq * (a.n_head / c.n_kv_head);
-    const int64_t least = c.head_dim == 64 ? 8192 : c.head_dim == 128 ? 1024 : 3072;
+    const int64_t least = c.head_dim == 64 ? 8192 : c.head_dim == 128 ? 1024 : 2560;
     const char* env = getenv("GGQ_KV_PLANES");
     if (a.row_off && (env && *env ? atoi(env) != 0 : mean >= least && mean * a.q.n_seq * c.n_kv_head * records >= 1000000)) {
         const AttnPromptPlan planes = attn_kv_planes_plan(a);

@@ -50,7 +50,8 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
     __shared__ float redf[TPB / 64];
     extern __shared__ double parts[];  // a square sum a run, where groups are neither the row nor a power of two of lanes
     const ggq_norm_params& p = a.p;
-    const int64_t m = blockIdx.x;
+    const int64_t m = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (m >= a.p.n_rows) return;
     const int tid = threadIdx.x, K = p.n_cols;
     const float* xr = p.x + m * p.ldx;
     float4 v[R], g[R];
@@ -183,7 +184,9 @@ hipError_t launch_norm(const ggq_norm_params& p, hipStream_t s) {
     const int lanes = a.len / 4;
     if (lanes <= 64 && !(lanes & (lanes - 1))) a.lanes = lanes;
     const size_t lds = a.len == p.n_cols || a.lanes ? 0 : sizeof(double) * (size_t)(p.n_cols / 4);
-#define L(TPB_, R_) norm_kernel<TPB_, R_><<<dim3((unsigned)p.n_rows), TPB_, lds, s>>>(a)
+    // (a grid has fewer than 2^32 threads a dimension)
+    const unsigned x = (unsigned)std::min(p.n_rows, 1 << 20), y = ((unsigned)p.n_rows + x - 1) / x;
+#define L(TPB_, R_) norm_kernel<TPB_, R_><<<dim3(x, y), TPB_, lds, s>>>(a)
     if (p.n_cols <= 256) L(64, 1);
     else if (p.n_cols <= 512) L(64, 2);
     else if (p.n_cols <= 1024) L(64, 4);

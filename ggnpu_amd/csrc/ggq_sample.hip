@@ -627,8 +627,12 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
                 if (sub == 15) {
                     const Bin b = bin_of(of_key((uint32_t)(mine >> 32)), c);
                     few_rank[i] = r;
-                    few_w[i] = phase == ALL ? (flt.by_k && r >= (uint32_t)flt.k ? 0.0 : (double)b.factor * tab[below(first, b.top)])
-                                            : __builtin_bit_cast(double, b.factor);
+                    if (phase == ALL) {  // (in their order: sums in 64 bits depend on it)
+                        place[r] = mine;
+                        few_w[r] = flt.by_k && r >= (uint32_t)flt.k ? 0.0 : (double)b.factor * tab[below(first, b.top)];
+                    } else {
+                        few_w[i] = __builtin_bit_cast(double, b.factor);
+                    }
                 }
             }
             __syncthreads();
@@ -651,6 +655,11 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
                 __syncthreads();
                 continue;
             }
+            if (tid < nf) {
+                few[tid] = place[tid];
+                few_rank[tid] = (uint32_t)tid;
+            }
+            __syncthreads();
             double whole = 0.0;
             if (flt.by_p && !flt.by_k) {  // top_p's share is of the whole row
 #pragma unroll

@@ -91,7 +91,9 @@ int ggq_sync(ggq_ctx* ctx);
  * ninth on share eight, and their calls wait for one another where they meet
  * on one), and other kernels where it cannot be had: the same products, rounded
  * in another order, in several times the time (attention: up to 26 times, a
- * prompt of 8191 rows 18 ms for 1.4, one sequence of 131001 positions 580 us for 22).  A stream's work is complete
+ * prompt of 8191 rows 18 ms for 1.4, one sequence of 131001 positions 580 us for 22).
+ * The delta rule without it goes row by row (a prompt of 8191 rows 8 ms for 0.4); sampling
+ * has no other form and fails as above (GGQ_OUT_OF_MEMORY outside a capture).  A stream's work is complete
  * before the stream is destroyed.  Each capture gets a buffer of its
  * own that stays with its graph: a call outside a capture, on any stream, sets
  * aside what eight captures of the largest such call so far need (two where
@@ -392,7 +394,8 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * defined result (the others keep theirs).  Products are exact in fp32
  * terms, as above; where long prompts go through planes of fp16 operands, a
  * weight is besides off by up to 2^-28 of the row's largest product of weight
- * and value.  q and out 16-byte aligned, ldq and ldo multiples of 4. */
+ * and value.  q and out 16-byte aligned, ldq and ldo multiples of 4;
+ * n_rows * n_head / n_kv_head below 2^28. */
 int ggq_attention_kv_rows_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off,
                               int n_rows, const float* q, int64_t ldq, int n_head, float scale, int window, float* out,
                               int64_t ldo, void* stream);
@@ -464,15 +467,15 @@ int ggq_attention_prompt_dev(ggq_ctx* ctx, const ggq_attention_prompt_params* pa
  * outside [0, n_slots) is passed over: its rows of out stay as they were.  One
  * without rows has its state copied.  Slots of no sequence and rows of no
  * sequence stay as they were.
- * All sums and states are fp32.  Sequences of up to about 24 rows in the mean
- * go row by row, longer ones in parts of 16 rows, for which the rows' values are
- * solved together (the same result, rounded in another order); without workspace
- * for that (a buffer per stream, as for the matmuls) they go row by row.
+ * All sums and states are fp32.  Short sequences (up to 8 or 16 rows, by what is
+ * in the call) go row by row, longer ones in parts of 16 rows, for which the rows'
+ * values are solved together (the same result, rounded in another order); without workspace
+ * for that (a buffer per stream, as for the matmuls) all go row by row.
  * Rows are dense heads: q and k [n_k_head][k_dim], v and out
  * [n_v_head][v_dim], gate and beta [n_v_head], with row strides ld*.  k_dim
  * 64, 128 or 256, v_dim a multiple of 16 up to 512; all pointers but gate,
  * beta, gate_rate, gate_bias, slot and row_off 16-byte aligned, ldq, ldk, ldv and ldo
- * multiples of 4, at most 2^24. */
+ * multiples of 4, at most 2^24; n_rows at most 2^27, n_seq 65535. */
 #define GGQ_DELTA_BETA_SIGMOID 1
 #define GGQ_DELTA_QK_NORM 2
 typedef struct {

@@ -324,7 +324,7 @@ def test_refusals(ctx):
                dict(v_dim=528, ldv=2000, ldo=2000), dict(ldq=60), dict(ldk=60), dict(ldv=28), dict(ldo=28), dict(ld_gate=1), dict(ld_beta=1),
                dict(ldq=66), dict(ldq=1 << 25), dict(ldo=34), dict(q=None), dict(k=None), dict(v=None), dict(gate=None), dict(beta=None),
                dict(out=None), dict(state=None), dict(state_out=None), dict(q=P + 4), dict(state=P + 8), dict(out=P + 12), dict(flags=4),
-               dict(flags=-1), dict(n_seq=-1), dict(n_seq=65536), dict(n_rows=-1), dict(n_slots=-1), dict(eps=-1.0), dict(eps=float("nan")),
+               dict(flags=-1), dict(n_seq=-1), dict(n_seq=65536), dict(n_rows=-1), dict(n_rows=(1 << 27) + 1), dict(n_slots=-1), dict(eps=-1.0), dict(eps=float("nan")),
                dict(scale=float("inf")), dict(gate_bias=P), dict(n_v_head=65536)):
         assert st(**kw) == gl.Status.INVALID_PARAM, kw
         assert ctx.lib.ggq_last_error_message(ctx.h)

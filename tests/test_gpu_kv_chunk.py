@@ -309,6 +309,6 @@ def test_refusals(ctx):
                dict(c=cache(pages=mem.data_ptr() + 8)), dict(s=seqs(n_seq=-1)), dict(s=seqs(n_seq=65536)), dict(s=seqs(table_len=0)),
                dict(s=seqs(max_len=-1)), dict(s=seqs(pages=None)), dict(s=seqs(len=None)), dict(n_rows=-1), dict(q=None), dict(out=None),
                dict(q=P + 4), dict(out=P + 4), dict(ldq=127), dict(ldq=126), dict(ldq=130), dict(ldo=124), dict(ldo=130), dict(n_head=0),
-               dict(c=cache(n_kv_head=2), n_head=3), dict(n_head=65536), dict(scale=float("nan")), dict(window=-1), dict(n_rows=2147483647, n_head=64)):
+               dict(c=cache(n_kv_head=2), n_head=3), dict(n_head=65536), dict(scale=float("nan")), dict(window=-1), dict(n_rows=2147483647, n_head=64), dict(n_rows=1 << 28)):
         assert st(**kw) == gl.Status.INVALID_PARAM, kw
     torch.cuda.synchronize()

@@ -180,3 +180,22 @@ def test_refusals(ctx):
         assert st(**kw) == bad, kw
         assert ctx.lib.ggq_last_error_message(ctx.h)
     torch.cuda.synchronize()
+
+
+def test_more_rows_than_a_grid_dimension_holds(ctx):
+    """2^26 + 3 rows of 4 values: 64 threads each are more than 2^32."""
+    import torch
+    n = (1 << 26) + 3
+    x, out = torch.full((n, 4), 2.0, device="cuda"), torch.zeros((n, 4), device="cuda")
+    at = [0, 1, (1 << 20) - 1, 1 << 20, (1 << 25) + 5, n - 2, n - 1]
+    rng = np.random.default_rng(0)
+    some = rng.standard_normal((len(at), 4)).astype(np.float32)
+    x[at] = t(some)
+    p = gl.NormParams(n_rows=n, n_cols=4, x=x.data_ptr(), ldx=4, eps=0.0, out=out.data_ptr(), ldo=4)
+    ctx.check(ctx.lib.ggq_norm_dev(ctx.h, p, stream_handle()), "norm")
+    want = su.norm(some, eps=0.0)[1]
+    got = host(out[at])
+    assert (np.abs(got - want) <= (1 + 2.0 ** -20) * su.U32 * np.abs(want)).all()
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert bool((out[rest] == 1.0).all())
