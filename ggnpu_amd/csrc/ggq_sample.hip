@@ -101,6 +101,7 @@ __device__ __forceinline__ double eighths_of(const ggq_sample_params& p, int row
 struct Bin {
     double top;  // floor(z)
     u64 factor;  // 2^(frac / 8) in units of 2^-36
+    __device__ double weight() const { return (__builtin_bit_cast(double, factor + __builtin_bit_cast(u64, 65536.0)) - 65536.0) * 68719476736.0; }
 };
 // 2^(x / 8), x from 0 to 1
 __device__ __forceinline__ double factor_of(double x) {
@@ -283,8 +284,10 @@ template <typename T> __device__ __forceinline__ T sum16(T v) {
 }
 
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
-    __shared__ u64 mass[kBins];       // factors of a bin, in units of 2^-36
-    __shared__ uint32_t count[kBins];
+    // factors of a bin, in units of 2^-36, and its count; a lane's eight are followed by a gap, which keeps lanes off each other's banks
+    __shared__ u64 mass[kBins / 8 * 9];
+    __shared__ uint32_t count[kBins / 8 * 9];
+    auto apart = [](int j) { return j + (j >> 3); };
     __shared__ double tab[kBins];     // 2^(-j / 8)
     __shared__ int32_t shift[kMaxParts];
     __shared__ uint32_t run_at[kMaxParts], run_from[kMaxParts];  // of the tokens that are looked through: each part's first
@@ -361,22 +364,24 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
             uint32_t n = 0;
             u64 m = 0;
             if (tid < kRest)
-#pragma unroll 16
+#pragma unroll 32
                 for (int q = 0; q < a.parts; q++) {
                     const int j = tid - shift[q];
                     const u64 w = j >= 0 ? bins[(int64_t)q * kBins + j] : 0;
                     n += (uint32_t)(w >> kCount);
                     m += w & ((u64(1) << kCount) - 1);
                 }
-            count[tid] = n;
-            mass[tid] = m;
+            count[apart(tid)] = n;
+            mass[apart(tid)] = m;
             __syncthreads();
         }
         // running sums, eight bins a lane (in every wavefront)
         uint32_t nb[8], n_before, n_own = 0;
+        double wb[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            nb[i] = 8 * lane + i < kRest ? count[8 * lane + i] : 0;
+            nb[i] = 8 * lane + i < kRest ? count[9 * lane + i] : 0;
+            wb[i] = 8 * lane + i < kRest ? (double)mass[9 * lane + i] * ldexp(step_down(i), -lane) : 0.0;
             n_own += nb[i];
         }
         n_before = scan_add(n_own) - n_own;
@@ -416,7 +421,10 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
         // border's bin by parts; or, first of all, everything up to the border where that is little.
         enum { ALL = -1, TOP_K = 0, TOP_P = 1, KEEP = 2 };
         int listed_lo = -1, listed_hi = -1;
-        u64 kmass = bin_k < kRest ? mass[bin_k] : 0;  // factors that top-k keeps of its bin
+        int bin = kRest;  // top_p's
+        u64 left_p = 0;
+        const int most = a.parts > 1 ? 1 << (31 - __builtin_clz(a.parts - 1)) : 0;  // the largest power of two below the parts
+        u64 kmass = bin_k < kRest ? mass[apart(bin_k)] : 0;  // factors that top-k keeps of its bin
         border.bin = bin_k;
 #pragma nounroll
         for (int phase = ALL; phase <= KEEP; phase++) {
@@ -427,23 +435,24 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
             if (phase == TOP_K) {
                 if (bin_k == kRest) continue;
                 lo = hi = bin_k;
-                n = count[bin_k];
+                n = count[apart(bin_k)];
                 need = (uint32_t)flt.k - before_k;
                 if (need >= n) continue;
             } else if (phase == KEEP) {
                 if (border_m.bin < kRest && nearer(border_m, border)) border = border_m;
                 if (border.bin == kRest) break;
                 lo = hi = border.bin;
-                n = count[lo];
+                n = count[apart(lo)];
             } else {
                 // the first bin in which the weights reach top_p of their sum, by what is known of top-k's border
-                int bin = kRest;
-                if (flt.by_p) {
+                if (flt.by_p && (phase == ALL || bin_k < kRest)) {
                     double w[8], mine = 0.0;
+                    const double cut = border.bin < kRest ? (double)kmass * tab[border.bin] : 0.0;
+                    bin = kRest;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int j = 8 * lane + i;
-                        w[i] = j >= kRest || j > border.bin ? 0.0 : (double)(j == border.bin ? kmass : mass[j]) * tab[j];
+                        w[i] = j > border.bin ? 0.0 : j == border.bin && j < kRest ? cut : wb[i];
                         mine += w[i];
                     }
                     const double run = scan_add(mine);
@@ -459,12 +468,13 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
                     const int l = any ? __ffsll(any) - 1 : 0;
                     bin = lane_of(bin, l);
                     const double in = (want - lane_of(hb, l)) / tab[bin];  // in the bin's own units, rounded up
-                    left = in > 0.0 ? (u64)ceil(in) : 0;
+                    left_p = in > 0.0 ? (u64)ceil(in) : 0;
                 }
+                left = left_p;
                 if (phase == TOP_P) {
                     if (bin == kRest) continue;
                     lo = hi = bin;
-                    n = count[bin];
+                    n = count[apart(bin)];
                     by_mass = true;
                 } else {
                     // (top_p's share is of exactly what top-k leaves)
@@ -502,18 +512,35 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
                     __syncthreads();
                 }
             }
-            auto token_at = [&](uint32_t i) {
-                int q = 0;  // the last part whose run begins at i or before (parts without any share their begin with the next)
-                for (int s = 512; s > 0; s >>= 1)
+            auto part_at = [&](uint32_t i) {  // the last part whose run begins at i or before (parts without any share their begin with the next)
+                int q = 0;
+                for (int s = most; s > 0; s >>= 1)
                     if (q + s < a.parts && run_at[q + s] <= i) q += s;
-                const int idx = q * kPart + a.order[((int64_t)row * a.parts + q) * kPart + run_from[q] + i - run_at[q]];
+                return q;
+            };
+            auto index_at = [&](int q, uint32_t i) {
+                return q * kPart + a.order[((int64_t)row * a.parts + q) * kPart + run_from[q] + i - run_at[q]];
+            };
+            auto token_at = [&](uint32_t i) {
+                const int idx = index_at(part_at(i), i);
                 return place_of(key_of(x[idx]), (uint32_t)idx);
             };
             if (listed_lo != lo || listed_hi != hi) {
                 listed_lo = lo;
                 listed_hi = hi;
                 if (n <= kList) {
-                    for (uint32_t i = tid; i < n; i += kThreads) place[i] = token_at(i);
+                    // (four of a thread at a time: their loads depend on each other)
+                    for (uint32_t i = tid; i < n; i += 4 * kThreads) {
+                        int idx[4];
+                        float v[4];
+#pragma unroll
+                        for (int t = 0; t < 4; t++) idx[t] = i + t * kThreads < n ? index_at(part_at(i + t * kThreads), i + t * kThreads) : 0;
+#pragma unroll
+                        for (int t = 0; t < 4; t++) v[t] = x[idx[t]];
+#pragma unroll
+                        for (int t = 0; t < 4; t++)
+                            if (i + t * kThreads < n) place[i + t * kThreads] = place_of(key_of(v[t]), (uint32_t)idx[t]);
+                    }
                     __syncthreads();
                 }
             }
@@ -663,7 +690,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
             double whole = 0.0;
             if (flt.by_p && !flt.by_k) {  // top_p's share is of the whole row
 #pragma unroll
-                for (int i = 0; i < 8; i++) whole += 8 * lane + i < kRest ? (double)mass[8 * lane + i] * tab[8 * lane + i] : 0.0;
+                for (int i = 0; i < 8; i++) whole += wb[i];
                 whole = wave_sum(whole);
             }
             double kept[kFew * 16 / kThreads];
@@ -772,8 +799,20 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
     constexpr int V = kPart / kThreads;
     const int base = part * kPart + V * tid;
     float l[V];
+    static_assert(V % 4 == 0, "runs of four");
 #pragma unroll
-    for (int i = 0; i < V; i++) l[i] = base + i < p.n_vocab ? x[base + i] : -INFINITY;
+    for (int i = 0; i < V; i += 4) {
+        float4 y;
+        if (((uintptr_t)x & 15) == 0 && base + i + 3 < p.n_vocab) {
+            y = *(const float4*)(x + base + i);
+        } else {
+            float z[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) z[e] = base + i + e < p.n_vocab ? x[base + i + e] : -INFINITY;
+            y = make_float4(z[0], z[1], z[2], z[3]);
+        }
+        l[i] = y.x; l[i + 1] = y.y; l[i + 2] = y.z; l[i + 3] = y.w;
+    }
     double w[V], mine = 0.0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
@@ -782,7 +821,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
             const Bin b = bin_of(l[i], c);
             const int j = below(first, b.top);
             if (j < kRest && (j < border.bin || (j == border.bin && place_of(key_of(l[i]), (uint32_t)(base + i)) >= border.place)))
-                w[i] = (double)b.factor * tab[j];
+                w[i] = b.weight() * tab[j];
         }
         mine += w[i];
     }
