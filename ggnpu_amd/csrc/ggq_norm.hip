@@ -23,9 +23,39 @@ struct NormArgs {
     int lanes;  // a group's lanes where it is a power of two of up to a wavefront's (reduced by shuffles), else 0
 };
 
-template <int TPB, typename T, typename F> __device__ __forceinline__ T wg_reduce(T v, T* red, F f) {
+// Over neighbouring lanes (a power of two of them), by data-parallel moves: pairs, quads, halves and rows of 16 turned round, then
+// rows and halves swapped.  All lanes get the result.
+template <int CTRL, typename T> __device__ __forceinline__ T turned(T v) {
+    constexpr int W = sizeof(T) / 4;
+    struct Words { int w[W]; } x = __builtin_bit_cast(Words, v);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
+    for (int i = 0; i < W; i++) x.w[i] = __builtin_amdgcn_update_dpp(0, x.w[i], CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(T, x);
+}
+template <bool HALVES, typename T, typename F> __device__ __forceinline__ T swapped(T v, F f) {
+    constexpr int W = sizeof(T) / 4;
+    struct Words { uint32_t w[W]; } x = __builtin_bit_cast(Words, v), y = x;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        const auto r = HALVES ? __builtin_amdgcn_permlane32_swap(x.w[i], x.w[i], false, false)
+                              : __builtin_amdgcn_permlane16_swap(x.w[i], x.w[i], false, false);
+        x.w[i] = r[0];
+        y.w[i] = r[1];
+    }
+    return f(__builtin_bit_cast(T, x), __builtin_bit_cast(T, y));
+}
+template <typename T, typename F> __device__ __forceinline__ T lanes_reduce(T v, int lanes, F f) {
+    if (lanes > 1) v = f(v, turned<0xB1>(v));
+    if (lanes > 2) v = f(v, turned<0x4E>(v));
+    if (lanes > 4) v = f(v, turned<0x141>(v));
+    if (lanes > 8) v = f(v, turned<0x140>(v));
+    if (lanes > 16) v = swapped<false>(v, f);
+    if (lanes > 32) v = swapped<true>(v, f);
+    return v;
+}
+
+template <int TPB, typename T, typename F> __device__ __forceinline__ T wg_reduce(T v, T* red, F f) {
+    v = lanes_reduce(v, 64, f);
     if constexpr (TPB > 64) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -42,7 +72,38 @@ __device__ __forceinline__ uint32_t codes_of(const float4& y, float inv) {
     return code_of(y.x, inv) | code_of(y.y, inv) << 8 | code_of(y.z, inv) << 16 | code_of(y.w, inv) << 24;
 }
 __device__ __forceinline__ float step_of(float amax) { return amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f; }
-__device__ __forceinline__ double silu64(float z) { return (double)z / (1.0 + exp(-(double)z)); }
+// z / (1 + exp(-z)) within 2^-44, in half the instructions of the library's exp and division: a row's gate is most of its
+// arithmetic.  exp(x) = 2^n exp(r) with |r| <= ln(2) / 2, eleven terms (the next one is 2^-47 of the sum); a reciprocal and one step of Newton's.
+// (Beyond 700 the result is 0 after rounding to fp32, and the quotient of infinities NaN as it is.)
+__device__ __forceinline__ double silu64(float z) {
+    const double x = fmin(fmax(-(double)z, -700.0), 700.0), n = rint(x * 1.44269504088896340736);
+    const double r = fma(n, -1.6465949582897082e-12, fma(n, -0.6931471805582987, x));
+    double e = 1.0 / 39916800.0;
+    e = fma(e, r, 1.0 / 3628800.0);
+    e = fma(e, r, 1.0 / 362880.0);
+    e = fma(e, r, 1.0 / 40320.0);
+    e = fma(e, r, 1.0 / 5040.0);
+    e = fma(e, r, 1.0 / 720.0);
+    e = fma(e, r, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    const double d = 1.0 + ldexp(e, (int)n);
+    double q = __builtin_amdgcn_rcp(d);
+    q = fma(q, fma(-d, q, 1.0), q);
+    return (double)(z == -INFINITY ? __builtin_nanf("") : z) * q;
+}
+
+// 1 / sqrt(x) to 2^-50: the reciprocal root and two steps of Newton's (of 0: infinity, of infinity: 0).
+__device__ __forceinline__ double one_over_root(double x) {
+    double q = __builtin_amdgcn_rsq(x);
+    if (!(x > 0.0 && x < INFINITY)) return q;
+#pragma unroll
+    for (int i = 0; i < 2; i++) q = fma(0.5 * q, fma(-x * q, q, 1.0), q);
+    return q;
+}
 
 template <int TPB, int R>
 __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
@@ -54,7 +115,9 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
     if (m >= a.p.n_rows) return;
     const int tid = threadIdx.x, K = p.n_cols;
     const float* xr = p.x + m * p.ldx;
-    float4 v[R], g[R];
+    // (the longest rows fill the registers: their gate is read where it is used)
+    constexpr int NG = R > 4 ? 1 : R;
+    float4 v[R], g[NG];
 #pragma unroll
     for (int i = 0; i < R; i++) {
         const int k = 4 * (tid + TPB * i);
@@ -62,19 +125,26 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
     }
     if (p.add) {
         const float* ar = p.add + m * p.ld_add;
-        float4 b[R];
+        constexpr int B = R > 4 ? 4 : R;
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            const int k = 4 * (tid + TPB * i);
-            b[i] = k < K ? *(const float4*)(ar + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j = 0; j < R; j += B) {
+            float4 b[B];
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                const int k = 4 * (tid + TPB * (i + j));
+                b[i] = k < K ? *(const float4*)(ar + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                float4& x = v[i + j];
+                x = make_float4(x.x + b[i].x, x.y + b[i].y, x.z + b[i].z, x.w + b[i].w);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < R; i++) v[i] = make_float4(v[i].x + b[i].x, v[i].y + b[i].y, v[i].z + b[i].z, v[i].w + b[i].w);
     }
-    if (p.gate) {
-        const float* gr = p.gate + m * p.ld_gate;
+    const float* gr = p.gate + m * p.ld_gate;
+    if (p.gate && NG == R) {
 #pragma unroll
-        for (int i = 0; i < R; i++) {
+        for (int i = 0; i < NG; i++) {
             const int k = 4 * (tid + TPB * i);
             g[i] = k < K ? *(const float4*)(gr + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
@@ -100,14 +170,14 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < R; i++) ss += f[i];
         ss = wg_reduce<TPB>(ss, red, [](double s, double t) { return s + t; });
-        const double r = 1.0 / sqrt(ss / n + eps);
+        const double r = one_over_root(ss / n + eps);
 #pragma unroll
         for (int i = 0; i < R; i++) f[i] = r;
     } else if (a.lanes) {
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            for (int o = 1; o < a.lanes; o <<= 1) f[i] += __shfl_xor(f[i], o, 64);
-            f[i] = 1.0 / sqrt(f[i] / n + eps);
+            f[i] = lanes_reduce(f[i], a.lanes, [](double s, double t) { return s + t; });
+            f[i] = one_over_root(fma(f[i], 1.0 / n, eps));
         }
     } else {
 #pragma unroll
@@ -121,7 +191,7 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
             if (k >= K / 4) break;
             double ss = 0.0;
             for (int j = k / runs * runs, e = j + runs; j < e; j++) ss += parts[j];
-            f[i] = 1.0 / sqrt(ss / n + eps);
+            f[i] = one_over_root(ss / n + eps);
         }
     }
 #pragma unroll
@@ -134,7 +204,8 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
             y[0] *= (double)w.x; y[1] *= (double)w.y; y[2] *= (double)w.z; y[3] *= (double)w.w;
         }
         if (p.gate) {
-            y[0] *= silu64(g[i].x); y[1] *= silu64(g[i].y); y[2] *= silu64(g[i].z); y[3] *= silu64(g[i].w);
+            const float4 z = NG == R ? g[NG == R ? i : 0] : *(const float4*)(gr + k);
+            y[0] *= silu64(z.x); y[1] *= silu64(z.y); y[2] *= silu64(z.z); y[3] *= silu64(z.w);
         }
         v[i] = make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
     }
@@ -165,9 +236,7 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < R; i++) {
             float t = top[i];
-            t = fmaxf(t, __shfl_xor(t, 1, 64));
-            t = fmaxf(t, __shfl_xor(t, 2, 64));
-            t = fmaxf(t, __shfl_xor(t, 4, 64));
+            t = lanes_reduce(t, 8, [](float s, float u) { return fmaxf(s, u); });
             const int k = tid + TPB * i;
             const float sc = step_of(t);
             if (k >= K / 4) continue;
