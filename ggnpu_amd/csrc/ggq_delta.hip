@@ -8,7 +8,7 @@
 // Row by row (delta_rows_kernel): a column is spread over 16 lanes, k_dim / 16
 // numbers each; both dots of a row are taken of the state before it (S^T q after
 // it is a S^T q + (k.q) u), so that their sums over the lanes run side by side.
-// Single tokens are bound by their states' bytes.
+// Single tokens are bound by their states' bytes: 48 of 32 heads of 128 x 128 34 us, 6 TB/s.
 //
 // In parts of 16 rows: with G the running sum of the decays' logarithms within
 // the part and c = exp(G), the rows' u obey
@@ -24,6 +24,9 @@
 // one barrier a part.  S^T's rows in a lane are those that the next product's operand
 // wants of that lane (step e of a product takes k = 4 g + e from lane group g), so the
 // state goes from product to product in its registers.
+// Bound: the chain of a part's steps.  8191 rows of 32 heads of 128 x 128: parts 51 us (their rows' bytes 33), scan 365, a part 1750 cycles, of which its 29 products
+// take 960 (the four products of a part's rows and the state 200 us in all); the other half is what cannot stand beside
+// an fp32 product of the same wavefront: own arithmetic, the sums' way through LDS, the barrier.
 #include <algorithm>
 #include <climits>
 #include <cstdlib>

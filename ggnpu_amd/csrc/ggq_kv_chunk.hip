@@ -11,6 +11,11 @@
 // once, and no column is empty where the pairs fill the tiles.
 //   A workgroup has 16 CT columns; its wavefronts take the records of its part of the
 // positions in turn and add up in LDS, kv_chunk_join_kernel adds up the parts.
+// Two tiles where a sequence's pairs fill more than one: a record is decoded once for 32
+// columns.  Calls of many rows go through planes of operands (kv_chunk_plan).
+// Bound: few pairs a kv head, loads in flight (24 sequences of 4 rows over 6000 positions, 32 x 8 heads
+// of 128 in 8 / 4 bits, 43 + 5 us, 4.0 TB/s); more, decoding each record a tile again (64 rows over 65000 positions 294 us in
+// eight tiles of 37).
 #include <algorithm>
 #include <cstdlib>
 
