@@ -500,12 +500,14 @@ KvChunkPlan kv_chunk_plan(const KvChunkArgs& a, bool workspace) {
     if (a.window > 0) span = std::min<int64_t>(span, (int64_t)a.window + a.n_rows / a.q.n_seq + kKvTile);
     const int64_t records = (span + kKvTile - 1) / kKvTile;
     // Planes of operands (codes decoded once, two fp16 products where this kernel has three) from so many pairs a sequence
-    // on that they pay for the planes, in calls that are more than their launches (us, tiles -> planes; rows against positions):
-    //   32x8x128: 256 x 7000 122 -> 98, 64 58 -> 63; 512 x 700 42 -> 51, 1024 94 -> 79; 8 sequences 256 x 2000 149 -> 143
-    //   32x8x64: 512 x 4000 86 -> 78, 1024 130 -> 137, 1500 190 -> 245, 2048 281 -> 272
-    //   16x2x256: 256 x 4000 71 -> 77, 384 104 -> 91, 1024 230 -> 193
+    // on that they pay for the planes, in calls that are more than their launches (us, tiles -> planes; pairs: rows times heads of
+    // a kv head; 8 / 8 bits):
+    //   32x8x128: one of 7000 positions 384 pairs 53 -> 67, 512 85 -> 75, 1024 103 -> 94, 2048 166 -> 144; of 65000, 384 346 -> 349,
+    //     512 548 -> 370, 1024 741 -> 596; 16 of 4000, 384 313 -> 318, 512 395 -> 347, 1024 757 -> 620
+    //   32x8x64: one of 7000, 2048 124 -> 127, 4096 191 -> 230; of 65000, 1024 447 -> 500, 2048 873 -> 939
+    //   16x2x256: one of 7000, 1024 59 -> 87, 4096 172 -> 164; of 65000, 512 204 -> 227, 1024 388 -> 364, 2048 756 -> 650
     const int64_t mean = ((int64_t)a.n_rows + a.q.n_seq - 1) / a.q.n_seq * (a.n_head / c.n_kv_head);
-    const int64_t least = c.head_dim == 64 ? 8192 : c.head_dim == 128 ? 1024 : 2560;
+    const int64_t least = c.head_dim == 64 ? 8192 : c.head_dim == 128 ? 512 : 1024;
     const char* env = getenv("GGQ_KV_PLANES");
     if (a.row_off && (env && *env ? atoi(env) != 0 : mean >= least && mean * a.q.n_seq * c.n_kv_head * records >= 1000000)) {
         const AttnPromptPlan planes = attn_kv_planes_plan(a);
