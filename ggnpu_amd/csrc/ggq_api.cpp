@@ -1322,8 +1322,8 @@ int ggq_attention_kv_rows_dev(ggq_ctx* c, const ggq_kv_cache* cache, const ggq_k
     if (n_rows < 0 || ldq < row || ldo < row || window < 0 || !std::isfinite(scale))
         return set_status(c, GGQ_INVALID_PARAM, "need n_rows >= 0, ldq, ldo of a row or more, window >= 0 and a finite scale");
     // (a grid has fewer than 2^32 threads a dimension)
-    if ((int64_t)n_rows * (n_head / cache->n_kv_head) / 16 + seqs->n_seq >= 1 << 24)
-        return set_status(c, GGQ_INVALID_PARAM, "n_rows * n_head / n_kv_head is too large");
+    if (((int64_t)n_rows * (n_head / cache->n_kv_head) / 16 + seqs->n_seq) * cache->n_kv_head >= 1 << 24)
+        return set_status(c, GGQ_INVALID_PARAM, "n_rows * n_head is too large");
     if (n_rows == 0 || seqs->n_seq == 0) return set_status(c, GGQ_OK);
     if (!q || !out) return set_status(c, GGQ_INVALID_PARAM, "null q/out");
     if (!aligned16(q) || !aligned16(out) || ldq % 4 || ldo % 4)

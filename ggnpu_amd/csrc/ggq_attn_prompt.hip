@@ -563,7 +563,7 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
                 if (w < wave) run += s_sum[w];
                 all += s_sum[w];
             }
-            return all;
+            return __builtin_amdgcn_readfirstlane(all);
         };
         int total = 0, mine = 0, run = 0;
         if (p.n_seq == 1) {

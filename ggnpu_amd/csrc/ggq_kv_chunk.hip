@@ -67,24 +67,22 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
     auto so = (float(*)[NC][HD + 1])lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r = lane & 15;
-    const int kvh = blockIdx.y, split = blockIdx.z, id = blockIdx.x;
+    const int kvh = blockIdx.x % a.c.n_kv_head;
+    const unsigned turn = blockIdx.x / (unsigned)a.c.n_kv_head;
     const int G = a.n_head / a.c.n_kv_head;  // query heads of this kv head
     const int tpp = a.c.page_len / kKvTile;
-    // The tile's sequence: tiles are numbered through, by a running sum over the offsets.  (Numbers behind the last tile are
-    // the last workgroups: they do not hold up others.)
+    // The tile's sequence: tiles are numbered through, once for each part, by a running sum over the offsets.  (Numbers behind the
+    // last tile are the last workgroups: they do not hold up others.)
     __shared__ int32_t s_sum[NW], s_find[5];
-    if (tid == 0) s_find[0] = -1;
-    int before = 0;
-    for (int i = 0; i < a.q.n_seq; i += NW * 64) {
-        const int j = i + tid;
-        int off0 = 0, off1 = 0, len = 0;
+    int off0, off1, len_j, mine, run;
+    auto scan = [&](int j) {  // tiles up to sequence j of this turn's threads; returns their sum
+        off0 = off1 = len_j = 0;
         if (j < a.q.n_seq) {
             off0 = a.row_off ? a.row_off[j] : j;
             off1 = a.row_off ? a.row_off[j + 1] : j + 1;
-            len = a.q.len[j];
+            len_j = a.q.len[j];
         }
-        const int mine = tiles_in(off0, off1, a.n_rows, G, NC);
-        int run = mine;
+        mine = run = tiles_in(off0, off1, a.n_rows, G, NC);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int t = __shfl_up(run, o, 64);
@@ -99,23 +97,44 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
             if (w < wave) run += s_sum[w];
             all += s_sum[w];
         }
-        run += before;
-        if (id >= run - mine && id < run) {
-            s_find[1] = id - (run - mine);
-            s_find[2] = min(max(off0, 0), a.n_rows);
-            s_find[3] = min(max(off1, 0), a.n_rows);
-            s_find[4] = len;
-            s_find[0] = j;
+        return __builtin_amdgcn_readfirstlane(all);
+    };
+    int total = 0, seq = 0, split, id, r0, nr;
+    int64_t len;
+    if (a.q.n_seq == 1) {
+        r0 = a.row_off ? min(max(a.row_off[0], 0), a.n_rows) : 0;
+        nr = (a.row_off ? min(max(a.row_off[1], 0), a.n_rows) : min(1, a.n_rows)) - r0;
+        len = a.q.len[0];
+        total = tiles_in(r0, r0 + nr, a.n_rows, G, NC);
+        if (turn >= (unsigned)total * (unsigned)splits) return;
+        split = (int)(turn / (unsigned)total);
+        id = (int)(turn % (unsigned)total);
+    } else {
+        for (int i = 0; i < a.q.n_seq; i += NW * 64) total += scan(i + tid);
+        if (turn >= (unsigned)total * (unsigned)splits) return;
+        split = (int)(turn / (unsigned)total);
+        id = (int)(turn % (unsigned)total);
+        for (int i = 0, before = 0; before <= id; i += NW * 64) {
+            const int all = a.q.n_seq > NW * 64 ? scan(i + tid) : total;
+            const int at = id - (before + run - mine);
+            if (at >= 0 && at < mine) {
+                s_find[0] = i + tid;
+                s_find[1] = at;
+                s_find[2] = min(max(off0, 0), a.n_rows);
+                s_find[3] = min(max(off1, 0), a.n_rows);
+                s_find[4] = len_j;
+            }
+            before += all;
         }
-        before += all;
         __syncthreads();
-        if (s_find[0] >= 0) break;
+        seq = __builtin_amdgcn_readfirstlane(s_find[0]);
+        id = __builtin_amdgcn_readfirstlane(s_find[1]);
+        r0 = __builtin_amdgcn_readfirstlane(s_find[2]);
+        nr = __builtin_amdgcn_readfirstlane(s_find[3]) - r0;
+        len = __builtin_amdgcn_readfirstlane(s_find[4]);
     }
-    const int seq = __builtin_amdgcn_readfirstlane(s_find[0]);
-    if (seq < 0) return;
-    const int r0 = __builtin_amdgcn_readfirstlane(s_find[2]), nr = __builtin_amdgcn_readfirstlane(s_find[3]) - r0;
-    const int nf = nr * G, f0 = __builtin_amdgcn_readfirstlane(s_find[1]) * NC;
-    const int64_t len = __builtin_amdgcn_readfirstlane(s_find[4]), lim = min(min(len, (int64_t)a.q.max_len), (int64_t)a.q.table_len * a.c.page_len);
+    const int nf = nr * G, f0 = id * NC;
+    const int64_t lim = min(min(len, (int64_t)a.q.max_len), (int64_t)a.q.table_len * a.c.page_len);
     // columns: pair f has row f / G at position len - nr + f / G; it sees positions beg .. end - 1
     auto end_of = [&](int f) { return len - nr + f / G + 1; };
     auto see = [&](int f, int& b, int& e) {
@@ -471,7 +490,7 @@ template <int HD, int KB, int VB> int splits_go(const KvChunkArgs& a, int ct, in
 }
 
 template <int HD, int KB, int VB> hipError_t chunk_go(const KvChunkArgs& a, const KvChunkPlan& pl, float* ws, hipStream_t s) {
-    const dim3 grid((unsigned)tiles_of(a, 16 * pl.tiles), (unsigned)a.c.n_kv_head, (unsigned)pl.splits);
+    const dim3 grid((unsigned)(tiles_of(a, 16 * pl.tiles) * a.c.n_kv_head * pl.splits));
     bool done = false;
     if constexpr (HD < 256)
         if (pl.tiles == 2) {
