@@ -14,8 +14,8 @@
 // Two tiles where a sequence's pairs fill more than one: a record is decoded once for 32
 // columns.  Calls of many rows go through planes of operands (kv_chunk_plan).
 // Bound: few pairs a kv head, loads in flight (24 sequences of 4 rows over 6000 positions, 32 x 8 heads
-// of 128 in 8 / 4 bits, 43 + 5 us, 4.0 TB/s); more, decoding each record a tile again (64 rows over 65000 positions 294 us in
-// eight tiles of 37).
+// of 128 in 8 / 4 bits, 43 + 5 us, 4.0 TB/s); more, decoding each record a tile again (64 rows over 65000 positions 214 us in
+// eight tiles).
 #include <algorithm>
 #include <cstdlib>
 
@@ -72,7 +72,8 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
     const int G = a.n_head / a.c.n_kv_head;  // query heads of this kv head
     const int tpp = a.c.page_len / kKvTile;
     // The tile's sequence: tiles are numbered through, once for each part, by a running sum over the offsets.  (Numbers behind the
-    // last tile are the last workgroups: they do not hold up others.)
+    // last tile are the last workgroups: workgroups go round the shader engines by their numbers, and ones without work in between
+    // leave some of the engines with a second round; 64 rows over 65000 positions took 296 us so, 214 now.)
     __shared__ int32_t s_sum[NW], s_find[5];
     int off0, off1, len_j, mine, run;
     auto scan = [&](int j) {  // tiles up to sequence j of this turn's threads; returns their sum
@@ -521,10 +522,10 @@ KvChunkPlan kv_chunk_plan(const KvChunkArgs& a, bool workspace) {
     // Planes of operands (codes decoded once, two fp16 products where this kernel has three) from so many pairs a sequence
     // on that they pay for the planes, in calls that are more than their launches (us, tiles -> planes; pairs: rows times heads of
     // a kv head; 8 / 8 bits):
-    //   32x8x128: one of 7000 positions 384 pairs 53 -> 67, 512 85 -> 75, 1024 103 -> 94, 2048 166 -> 144; of 65000, 384 346 -> 349,
-    //     512 548 -> 370, 1024 741 -> 596; 16 of 4000, 384 313 -> 318, 512 395 -> 347, 1024 757 -> 620
-    //   32x8x64: one of 7000, 2048 124 -> 127, 4096 191 -> 230; of 65000, 1024 447 -> 500, 2048 873 -> 939
-    //   16x2x256: one of 7000, 1024 59 -> 87, 4096 172 -> 164; of 65000, 512 204 -> 227, 1024 388 -> 364, 2048 756 -> 650
+    //   32x8x128: one of 7000 positions 512 pairs 60 -> 76, 768 93 -> 82, 2048 159 -> 142; of 65000, 384 329 -> 345, 512 369 -> 351,
+    //     1024 715 -> 592; 16 of 4000, 384 281 -> 315, 512 366 -> 338, 1024 704 -> 592
+    //   32x8x64: one of 7000, 2048 119 -> 124; of 65000, 1024 432 -> 487, 2048 833 -> 910
+    //   16x2x256: one of 7000, 1024 57 -> 83, 4096 167 -> 162; of 65000, 512 198 -> 230, 1024 377 -> 365, 2048 736 -> 647
     const int64_t mean = ((int64_t)a.n_rows + a.q.n_seq - 1) / a.q.n_seq * (a.n_head / c.n_kv_head);
     const int64_t least = c.head_dim == 64 ? 8192 : c.head_dim == 128 ? 512 : 1024;
     const char* env = getenv("GGQ_KV_PLANES");
