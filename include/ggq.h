@@ -395,7 +395,7 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * terms, as above; where long prompts go through planes of fp16 operands, a
  * weight is besides off by up to 2^-28 of the row's largest product of weight
  * and value.  q and out 16-byte aligned, ldq and ldo multiples of 4;
- * n_rows * n_head / n_kv_head below 2^28. */
+ * n_rows * n_head / 16 + n_seq * n_kv_head below 2^24. */
 int ggq_attention_kv_rows_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off,
                               int n_rows, const float* q, int64_t ldq, int n_head, float scale, int window, float* out,
                               int64_t ldo, void* stream);

@@ -412,3 +412,55 @@ def test_rows_and_states_beyond_four_gigabytes(ctx):
     ctx.check(ctx.lib.ggq_norm_dev(ctx.h, p, stream()), "norm")
     want = su.norm(x, eps=EPS)[1]
     au.check(host(y), want, 2 * su.U32 * np.abs(want) + 1e-37)
+
+
+@pytest.mark.parametrize("planes", ["0", "1"])
+def test_captured_attention_of_prompts_in_flight_together(ctx, monkeypatch, planes):
+    """Two captured calls of many rows that need workspace and an eager one, at once on three streams; lengths and offsets
+    rewritten between replays; every replay equals the eager call bit for bit."""
+    import torch
+    monkeypatch.setenv("GGQ_KV_PLANES", planes)
+    rng = np.random.default_rng(7)
+    n_seq, per, rows = 3, 24, 400
+    st = Step(ctx, n_seq, per, 8)
+    total = n_seq * per * PAGE
+    k, v = (t(rng.standard_normal((total, NKV, HD)).astype(np.float32)) for _ in range(2))
+    full, all_ = t(np.full(n_seq, per * PAGE, np.int32)), t(np.arange(n_seq + 1, dtype=np.int32) * per * PAGE)
+    seqs = gl.KvSeqs(n_seq, per, per * PAGE, st.table.data_ptr(), full.data_ptr())
+    ctx.check(ctx.lib.ggq_kv_store_dev(ctx.h, st.cache, seqs, ptr(all_), total, ptr(k), NKV * HD, ptr(v), NKV * HD, 0, stream()), "store")
+    qs = [t(rng.standard_normal((rows, NH, HD)).astype(np.float32)) for _ in range(3)]
+    outs, refs = ([torch.zeros_like(q) for q in qs] for _ in range(2))
+    lens, offs = [torch.zeros(n_seq, dtype=torch.int32, device="cuda") for _ in qs], [torch.zeros(n_seq + 1, dtype=torch.int32, device="cuda") for _ in qs]
+
+    def call(i, out, s):
+        own = gl.KvSeqs(n_seq, per, per * PAGE, st.table.data_ptr(), lens[i].data_ptr())
+        ctx.check(ctx.lib.ggq_attention_kv_rows_dev(ctx.h, st.cache, own, ptr(offs[i]), rows, ptr(qs[i]), NH * HD, NH, 0.0, 0, ptr(out), NH * HD, s), "attention")
+
+    call(0, outs[0], stream())  # sizes the workspace, and what captures take
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream() for _ in range(3)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g, stream=streams[i]):
+            call(i, outs[i], streams[i].cuda_stream)
+    for turn in range(4):
+        for i in range(3):
+            cut = np.sort(rng.integers(0, rows + 1, 2))
+            off = np.array([0, *cut, rows - turn], np.int32)
+            off[1:3] = np.minimum(off[1:3], off[3])
+            offs[i].copy_(t(off))
+            lens[i].copy_(t(np.minimum(np.diff(off) + rng.integers(0, 300, n_seq), per * PAGE).astype(np.int32)))
+            outs[i].fill_(7.0)
+            refs[i].fill_(7.0)
+        torch.cuda.synchronize()
+        for i in range(3):
+            if i < 2:
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+            else:
+                call(i, outs[i], streams[i].cuda_stream)
+        torch.cuda.synchronize()
+        for i in range(3):
+            call(i, refs[i], stream())
+        torch.cuda.synchronize()
+        for o, r in zip(outs, refs):
+            assert torch.equal(o, r), turn
