@@ -199,3 +199,32 @@ def test_more_rows_than_a_grid_dimension_holds(ctx):
     rest = torch.ones(n, dtype=torch.bool, device="cuda")
     rest[at] = False
     assert bool((out[rest] == 1.0).all())
+
+
+@pytest.mark.parametrize("cols", [256, 4096, 30000])
+def test_gates_of_all_sizes(ctx, cols):
+    """Gates from tiny to infinite: z / (1 + exp(-z)) of 64 bits (rounded once, half a subnormal step where that is the step)."""
+    rng = np.random.default_rng(cols)
+    z = np.array([-np.inf, np.inf, np.nan, -1e30, -800, -709.5, -700.1, -699.9, -104, -100, -88, -20, -1, -1e-30, -0.0, 0.0, 1e-40, 1e-8, 0.5, 3, 40,
+                  699, 701, 900, 1e38], np.float32)
+    gate = np.resize(z, (3, cols)).astype(np.float32)
+    gate[2] = (rng.standard_normal(cols) * np.exp2(rng.integers(-20, 10, cols))).astype(np.float32)
+    x = rng.standard_normal((3, cols)).astype(np.float32)
+    got = call(ctx, x, gate=gate)["out"]
+    with np.errstate(all="ignore"):
+        want = su.norm(x, gate=gate)[1]
+        f32 = want.astype(np.float32)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(f32))
+    at = np.isfinite(f32)
+    assert (np.abs(got[at] - want[at]) <= (1 + 2.0 ** -20) * su.U32 * np.abs(want[at]) + 2.0 ** -150).all()
+
+
+@pytest.mark.parametrize("norm_len", [0, 64, 128, 96])
+def test_rows_of_all_sizes_without_eps(ctx, norm_len):
+    """Square sums from 1e-76 to 1e76, and of nothing: NaN as 0 / 0 is."""
+    rng = np.random.default_rng(norm_len)
+    x = rng.standard_normal((6, 384)).astype(np.float32) * np.float32([[1e-38], [1e-20], [1], [1e18], [1e37], [0]])
+    got = call(ctx, x, norm_len=norm_len, eps=0.0)["out"]
+    want = su.norm(x, norm_len=norm_len, eps=0.0)[1]
+    assert np.isnan(got[5]).all()
+    assert (np.abs(got[:5] - want[:5]) <= (1 + 2.0 ** -20) * su.U32 * np.abs(want[:5])).all()
