@@ -37,6 +37,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // A block's scale from its byte.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
+// Under a block's scale, codes of this magnitude and above read back as infinite or NaN: with e the code's exponent bits, an e4m3
+// one is 2^(e - 7) or more and below twice that, an e2m1 one (e > 0) 2^(e - 1), both times 2^(byte - 127); 2^128 is infinite.
+template <int BITS> __device__ __forceinline__ uint32_t first_not_finite(uint32_t byte) {
+    if (byte == 255u) return 0u;
+    return BITS == 8 ? min(127u, 8u * (262u - byte)) : 2u * (256u - byte);
+}
+
 union Frag {
     uint32_t w[4];
     bf16x8 v;

@@ -235,20 +235,27 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
                     for (int t = 0; t < 2; t++) st[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t].v, q, st[t][n], 0, 0, 0);
                 }
         }
-        uint32_t poison = 0;  // positions whose values read back as NaN, which some columns see and some do not
+        uint32_t poison = 0;  // positions with values that read back as infinite or NaN, which some columns see and some do not
         if (partial) {
-            // codes of positions that no column sees, or that are NaN: zero, with a finite scale
+            // codes of positions that no column sees, or that have such values (a weight of 0 would make NaN of them): zero, with a
+            // finite scale
             uint32_t keep[8];
+            // (values are infinite under scales of 2^113 and more only: a byte's upper four bits all set)
+            const uint32_t sx = x.vs.x & x.vs.x << 1, sy = x.vs.y & x.vs.y << 1;
+            const bool huge = __any((((sx & sx << 2) | (sy & sy << 2)) & 0x80808080u) != 0);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int pos = base + 16 * (j / 4) + 4 * g + j % 4;
                 keep[j] = pos >= lo && pos < hi ? 0xFFFFFFFFu : 0u;
-                uint32_t bad = ((j < 4 ? x.vs.x : x.vs.y) >> (8 * (j & 3)) & 255u) == 255u;
-                if constexpr (VB == 8) {
+                constexpr uint32_t MAG = VB == 8 ? 127u : 7u;
+                auto any_from = [&](uint32_t least) {  // codes of this magnitude and above
+                    bool is = false;
 #pragma unroll
-                    for (int d = 0; d < VD; d++)
-                        bad |= (x.v[(j * VD + d) / 4] >> (8 * ((j * VD + d) % 4)) & 127u) == 127u;
-                }
+                    for (int d = 0; d < VD; d++) is |= (x.v[(j * VD + d) * VB / 32] >> ((j * VD + d) * VB % 32) & MAG) >= least;
+                    return is;
+                };
+                bool bad = VB == 8 && any_from(MAG);
+                if (huge) bad = any_from(first_not_finite<VB>((j < 4 ? x.vs.x : x.vs.y) >> (8 * (j & 3)) & 255u));
                 if (bad && keep[j]) {
                     poison |= 1u << j;
                     keep[j] = 0;

@@ -312,3 +312,44 @@ def test_refusals(ctx):
                dict(c=cache(n_kv_head=2), n_head=3), dict(n_head=65536), dict(scale=float("nan")), dict(window=-1), dict(n_rows=2147483647, n_head=64), dict(n_rows=1 << 28)):
         assert st(**kw) == gl.Status.INVALID_PARAM, kw
     torch.cuda.synchronize()
+
+
+def infinite_at(c, s, pos, keys=True, byte=254, code=None):
+    """Position pos of sequence s reads back as infinite, keys (if they are meant) and values: the largest code under 2^127, or another."""
+    v0, ks, vs, end = au.kv_record(c.hd, c.kt, c.vt)
+    rec = c.pool[c.table[s, pos // c.page_len]].reshape(c.n_kv, c.page_len // 32, end)[:, pos % c.page_len // 32]
+    p = pos % 32
+    for bits, value, at, sc in ((c.kt, False, 0, ks), (c.vt, True, v0, vs)):
+        if not (keys or value):
+            continue
+        places, _, scale = au.kv_places(c.hd, bits, value)
+        rec[:, at + places[p]] = (0x77 if bits == 4 else 0x7E) if code is None else code
+        rec[:, sc + scale[p]] = byte
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kt,vt", [(8, 4), (4, 8), (8, 8)])
+def test_hidden_positions_may_be_infinite(ctx, form, hd, kt, vt):
+    """Behind the sequences' ends, in front of their windows, and at the positions of later rows of the same tile."""
+    c = Case(30, [75, 64], [20, 10], 4, 2, hd, kt, vt, page_len=32)
+    clean, kept = c.call(ctx, window=30), c.pool.copy()
+
+    def check(rows):
+        dirty = c.call(ctx, window=30)
+        if form == "tiles":
+            assert np.array_equal(clean[rows], dirty[rows])
+        for r in rows:  # (by planes hidden values have a say in the powers of two, which is a matter of roundings)
+            s = int(r >= 20)
+            end = c.lens[s] - c.rows[s] + r - c.off[s] + 1
+            k, v, _ = c.seq_values(s)
+            au.check(dirty[r:r + 1], *row_of(c.q[r:r + 1], k[max(0, end - 30):end], v[max(0, end - 30):end], None, form == "planes"))
+
+    for s, n in enumerate(c.lens):
+        for pos in [p for p in range(c.table.shape[1] * 32) if p >= n or p < n - c.rows[s] + 1 - 30]:
+            infinite_at(c, s, pos)
+    check(range(30))
+    # seen by some of a tile's rows: the others keep theirs
+    c.pool = kept
+    infinite_at(c, 0, 75 - 8)  # rows 12 .. 19
+    infinite_at(c, 1, 64 - 10 + 1 - 30)  # row 0 of the second, by the window
+    check([r for r in range(30) if not (12 <= r < 20 or r == 20)])
