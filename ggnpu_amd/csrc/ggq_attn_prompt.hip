@@ -509,17 +509,17 @@ __device__ __forceinline__ void phase_end(bool loads) {
     else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// Whether position x of a record has a value that reads back as NaN.
-template <int HD> __device__ bool nan_value(const ggq_kv_cache& c, const uint8_t* rec, int x) {
+// What value d of a record's position x reads back as, if that is infinite or NaN, else 0.
+template <int HD> __device__ float not_finite_value(const ggq_kv_cache& c, const uint8_t* rec, int x, int d) {
     const int VB = c.v_type, VD = HD / 16;
     const uint8_t *vc = rec + kUnit * HD * c.k_type / 8, *vs = vc + kUnit * HD * VB / 8 + HD;
-    for (int blk = 0; blk < HD / 32; blk++)
-        if (vs[(4 * blk + x % 16 / 4) * 8 + 4 * (x / 16) + x % 4] == 255) return true;
-    for (int e = 0; VB == 8 && e < HD; e++) {
-        const int b = (4 * (x / 16) + x % 4) * VD + e % VD;
-        if ((vc[1024 * (b / 16) + 16 * (16 * (x % 16 / 4) + e / VD) + b % 16] & 127) == 127) return true;
-    }
-    return false;
+    const uint32_t byte = vs[(4 * (d / 32) + x % 16 / 4) * 8 + 4 * (x / 16) + x % 4];
+    const int at = (4 * (x / 16) + x % 4) * VD + d % VD, b = at * VB / 8;
+    const uint32_t w = vc[1024 * (b / 16) + 16 * (16 * (x % 16 / 4) + d / VD) + b % 16];
+    const uint32_t code = VB == 8 ? w : at % 2 ? w >> 4 : w & 15u, m = code & (VB == 8 ? 127u : 7u);
+    if (byte == 255u || (VB == 8 && m == 127u)) return __builtin_nanf("");
+    if (m < (VB == 8 ? first_not_finite<8>(byte) : first_not_finite<4>(byte))) return 0.0f;
+    return code == m ? INFINITY : -INFINITY;
 }
 
 template <int HD, typename T>
@@ -900,14 +900,18 @@ __global__ __launch_bounds__(waves_of<HD>() * 64) void attn_kernel(PromptArgs a)
         // infinities and NaN among the values are zero in the planes: here they come, to the rows that see them
         for (int u = u0; u < u1; u++) {
             if (!(*(const uint32_t*)(units + (u - u0) * stride + Head<HD>::info) & BAD_V)) continue;
-            if constexpr (Source<T>::cache) {  // (a NaN, whose row has no defined result)
+            if constexpr (Source<T>::cache) {
                 const uint8_t* rec = record_of(a, seq, kvh, u);
                 if (!rec) continue;
-                for (int x = max(u * kUnit, beg) - u * kUnit; x < min((u + 1) * kUnit, end) - u * kUnit; x++)
-                    if (nan_value<HD>(a.kv.c, rec, x)) {
+                for (int x = max(u * kUnit, beg) - u * kUnit; x < min((u + 1) * kUnit, end) - u * kUnit; x++) {
 #pragma unroll
-                        for (int d = 0; d < DB; d++) o[d] += __builtin_nanf("");
+                    for (int d = 0; d < DB; d++) {
+                        int d0 = 32 * d + 4 * h;
+                        asm volatile("" : "+v"(d0));  // (addresses are made here, not kept in registers throughout)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[d][i] += not_finite_value<HD>(a.kv.c, rec, x, d0 + 8 * (i / 4) + i % 4);
                     }
+                }
                 continue;
             } else
             for (int at = max(u * kUnit, beg); at < min((u + 1) * kUnit, end); at++) {

@@ -390,8 +390,9 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * those.  Rows in front of position 0 see nothing and get zeros, and so does
  * a row whose positions have no page; rows of no sequence stay as they were.
  * Positions that a row does not see, or that have no page, do not count,
- * whatever they hold; a row that sees a key or value that reads back as NaN has no
- * defined result (the others keep theirs).  Products are exact in fp32
+ * whatever they hold.  Where a row sees a value that reads back as infinite or
+ * NaN, its result is not finite; what it has elsewhere is not defined then, nor is
+ * a row that sees such a key (the others keep theirs).  Products are exact in fp32
  * terms, as above; where long prompts go through planes of fp16 operands, a
  * weight is besides off by up to 2^-28 of the row's largest product of weight
  * and value.  q and out 16-byte aligned, ldq and ldo multiples of 4;

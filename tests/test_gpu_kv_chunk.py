@@ -353,3 +353,18 @@ def test_hidden_positions_may_be_infinite(ctx, form, hd, kt, vt):
     infinite_at(c, 0, 75 - 8)  # rows 12 .. 19
     infinite_at(c, 1, 64 - 10 + 1 - 30)  # row 0 of the second, by the window
     check([r for r in range(30) if not (12 <= r < 20 or r == 20)])
+
+
+@pytest.mark.parametrize("kt,vt,byte,code", [(8, 4, 254, 0x77), (8, 4, 254, 0x44), (8, 4, 253, 0x66), (8, 8, 254, 0x7E), (8, 8, 247, 0x78), (8, 8, 250, 0xE1),
+                                             (4, 8, 253, 0x48)])
+def test_infinite_values_do_not_vanish(ctx, form, kt, vt, byte, code):
+    """A row that sees one is not finite, in both forms; rows that do not see it keep theirs.  (The codes are the largest, and those
+    that just pass 2^128.)"""
+    c = Case(31, [90], [40], 2, 1, 64, kt, vt, page_len=32)
+    clean = c.call(ctx)
+    infinite_at(c, 0, 70, keys=False, byte=byte, code=code)  # seen by rows 20 .. 39
+    assert (np.abs(c.seq_values(0)[1][70]) >= 2.0 ** 128).all()
+    o = c.call(ctx)
+    assert np.isfinite(o[:20]).all() and not np.isfinite(o[20:]).any()
+    if form == "tiles":
+        assert np.array_equal(o[:20], clean[:20])
