@@ -421,6 +421,26 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
         for (int e = 0; e < 4; e++) col_at[t][e] = ring + (((4 * g + e) * RPR + ((4 * (tile0 + t) + (r >> 2)) ^ (4 * g + e))) * 4 + (r & 3)) * 4;
     }
     f32x4 k[NT], q[NT];
+    // A row's number of u that is not finite makes all rows of its column so (a zero of T times one is NaN), and the results of the rows
+    // before it.  Their results again: row i is bad if T or the rest has such a number at i or, in its triangle, before; a bad row's u is
+    // taken as 0 and its result as NaN.  (The column's state is not finite any more, as it is row by row.)
+    auto results_again = [&](const f32x4& tr, const f32x4& rest, float ar, f32x4 of) {
+        f32x4 x{}, bad{};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool in = 4 * g + e <= r, t_is = __builtin_isfinite(tr[e]), r_is = __builtin_isfinite(rest[e]);
+            x = __builtin_amdgcn_mfma_f32_16x16x4f32(in && t_is ? tr[e] : 0.0f, r_is ? rest[e] : 0.0f, x, 0, 0, 0);
+            bad = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? 1.0f : 0.0f, r_is ? 0.0f : 1.0f, bad, 0, 0, 0);
+            bad = __builtin_amdgcn_mfma_f32_16x16x4f32(in && !t_is ? 1.0f : 0.0f, 1.0f, bad, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool is = bad[e] > 0.0f || !__builtin_isfinite(x[e]);
+            x[e] = is ? 0.0f : x[e];
+            of[e] = is ? __builtin_nanf("") : of[e];
+        }
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(ar, wave & 2 ? (wave & 1 ? x[3] : x[2]) : wave & 1 ? x[1] : x[0], of, 0, 0, 0);
+    };
     // One part.  Issue is in order, and an fp32 product keeps its own wavefront's other arithmetic out (an instruction
     // behind a product costs the product's end and 4 cycles each): so products stand in rows, arithmetic in a few groups, and
     // what waits (this part's other operands, the sums' way through LDS) in the shadow of products.  The slots of the ring
@@ -461,7 +481,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         q_s(2 * NT, 4 * NT);
         __builtin_amdgcn_sched_barrier(0);
-        f32x4 rest, of = (qs[0] + qs[1]) * qc, u{0, 0, 0, 0};
+        f32x4 rest, of_q = (qs[0] + qs[1]) * qc, u{0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 4; e++) rest[e] = fmaf(-kc[e], (x0[e] + x1[e]) + (x2[e] + x3[e]), v[e]);
 #pragma unroll
@@ -477,11 +497,12 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
         const f32x4 w = u * kf;
         const float ue = wave & 2 ? (wave & 1 ? u[3] : u[2]) : wave & 1 ? u[1] : u[0];
         __builtin_amdgcn_sched_barrier(0);
-        of = __builtin_amdgcn_mfma_f32_16x16x4f32(ar, ue, of, 0, 0, 0);
+        f32x4 of = __builtin_amdgcn_mfma_f32_16x16x4f32(ar, ue, of_q, 0, 0, 0);
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
             for (int t = 0; t < NT; t++) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kt[t][e], w[e], s[t], 0, 0, 0);
+        if (__any(!__builtin_isfinite(u[0]))) of = results_again(tr, rest, ar, of_q);
         s_o[odd][wave][lane] = of;
         __builtin_amdgcn_sched_barrier(0);
     };

@@ -472,6 +472,7 @@ int ggq_attention_prompt_dev(ggq_ctx* ctx, const ggq_attention_prompt_params* pa
  * in the call) go row by row, longer ones in parts of 16 rows, for which the rows'
  * values are solved together (the same result, rounded in another order); without workspace
  * for that (a buffer per stream, as for the matmuls) all go row by row.
+ * Numbers that are not finite reach no row before theirs, those of q no other row.
  * Rows are dense heads: q and k [n_k_head][k_dim], v and out
  * [n_v_head][v_dim], gate and beta [n_v_head], with row strides ld*.  k_dim
  * 64, 128 or 256, v_dim a multiple of 16 up to 512; all pointers but gate,

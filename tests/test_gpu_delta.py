@@ -330,3 +330,73 @@ def test_refusals(ctx):
         assert ctx.lib.ggq_last_error_message(ctx.h)
     assert i32 is not None
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("what", ["v", "v infinite", "one column of v", "k", "k infinite", "beta", "gate", "beta infinite"])
+@pytest.mark.parametrize("row", [0, 7, 15, 16, 37, 49])
+def test_a_row_that_is_not_finite_does_not_reach_back(ctx, form, what, row):
+    """Rows before it keep their results, also those that are solved together with it, and so do columns without it; what comes after
+    it is not finite."""
+    c = Case(40, [3, 50, 20], 1, 2, 64, 48)
+    clean = c.call(ctx)
+    at, end, odd = 3 + row, 53, [5] if what == "one column of v" else list(range(48))
+    bad = np.inf if "infinite" in what else np.nan
+    if what == "one column of v":
+        c.v[at, :, 5] = bad
+    elif what[0] == "k":
+        c.k[at, 0, 3] = bad
+    else:
+        {"v": c.v, "b": c.beta, "g": c.gate}[what[0]][at] = bad
+    o, so = c.call(ctx)
+    out, S, tol, S_tol = su.delta(*(x[3:at] for x in (c.q, c.k, c.v, c.gate, c.beta)), c.state[c.slot[1]])
+    check(o[3:at], out, tol)
+    assert not np.isfinite(o[at:end][:, :, odd]).any() and not np.isfinite(so[c.slot[1]][:, odd]).any()
+    for s in (0, 2):
+        r = slice(c.off[s], c.off[s + 1])
+        assert np.array_equal(o[r], clean[0][r]) and np.array_equal(so[c.slot[s]], clean[1][c.slot[s]])
+    if what == "one column of v":
+        rest = [d for d in range(48) if d != 5]
+        x, y = c.v.copy(), c.v.copy()
+        y[at, :, 5] = 0
+        c.v = y
+        want, S, tol, S_tol = su.delta(*(z[3:end] for z in (c.q, c.k, c.v, c.gate, c.beta)), c.state[c.slot[1]])
+        check(o[3:end][:, :, rest], want[:, :, rest], tol[:, :, rest])
+        check(so[c.slot[1]][:, rest], S[:, rest], S_tol[:, rest])
+
+
+def test_a_query_that_is_not_finite_spoils_its_row_only(ctx, form):
+    c = Case(41, [40], 1, 2, 64, 16)
+    a = c.call(ctx)
+    c.q[21, 0, 9] = np.nan
+    b = c.call(ctx)
+    rest = [r for r in range(40) if r != 21]
+    assert np.array_equal(a[0][rest], b[0][rest]) and np.array_equal(a[1], b[1]) and np.isnan(b[0][21]).all()
+
+
+@pytest.mark.parametrize("env", ["", "1", "2"])
+def test_not_finite_rows_of_many_sequences(ctx, monkeypatch, env):
+    """Long and short sequences, states in place, one state that is not finite from the start, several workgroups' worth of columns."""
+    monkeypatch.setenv("GGQ_DELTA_PARTS", env)
+    lens = [90, 1, 40, 5, 33, 64] + [1] * 20
+    c = Case(42, lens, 2, 4, 128, 32)
+    at = {0: 20, 2: 39, 3: 2, 5: 0}
+    for s, i in at.items():
+        c.v[c.off[s] + i, 1, 3] = np.nan
+    c.state[c.slot[4], 2, 7, 11] = np.nan
+    o, so = c.call(ctx, in_place=True)
+    for s in range(len(lens)):
+        a, e = c.off[s], c.off[s + 1]
+        v, S0 = c.v[a:e].copy(), c.state[c.slot[s]].copy()
+        spoilt, late = np.zeros((e - a, 4, 32), bool), np.zeros((4, 32), bool)
+        if s in at:
+            spoilt[at[s]:, 1, 3], late[1, 3], v[at[s], 1, 3] = True, True, 0
+        if s == 4:
+            spoilt[:, 2, 7], late[2, 7], S0[2, 7] = True, True, 0
+        want, S, tol, S_tol = su.delta(c.q[a:e], c.k[a:e], v, c.gate[a:e], c.beta[a:e], S0)
+        if s in at:  # (the rows before it)
+            x = su.delta(c.q[a:a + at[s]], c.k[a:a + at[s]], c.v[a:a + at[s]], c.gate[a:a + at[s]], c.beta[a:a + at[s]], S0)
+            want[:at[s]], tol[:at[s]] = x[0], x[2]
+        got, gS = o[a:e], so[c.slot[s]]
+        assert np.isnan(got[spoilt]).all() and np.isnan(gS[late]).all()
+        check(got[~spoilt], want[~spoilt], tol[~spoilt])
+        check(gS[~late], S[~late], S_tol[~late])
