@@ -7,7 +7,8 @@
 //   A logit l has z = 8 log2(e) l / T in 64 bits; its bin is floor(z) counted
 // down from the largest one's, its weight 2^(-bin / 8) * 2^(frac / 8), the
 // second factor (1 .. 1.09) in 36 bits after the point: sums over a bin are
-// integers, which no order of additions changes.
+// integers, which no order of additions changes.  frac is of the product before it was rounded to z: logits
+// millions of temperatures away from 0 keep the bits of their differences.
 //   sample_bins_kernel: parts of 4096 tokens; a part counts its tokens and
 // adds up their factors in 512 bins below its own largest (64 powers of two: what
 // is below counts as nothing), count and sum in one 64-bit LDS atomic, and puts its
@@ -112,11 +113,14 @@ __device__ __forceinline__ double factor_of(double x) {
     e = fma(e, x, 0.08664339759143012);
     return fma(e, x, 0.9999999999997022);
 }
+// What the product l c has above fl, which is floor of it rounded: from 0 to 1 but for that rounding.  (Where that is as large as 1, z beyond
+// 2^53, bins of different logits are 2^28 apart and more, and only equal ones, whose factors are equal, count: any factor will do.)
+__device__ __forceinline__ double frac_of(float l, double c, double fl) { return fmin(fmax(fma((double)l, c, -fl), -1.0), 2.0); }
 __device__ __forceinline__ Bin bin_of(float l, double c) {
-    const double z = (double)l * c, fl = floor(z);
+    const double fl = floor((double)l * c);
     if (l == INFINITY) return Bin{INFINITY, u64(1) << 36};
     // (a sum of 2^16 and more has its last bit at 2^-36)
-    return Bin{fl, __builtin_bit_cast(u64, factor_of(z - fl) + 65536.0) - __builtin_bit_cast(u64, 65536.0)};
+    return Bin{fl, __builtin_bit_cast(u64, factor_of(frac_of(l, c, fl)) + 65536.0) - __builtin_bit_cast(u64, 65536.0)};
 }
 __device__ __forceinline__ double floor_of(float l, double c) { return l == INFINITY ? INFINITY : floor((double)l * c); }
 // Bins that `at` lies below `top`, at most kRest.
@@ -211,9 +215,9 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a) 
         double m = 0.0;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const double z = (double)v[i] * c, fl = floor_of(v[i], c);
+            const double fl = floor_of(v[i], c);
             const double w = there(v[i]) ? __builtin_bit_cast(double, bins[below(first, fl)]) : 0.0;
-            m = fma(v[i] == INFINITY || !there(v[i]) ? 1.0 : factor_of(z - fl), w, m);
+            m = fma(v[i] == INFINITY || !there(v[i]) ? 1.0 : factor_of(frac_of(v[i], c, fl)), w, m);
         }
         m = wave_sum(m);
         if (lane == 0) sums[tid >> 6] = m;

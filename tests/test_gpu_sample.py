@@ -265,3 +265,38 @@ def test_no_workspace_while_capturing(ctx):
         torch.cuda.synchronize()
         assert int(tok[0]) == i
     c.close()
+
+
+def test_logits_far_from_zero_at_low_temperatures(ctx):
+    """A token and thousands of equal ones a step of fp32 below it, millions of temperatures away from 0: the border between them stays
+    where 64 bits have it.  u is the fp32 number next to the border, more than 2^-30 and less than 2^-26 away from it."""
+    rng = np.random.default_rng(20)
+    V, rows = 9001, []
+    while len(rows) < 60:
+        l0 = np.float32(np.exp2(rng.uniform(3, 17)))
+        l1 = np.nextafter(l0, np.float32(0), dtype=np.float32)
+        n = int(rng.integers(2000, 8000))
+        T = np.float32((float(l0) - float(l1)) / (np.log(n) + rng.uniform(-1, 1)))
+        w = np.exp((float(l1) - float(l0)) / float(T))
+        border = 1 / (1 + n * w)
+        u = np.float32(border)
+        if 2.0 ** -30 < abs(float(u) - border) < 2.0 ** -26:
+            x = np.full(V, -np.inf, np.float32)
+            x[7:7 + n], x[rng.integers(0, 7)] = l1, l0
+            rows.append((x, T, u))
+    x, T, u = (np.array([r[i] for r in rows], np.float32) for i in range(3))
+    check(ctx, x, u, temp=T)
+    check(ctx, x, u, temp=T, p=0.99999994)
+    check(ctx, x, u, temp=T, k=8999, m=1e-6)
+
+
+@pytest.mark.parametrize("T", [1e-40, 1e-25, 1e-12, 1e-9])
+def test_equal_logits_far_from_zero(ctx, T):
+    """Logits so many temperatures away from 0 that only equal ones have a weight."""
+    rng = np.random.default_rng(21)
+    x = rng.standard_normal((6, 9000)).astype(np.float32) * 10
+    x[:, 8999] = x[:, 17] = x[:, 5000] = x.max() + 3
+    x[3:] -= 1000
+    u = np.array([0.1, 0.5, 0.9] * 2, np.float32)
+    for kw in (dict(), dict(k=2), dict(p=0.5), dict(m=0.5), dict(k=100, p=0.9)):
+        check(ctx, x, u, temp=np.float32(T), **kw)
