@@ -418,6 +418,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
                 const int bin = below(first, floor_of(v, c));
                 if (bin < kRest) border_m = Border{bin, (u64)key << 32};
             }
+            if (flt.m > 1.0f) border_m = Border{0, top};  // (no weight is so large: the first token alone)
         }
         // What the filters look through, one after the other: the border of top-k, then of top-p, then what is kept of the
         // border's bin by parts; or, first of all, everything up to the border where that is little.

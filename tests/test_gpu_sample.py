@@ -300,3 +300,18 @@ def test_equal_logits_far_from_zero(ctx, T):
     u = np.array([0.1, 0.5, 0.9] * 2, np.float32)
     for kw in (dict(), dict(k=2), dict(p=0.5), dict(m=0.5), dict(k=100, p=0.9)):
         check(ctx, x, u, temp=np.float32(T), **kw)
+
+
+def test_min_p_above_one_keeps_the_first_token(ctx):
+    """No weight is above 1: the first token is left, also where others equal it (few of them and many, with and without other filters)."""
+    rng = np.random.default_rng(22)
+    x = rng.standard_normal((3, 9001)).astype(np.float32)
+    x[0, [40, 7000]] = 9.0
+    x[1, 100:5000] = 9.0
+    x[2, [3, 8000]] = np.inf
+    for m in (1.0000001, 2.0, np.inf):
+        for kw in (dict(), dict(k=3), dict(p=0.9), dict(k=3000, p=0.99)):
+            tok, pr = call(ctx, x, 0.99, m=m, **kw)
+            assert tok.tolist() == [40, 100, 3] and (pr == 1).all(), (m, kw)
+    tok, pr = call(ctx, x, 0.99, m=1.0)  # (1 itself: all that equal it)
+    assert tok.tolist() == [7000, 100 + int(np.float32(0.99) * np.float64(4900)), 8000]
