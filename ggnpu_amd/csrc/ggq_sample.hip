@@ -405,7 +405,8 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
         Border border_m{kRest, 0};
         if (flt.by_m) {
             // the smallest value with (value - largest) / T >= ln min_p
-            const double lim = flt.m >= 1.0f ? 0.0 : (double)t_row * log((double)flt.m);
+            // (at an infinite T all finite ones have the weight 1)
+            const double lim = t_row == INFINITY ? -INFINITY : flt.m >= 1.0f ? 0.0 : (double)t_row * log((double)flt.m);
             float v = (float)((double)mx + lim);
             if (!(v <= mx) || mx == INFINITY) v = mx;
             uint32_t key = key_of(v);

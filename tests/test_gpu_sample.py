@@ -315,3 +315,12 @@ def test_min_p_above_one_keeps_the_first_token(ctx):
             assert tok.tolist() == [40, 100, 3] and (pr == 1).all(), (m, kw)
     tok, pr = call(ctx, x, 0.99, m=1.0)  # (1 itself: all that equal it)
     assert tok.tolist() == [7000, 100 + int(np.float32(0.99) * np.float64(4900)), 8000]
+
+
+def test_min_p_at_an_infinite_temperature(ctx):
+    """All weights are 1: min_p up to 1 keeps every token."""
+    x = np.random.default_rng(23).standard_normal((1, 1000)).astype(np.float32)
+    for m in (1e-30, 0.5, 1.0):
+        assert call(ctx, x, 0.5004, temp=np.inf, m=m)[0][0] == 500
+        assert call(ctx, x, 0.5004, temp=np.inf, m=m, k=900, p=0.999)[0][0] == su.sample(x[0], np.inf, 900, 0.999, 0.0, 0.5004)[0]
+    assert call(ctx, x, 0.5004, temp=np.inf, m=2.0)[0][0] == x[0].argmax()
