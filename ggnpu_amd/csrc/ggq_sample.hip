@@ -411,8 +411,14 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
             if (!(v <= mx) || mx == INFINITY) v = mx;
             uint32_t key = key_of(v);
             if (v > -INFINITY && mx < INFINITY) {
-                while (key < top_key && (double)of_key(key) - (double)mx < lim) key++;
-                while (key > 0x00800000u && (double)of_key(key - 1) - (double)mx >= lim) key--;
+                // A step or two from here, but half a billion where v is next to nothing beside the largest (differences from
+                // that round to the same): strides that double, then halve.  (0x00800000: the smallest finite number's key.)
+                auto within = [&](uint32_t k) { return (double)of_key(k) - (double)mx >= lim; };
+                while (key < top_key && !within(key)) key++;
+                uint32_t stride = 1;
+                for (; key - 0x00800000u >= stride && within(key - stride); stride *= 2) key -= stride;
+                for (; stride; stride /= 2)
+                    if (key - 0x00800000u >= stride && within(key - stride)) key -= stride;
             }
             v = of_key(key);
             if (v > -INFINITY) {

@@ -324,3 +324,43 @@ def test_min_p_at_an_infinite_temperature(ctx):
         assert call(ctx, x, 0.5004, temp=np.inf, m=m)[0][0] == 500
         assert call(ctx, x, 0.5004, temp=np.inf, m=m, k=900, p=0.999)[0][0] == su.sample(x[0], np.inf, 900, 0.999, 0.0, 0.5004)[0]
     assert call(ctx, x, 0.5004, temp=np.inf, m=2.0)[0][0] == x[0].argmax()
+
+
+@pytest.mark.parametrize("T,m,top", [("0x1.d816cep-1", "0x1.b73bf4p-4", "0x1.078324p+1"), ("0x1.5530b2p-1", "0x1.a5ba9ep-4", "0x1.83d4dcp+0"),
+                                     ("0x1.76bf42p-1", "0x1.e081bcp-4", "0x1.918706p+0")])
+def test_min_p_whose_border_is_at_zero(ctx, T, m, top):
+    """T ln(min_p) is minus the largest logit to within 2^-53: hundreds of millions of numbers around 0 have that difference from it
+    in 64 bits."""
+    T, m, top = (np.float32(float.fromhex(v)) for v in (T, m, top))
+    x = np.full((2, 5000), -5, np.float32)
+    x[0, [9, 40, 41, 42]] = top, 1e-10, -1e-10, 0.01
+    x[1, 1000:3000], x[1, 3000:4000], x[1, 77] = 1e-10, -1e-10, top
+    w = np.exp((1e-10 - float(top)) / float(T))
+    tok, pr = call(ctx, x, 0.99999994, temp=T, m=m)
+    assert tok.tolist() == [42, 2999]
+    tok, pr = call(ctx, x, 0.99999994, temp=T, m=m, k=4000)
+    assert tok.tolist() == [42, 2999] and abs(pr[1] - w / (1 + 2000 * w)) <= pr[1] * (su.U32 + 2.0 ** -29)
+
+
+def test_min_p_borders(ctx):
+    """What min_p keeps, logit by logit, beside the largest ones of all sizes: the number at the border and its neighbours."""
+    rng = np.random.default_rng(24)
+    rows, temp, mins = [], [], []
+    for _ in range(200):
+        top = np.float32(rng.choice([-1, 1]) * np.exp2(rng.uniform(-20, 20)))
+        T, m = np.float32(np.exp2(rng.uniform(-8, 8))), np.float32(np.exp2(rng.uniform(-20, 0)))
+        at = float(top) + float(T) * np.log(float(m))
+        near = [np.float32(at)]
+        for _ in range(4):
+            near = [np.nextafter(near[0], np.float32(-np.inf))] + near + [np.nextafter(near[-1], np.float32(np.inf))]
+        # (a number whose weight is min_p's to within 2^-45 may be on either side)
+        near = [v for v in near if v <= top and abs((float(v) - float(top)) / float(T) - np.log(float(m))) > 2.0 ** -45 * max(1.0, abs(np.log(float(m))))]
+        x = np.full(300, -np.inf, np.float32)
+        x[0], x[100:100 + len(near)] = top, near
+        rows.append(x), temp.append(T), mins.append(m)
+    x, temp, mins = np.array(rows), np.array(temp), np.array(mins)
+    with np.errstate(all="ignore"):
+        keep = (x.astype(np.float64) - x[:, :1]) / temp[:, None].astype(np.float64) >= np.log(mins.astype(np.float64))[:, None]
+    keep[:, 0] = True
+    last = np.where(keep, np.arange(300), -1).max(1)
+    assert np.array_equal(call(ctx, x, 0.99999994, temp=temp, m=mins)[0], last)
