@@ -368,3 +368,47 @@ def test_infinite_values_do_not_vanish(ctx, form, kt, vt, byte, code):
     assert np.isfinite(o[:20]).all() and not np.isfinite(o[20:]).any()
     if form == "tiles":
         assert np.array_equal(o[:20], clean[:20])
+
+
+def test_the_rule_takes_planes_beyond_both_limits(ctx, monkeypatch):
+    """512 rows of four heads a kv head over 4000 positions: an unforced call is the one by planes, bit for bit."""
+    monkeypatch.delenv("GGQ_KV_PLANES", raising=False)
+    c = Case(32, [4000], [512], 32, 8, 128, 4, 4)
+    a = c.call(ctx)
+    monkeypatch.setenv("GGQ_KV_PLANES", "1")
+    assert np.array_equal(a, c.call(ctx))
+    monkeypatch.setenv("GGQ_KV_PLANES", "0")
+    b = c.call(ctx)
+    assert not np.array_equal(a, b)
+    k, v, _ = c.seq_values(0)
+    for r in (0, 300, 511):
+        n = 4000 - 512 + r + 1
+        for planes, o in ((True, a), (False, b)):
+            au.check(o[r:r + 1], *row_of(c.q[r:r + 1], k[:n], v[:n], None, planes))
+
+
+def test_planes_without_workspace_become_tiles(ctx, monkeypatch):
+    """A captured call of such a size in a context with nothing set aside goes by tiles, in one part: the same results within the bound
+    at every replay."""
+    import torch
+    monkeypatch.delenv("GGQ_KV_PLANES", raising=False)
+    c = Case(33, [4000], [512], 32, 8, 128, 4, 4)
+    k, v, _ = c.seq_values(0)
+    mem, table, lens, off, q = t(c.pool), t(c.table), t(np.asarray(c.lens, np.int32)), t(c.off), t(c.q)
+    out = torch.empty_like(q)
+    x, s, g = gl.Context(0), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    cache = gl.KvCache(mem.data_ptr(), len(c.pool), c.page_len, c.n_kv, c.hd, c.kt, c.vt)
+    seqs = gl.KvSeqs(1, c.table.shape[1], 4000, table.data_ptr(), lens.data_ptr())
+    with torch.cuda.graph(g, stream=s):
+        st = x.lib.ggq_attention_kv_rows_dev(x.h, cache, seqs, ptr(off), 512, ptr(q), 32 * 128, 32, 0.0, 0, ptr(out), 32 * 128,
+                                             ctypes.c_void_p(s.cuda_stream))
+    assert st == 0
+    for _ in range(3):
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        o = host(out)
+        for r in (0, 129, 511):
+            n = 4000 - 512 + r + 1
+            au.check(o[r:r + 1], *row_of(c.q[r:r + 1], k[:n], v[:n], None, False))
+    x.close()
