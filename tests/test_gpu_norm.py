@@ -228,3 +228,14 @@ def test_rows_of_all_sizes_without_eps(ctx, norm_len):
     want = su.norm(x, norm_len=norm_len, eps=0.0)[1]
     assert np.isnan(got[5]).all()
     assert (np.abs(got[:5] - want[:5]) <= (1 + 2.0 ** -20) * su.U32 * np.abs(want[:5])).all()
+
+
+@pytest.mark.parametrize("K,L", [(32768, 512), (32768, 8192), (32768, 16384), (32736, 1488)])
+def test_long_groups_of_the_longest_rows(ctx, K, L):
+    """Groups that are no power of two of lanes up to a wavefront's, in rows whose groups' sums take 64 KiB of LDS and what the rest takes."""
+    rng = np.random.default_rng(L)
+    x, w = rows(rng, 3, K), (1 + 0.2 * rng.standard_normal(L)).astype(np.float32)
+    gate = (3 * rng.standard_normal((3, K))).astype(np.float32)
+    for g in (None, gate):
+        for act in (0, 1, 2):
+            check(call(ctx, x, w=w, norm_len=L, gate=g, act=act), x, w=w, norm_len=L, gate=g, act=act)
