@@ -1394,9 +1394,9 @@ int ggq_norm_dev(ggq_ctx* c, const ggq_norm_params* p, void* stream) {
         return set_status(c, GGQ_INVALID_PARAM, "null x, no output, or codes without codes/scales");
     if (!aligned16(p->norm_w) || (p->act_mode != GGQ_ACT_F32 && !aligned16(p->codes)))
         return set_status(c, GGQ_INVALID_PARAM, "norm_w and codes must be 16-byte aligned");
-    if ((p->sum && ((p->sum == p->x && p->ld_sum != p->ldx) || (p->sum == p->add && p->ld_sum != p->ld_add))) ||
-        (p->out && p->out == p->x && p->ldo != p->ldx) || (p->out && p->out == p->sum))
-        return set_status(c, GGQ_INVALID_PARAM, "sum over x or add and out over x take the same stride; out and sum are apart");
+    if ((p->sum && ((p->sum == p->x && p->ld_sum != p->ldx) || (p->sum == p->add && p->ld_sum != p->ld_add) || p->sum == p->gate)) ||
+        (p->out && ((p->out == p->x && p->ldo != p->ldx) || p->out == p->add || p->out == p->gate || p->out == p->sum)))
+        return set_status(c, GGQ_INVALID_PARAM, "sum goes over x or add and out over x with the same stride, neither over the gate, out not over add or sum");
     return hip_status(c, ggq::launch_norm(*p, pick_stream(c, stream)), "norm");
     GGQ_END(c)
 }

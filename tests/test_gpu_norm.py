@@ -239,3 +239,16 @@ def test_long_groups_of_the_longest_rows(ctx, K, L):
     for g in (None, gate):
         for act in (0, 1, 2):
             check(call(ctx, x, w=w, norm_len=L, gate=g, act=act), x, w=w, norm_len=L, gate=g, act=act)
+
+
+def test_overlaps_that_are_refused(ctx):
+    """The sum may go over x or add and the rows over x; nothing goes over the gate, the rows not over add or the sum."""
+    import torch
+    b = torch.zeros(1 << 16, device="cuda")
+    P = b.data_ptr()
+    ok = dict(n_rows=2, n_cols=64, x=P, ldx=64, add=P + 4096, ld_add=64, gate=P + 8192, ld_gate=64, out=P + 16384, ldo=64, sum=P + 32768, ld_sum=64, eps=1e-6)
+    st = lambda **kw: ctx.lib.ggq_norm_dev(ctx.h, gl.NormParams(**{**ok, **kw}), stream_handle())  # noqa: E731
+    assert st() == 0 and st(sum=P) == 0 and st(sum=P + 4096) == 0 and st(out=P) == 0
+    for kw in (dict(sum=P + 8192), dict(out=P + 4096), dict(out=P + 8192), dict(out=P + 32768), dict(out=P, sum=P)):
+        assert st(**kw) == gl.Status.INVALID_PARAM, kw
+    torch.cuda.synchronize()
