@@ -252,3 +252,22 @@ def test_overlaps_that_are_refused(ctx):
     for kw in (dict(sum=P + 8192), dict(out=P + 4096), dict(out=P + 8192), dict(out=P + 32768), dict(out=P, sum=P)):
         assert st(**kw) == gl.Status.INVALID_PARAM, kw
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("act", [1, 2])
+@pytest.mark.parametrize("K", [96, 2048, 20000])
+def test_codes_are_those_of_the_quantizer(ctx, K, act):
+    """Codes and scales beside the rows are what ggq_quantize_act_dev makes of these, also of rows with numbers that are not finite."""
+    import torch
+    rng = np.random.default_rng(K)
+    x = rows(rng, 8, K)
+    x[1, 5], x[2, K - 1], x[3, ::3], x[4] = np.nan, np.inf, -np.inf, 0
+    x[5] *= 1e30
+    gate = (3 * rng.standard_normal((8, K))).astype(np.float32)
+    gate[6, 7], gate[7, 40:60] = np.inf, np.nan
+    r = call(ctx, x, gate=gate, act=act, eps=0.0)
+    y = t(r["out"])
+    q = torch.empty((8, K), dtype=torch.int8, device="cuda")
+    sc = torch.empty(r["scales"].shape, device="cuda")
+    ctx.check(ctx.lib.ggq_quantize_act_dev(ctx.h, ptr(y), K, 8, K, act, ptr(q), ptr(sc), stream_handle()), "quantize")
+    assert np.array_equal(r["codes"], host(q)) and np.array_equal(r["scales"], host(sc), equal_nan=True)
