@@ -206,6 +206,21 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
         }
         x.vs = *(const uint2*)(rec + HD + (4 * (r * VD / 32) + g) * 8);
     };
+    // Positions of this lane (a bit each) with values that read back as infinite or NaN: read anew, few caches hold any.
+    auto not_finite = [&](int it) {
+        const int t = first + wave + NW * it;
+        const uint8_t* rec = (const uint8_t*)a.c.pages +
+                             (((int64_t)a.q.pages[(int64_t)seq * a.q.table_len + t / tpp] * a.c.n_kv_head + kvh) * tpp + t % tpp) * RB + kKvTile * HD * KB / 8;
+        const uint8_t* scales = rec + kKvTile * HD * VB / 8 + HD + (4 * (r * VD / 32) + g) * 8;
+        uint32_t odd = 0;
+#pragma nounroll
+        for (int i = 0; i < 8 * VD; i++) {  // (in the order of the lane's codes)
+            const int b = i * VB / 8;
+            const uint32_t code = rec[1024 * (b / 16) + 16 * lane + b % 16] >> (i * VB % 8) & (VB == 8 ? 127u : 7u);
+            odd |= (code >= first_not_finite<VB>(scales[i / VD]) ? 1u : 0u) << (i / VD);
+        }
+        return odd;
+    };
     auto compute = [&](int it, Rec& x) {
         if (!x.there) return;
         const int base = (first + wave + NW * it) * kKvTile;
@@ -239,23 +254,20 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
         if (partial) {
             // codes of positions that no column sees, or that have such values (a weight of 0 would make NaN of them): zero, with a
             // finite scale
-            uint32_t keep[8];
-            // (values are infinite under scales of 2^113 and more only: a byte's upper four bits all set)
+            uint32_t keep[8], odd = 0;
+            // (but for e4m3's NaN they are under scales of 2^113 and more only: a byte's upper four bits all set)
             const uint32_t sx = x.vs.x & x.vs.x << 1, sy = x.vs.y & x.vs.y << 1;
-            const bool huge = __any((((sx & sx << 2) | (sy & sy << 2)) & 0x80808080u) != 0);
+            if (__any((((sx & sx << 2) | (sy & sy << 2)) & 0x80808080u) != 0)) odd = not_finite(it);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int pos = base + 16 * (j / 4) + 4 * g + j % 4;
                 keep[j] = pos >= lo && pos < hi ? 0xFFFFFFFFu : 0u;
-                constexpr uint32_t MAG = VB == 8 ? 127u : 7u;
-                auto any_from = [&](uint32_t least) {  // codes of this magnitude and above
-                    bool is = false;
+                uint32_t bad = odd >> j & 1u;
+                if constexpr (VB == 8) {
 #pragma unroll
-                    for (int d = 0; d < VD; d++) is |= (x.v[(j * VD + d) * VB / 32] >> ((j * VD + d) * VB % 32) & MAG) >= least;
-                    return is;
-                };
-                bool bad = VB == 8 && any_from(MAG);
-                if (huge) bad = any_from(first_not_finite<VB>((j < 4 ? x.vs.x : x.vs.y) >> (8 * (j & 3)) & 255u));
+                    for (int d = 0; d < VD; d++)
+                        bad |= (x.v[(j * VD + d) / 4] >> (8 * ((j * VD + d) % 4)) & 127u) == 127u;
+                }
                 if (bad && keep[j]) {
                     poison |= 1u << j;
                     keep[j] = 0;
