@@ -48,11 +48,12 @@ __device__ __forceinline__ void parts_of(float a, float b, uint32_t (&w)[3]) {
 }
 
 template <int HD, int CT> constexpr int chunk_waves() { return 4; }
-// Wavefronts of a SIMD, by their registers.
-template <int HD, int CT> constexpr int chunk_side() { return HD * CT <= 128 ? 4 : 2; }
+// Wavefronts of a SIMD, by their registers.  (Two records of 128-wide heads in 8 / 8 bits do not fit beside the rest four times: 9 registers
+// spilled, 24 sequences of 4 rows over 6000 positions 86 us and 64 single rows over 4000 134; 74 and 100 with three wavefronts.)
+template <int HD, int CT, int BITS> constexpr int chunk_side() { return HD * CT > 128 ? 2 : HD == 128 && BITS == 16 ? 3 : 4; }
 
 template <int HD, int KB, int VB, int CT>
-__global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>())) void kv_chunk_kernel(KvChunkArgs a, int splits, float* part) {
+__global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT, KB + VB>())) void kv_chunk_kernel(KvChunkArgs a, int splits, float* part) {
     constexpr int NW = chunk_waves<HD, CT>(), NC = 16 * CT;
     constexpr int KW = HD * KB / 64, VW = HD * VB / 64;  // dwords of a lane's K and V codes
     constexpr int NS = HD / 32;                          // k steps of S^T, blocks of a head
@@ -180,7 +181,13 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
         pages = it + lane < n_it ? a.q.pages[(int64_t)seq * a.q.table_len + t / tpp] : -1;
         if (pages >= a.c.n_pages) pages = -1;
     };
+    // A record's address is the wavefront's, a lane's offset an unsigned 32-bit one: loads take both as they are.  (The empty asm
+    // statements keep the offsets from being widened once for all: as 64-bit numbers they leave the 128-wide instances short of registers,
+    // and a spilled one is read back behind the loads in flight, which it then waits for: 24 sequences of 4 rows over 6000 positions
+    // in 8 / 4 bits 64 us so, 61 now.)
     auto load = [&](int it, Rec& x) {
+        uint32_t run_at = 16u * lane, vs_at = 8u * (4u * (r * VD / 32) + g), ks_at = 2u * (16u * (g * NS / 4) + r);
+        asm volatile("" : "+v"(run_at), "+v"(vs_at), "+v"(ks_at));
         const int page = __builtin_amdgcn_readlane(pages, it & 63);
         x.there = page >= 0;
         if (!x.there) return;
@@ -188,35 +195,36 @@ __global__ __launch_bounds__((chunk_waves<HD, CT>() * 64), (chunk_side<HD, CT>()
         const uint8_t* rec = (const uint8_t*)a.c.pages + (((int64_t)page * a.c.n_kv_head + kvh) * tpp + t % tpp) * RB;
 #pragma unroll
         for (int i = 0; i < KW; i += 4) {
-            const uint4 v = *(const uint4*)(rec + 256 * i + 16 * lane);
+            const uint4 v = *(const uint4*)(rec + 256 * i + run_at);
             x.k[i] = v.x; x.k[i + 1] = v.y; x.k[i + 2] = v.z; x.k[i + 3] = v.w;
         }
         rec += kKvTile * HD * KB / 8;
+        asm volatile("" : "+s"(rec));
 #pragma unroll
         for (int i = 0; i < VW; i += 4) {
-            const uint4 v = *(const uint4*)(rec + 256 * i + 16 * lane);
+            const uint4 v = *(const uint4*)(rec + 256 * i + run_at);
             x.v[i] = v.x; x.v[i + 1] = v.y; x.v[i + 2] = v.z; x.v[i + 3] = v.w;
         }
         rec += kKvTile * HD * VB / 8;
+        asm volatile("" : "+s"(rec));
         // K scales: a lane's quarter of the head lies in block g * NS / 4 (and the next one of 256-wide heads)
-        if constexpr (NS <= 4) x.ks[0] = *(const uint16_t*)(rec + (16 * (g * NS / 4) + r) * 2);
-        else {
-            x.ks[0] = *(const uint16_t*)(rec + (16 * (2 * g) + r) * 2);
-            x.ks[1] = *(const uint16_t*)(rec + (16 * (2 * g + 1) + r) * 2);
-        }
-        x.vs = *(const uint2*)(rec + HD + (4 * (r * VD / 32) + g) * 8);
+        x.ks[0] = *(const uint16_t*)(rec + ks_at);
+        if constexpr (NS > 4) x.ks[1] = *(const uint16_t*)(rec + 32 + ks_at);
+        x.vs = *(const uint2*)(rec + HD + vs_at);
     };
     // Positions of this lane (a bit each) with values that read back as infinite or NaN: read anew, few caches hold any.
     auto not_finite = [&](int it) {
         const int t = first + wave + NW * it;
         const uint8_t* rec = (const uint8_t*)a.c.pages +
                              (((int64_t)a.q.pages[(int64_t)seq * a.q.table_len + t / tpp] * a.c.n_kv_head + kvh) * tpp + t % tpp) * RB + kKvTile * HD * KB / 8;
-        const uint8_t* scales = rec + kKvTile * HD * VB / 8 + HD + (4 * (r * VD / 32) + g) * 8;
+        uint32_t run_at = 16u * lane, vs_at = 8u * (4u * (r * VD / 32) + g);
+        asm volatile("" : "+v"(run_at), "+v"(vs_at));
+        const uint8_t *run = rec + run_at, *scales = rec + kKvTile * HD * VB / 8 + HD + vs_at;
         uint32_t odd = 0;
 #pragma nounroll
         for (int i = 0; i < 8 * VD; i++) {  // (in the order of the lane's codes)
             const int b = i * VB / 8;
-            const uint32_t code = rec[1024 * (b / 16) + 16 * lane + b % 16] >> (i * VB % 8) & (VB == 8 ? 127u : 7u);
+            const uint32_t code = run[1024 * (b / 16) + b % 16] >> (i * VB % 8) & (VB == 8 ? 127u : 7u);
             odd |= (code >= first_not_finite<VB>(scales[i / VD]) ? 1u : 0u) << (i / VD);
         }
         return odd;

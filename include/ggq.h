@@ -395,7 +395,9 @@ int ggq_attention_kv_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_s
  * a row that sees such a key (the others keep theirs).  Products are exact in fp32
  * terms, as above; where long prompts go through planes of fp16 operands, a
  * weight is besides off by up to 2^-28 of the row's largest product of weight
- * and value.  q and out 16-byte aligned, ldq and ldo multiples of 4;
+ * and value.  Sums of weights times values are divided last: finite as long as the
+ * largest value times the positions that a row sees is below 2^119.  One row of each
+ * sequence is quicker by ggq_attention_kv_dev.  q and out 16-byte aligned, ldq and ldo multiples of 4;
  * n_rows * n_head / 16 + n_seq * n_kv_head below 2^24. */
 int ggq_attention_kv_rows_dev(ggq_ctx* ctx, const ggq_kv_cache* cache, const ggq_kv_seqs* seqs, const int32_t* row_off,
                               int n_rows, const float* q, int64_t ldq, int n_head, float scale, int window, float* out,
@@ -455,7 +457,8 @@ int ggq_attention_prompt_dev(ggq_ctx* ctx, const ggq_attention_prompt_params* pa
  *   S = exp(g_t) S;  S = S + b_t k_t (v_t - S^T k_t)^T;  out_t = scale * S^T q_t
  * with g_t (the decay's logarithm, normally <= 0; -infinity forgets
  * everything) and b_t of the row's head.  Value head h reads the q and k of
- * head h / (n_v_head / n_k_head).  gate and beta are g and b as they are, or
+ * head h / (n_v_head / n_k_head) (no file pins that a model's heads come so: where they
+ * are in another order, the caller permutes the projections' rows).  gate and beta are g and b as they are, or
  *   gate_rate set:          g = gate_rate[h] * softplus(gate + gate_bias[h])
  *                           (gate_bias NULL: 0; a GGUF file's ssm_a and ssm_dt.bias)
  *   GGQ_DELTA_BETA_SIGMOID  b = 1 / (1 + exp(-beta))
@@ -471,7 +474,9 @@ int ggq_attention_prompt_dev(ggq_ctx* ctx, const ggq_attention_prompt_params* pa
  * All sums and states are fp32.  Short sequences (up to 8 or 16 rows, by what is
  * in the call) go row by row, longer ones in parts of 16 rows, for which the rows'
  * values are solved together (the same result, rounded in another order); without workspace
- * for that (a buffer per stream, as for the matmuls) all go row by row.
+ * for that (a buffer per stream, as for the matmuls) all go row by row.  The lengths
+ * are on the device: with n_rows - n_seq below 16 every sequence is taken to be short, so a long
+ * one among sequences without rows goes row by row there (0.9 us a row).
  * Numbers that are not finite reach no row before theirs, those of q no other row.
  * Rows are dense heads: q and k [n_k_head][k_dim], v and out
  * [n_v_head][v_dim], gate and beta [n_v_head], with row strides ld*.  k_dim
@@ -567,7 +572,8 @@ int ggq_norm_dev(ggq_ctx* ctx, const ggq_norm_params* params, void* stream);
  * Weights are within 2^-33, their sums within 2^-30 of 64 bits': a token changes only
  * when u falls that close to the border between two.  A weight below 2^-60 of the largest counts as
  * that of its order alone: it is kept or not, but not drawn (u = 0 takes the first token that is).
- * Row stride ld >= n_vocab (any alignment of 4 bytes); n_vocab up to 2^22, n_rows up to 65535. */
+ * Row stride ld >= n_vocab (any alignment of 4 bytes); n_vocab up to 2^22, n_rows up to 65535.  The workspace
+ * is a little larger than the logits (17 KB for each 4096 of a row, whatever its filters are). */
 typedef struct {
     int n_rows;
     int n_vocab;
