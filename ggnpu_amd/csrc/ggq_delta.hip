@@ -24,8 +24,8 @@
 // one barrier a part.  S^T's rows in a lane are those that the next product's operand
 // wants of that lane (step e of a product takes k = 4 g + e from lane group g), so the
 // state goes from product to product in its registers.
-// Bound: the chain of a part's steps.  8191 rows of 32 heads of 128 x 128: parts 51 us (their rows' bytes 33), scan 365, a part 1750 cycles, of which its 29 products
-// take 960 (the four products of a part's rows and the state 200 us in all); the other half is what cannot stand beside
+// Bound: the chain of a part's steps.  8191 rows of 32 heads of 128 x 128: parts 51 us (their rows' bytes 33), scan 343, a part 1650 cycles, of which its 29 products
+// take 960 (the four products of a part's rows and the state 200 us in all); the rest is what cannot stand beside
 // an fp32 product of the same wavefront: own arithmetic, the sums' way through LDS, the barrier.
 #include <algorithm>
 #include <climits>
@@ -566,19 +566,19 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
 int64_t parts_of(const ggq_delta_rule_params& p) { return (int64_t)p.n_rows / kRows + p.n_seq; }
 
 // How many rows a sequence that goes row by row has at most (DeltaArgs::few).  A row's step takes 0.9 us where the chip
-// is not full, and 10 us are gone before the first part is through: one sequence of 32 heads of 128 x 128 with 8 rows takes 11.1 us
-// row by row and 11.4 in parts, with 16 rows 18.8 and 12.0.  Many sequences fill the chip better row by row (16 of 16 rows 50 and
-// 61 us, of 24 rows 68 and 70; 64 of 16 rows 176 and 225, of 32 rows 342 and 287).  The lengths are on the device: unless all are
+// is not full, and 10 us are gone before the first part is through: one sequence of 32 heads of 128 x 128 with 8 rows takes 11.2 us
+// row by row and 11.5 in parts, with 16 rows 19.1 and 12.2.  Many sequences fill the chip better row by row (16 of 16 rows 50 and
+// 61 us, of 24 rows 69 and 70; 64 of 16 rows 174 and 224, of 32 rows 337 and 287).  The lengths are on the device: unless all are
 // bound to be short or are long in the mean, both forms are launched and each takes its own sequences.  That costs 5 to 8 us
-// where all are short (64 of 4 rows 73 us, row by row 65) and bounds what one long one costs (64 single tokens and 1024
-// rows: 114 us, row by row 1835, in parts 308).
+// where all are short (64 of 4 rows 73 us, row by row 64) and bounds what one long one costs (64 single tokens and 1024
+// rows: 112 us, row by row 1840, in parts 305).
 int few_rows(const ggq_delta_rule_params& p) {
     if (!p.row_off) return INT_MAX;
     const char* env = getenv("GGQ_DELTA_PARTS");
     const bool many = (int64_t)p.n_seq * p.n_v_head * (p.v_dim / 16) > 1024;
     const int few = many ? kRows : kRows / 2;
     if (env && *env) return atoi(env) == 0 ? INT_MAX : atoi(env) == 1 ? -1 : few;
-    if (p.n_rows - p.n_seq < (p.n_seq == 1 ? few : kRows)) return INT_MAX;  // (sequences without rows aside, none is longer)
+    if (p.n_rows - p.n_seq < (p.n_seq == 1 ? few : kRows)) return INT_MAX;  // (none is longer, unless others have no rows: not known here)
     return p.n_rows > (many ? 64 : few) * (int64_t)p.n_seq ? -1 : few;
 }
 

@@ -251,7 +251,8 @@ __global__ __launch_bounds__(TPB) void norm_kernel(NormArgs a) {
 // A wavefront where four values a thread and run are enough (no barrier), else as many threads as leave a thread four
 // runs: loads of 64 bytes in flight a thread, and several rows a CU up to 8192 columns.  Measured (us): one row of 2048 4.3, of which 3 are the
 // launch; 2047 rows of 4096 with addition and codes 22 (4.9 TB/s); 2048 of 8192 42; 512 of 16384 24, of 30000 45 (4.4
-// TB/s: one row a CU); 513 rows of 32 gated heads of 128 9.5: sigmoids and 32 roots a row in 64 bits, 2.6 TB/s.
+// TB/s: one row a CU, 25 of its registers spilled); 513 rows of 32 gated heads of 128 9.5, 2.6 TB/s: two rows a CU, whose loads, arithmetic and
+// stores follow one another (4096 such rows 38, for bytes worth 39).
 hipError_t launch_norm(const ggq_norm_params& p, hipStream_t s) {
     NormArgs a{p, p.norm_len ? p.norm_len : p.n_cols, 0};
     const int lanes = a.len / 4;

@@ -886,10 +886,10 @@ size_t sample_ws_bytes(const ggq_sample_params& p) {
     return info_bytes(p) + ((sizeof(u64) + sizeof(double)) * kBins + sizeof(uint16_t) * (kBins + kPart)) * (size_t)p.n_rows * parts_of(p);
 }
 // Measured (us, first + second kernel): one row of 128256 by top-k, top-p and min-p 6 + 13; 33 rows by top-p 16 + 22; 200 rows of 32003
-// kept whole 16 + 8; 256 rows of 128256 by top-p 109, whole 71, greedy 36 (their bytes take 26).  The first is arithmetic (some 80
-// instructions a token) and LDS atomics, the second up to nine loads that wait for each other at about 1 us each.  Where a
+// kept whole 17 + 8; 256 rows of 128256 by top-p 106, whole 69, greedy 34 (their bytes take 26).  The first is arithmetic (90 vector
+// instructions a token of a row kept whole, 106 where there are filters) and LDS atomics, the second up to nine loads that wait for each other at about 1 us each.  Where a
 // border's bin holds more than kList tokens (temperatures above 4 at such sizes, logits all alike) it is read anew for
-// each digit by the row's one workgroup: one row of 151936 equal logits 580.
+// each digit by the row's one workgroup: one row of 151936 equal logits 583.
 hipError_t launch_sample(const ggq_sample_params& p, void* ws, hipStream_t s) {
     const size_t parts = (size_t)p.n_rows * parts_of(p);
     SampleArgs a{p, parts_of(p), (PartInfo*)ws, nullptr, nullptr, nullptr, nullptr};
