@@ -421,7 +421,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a) {
         for (int e = 0; e < 4; e++) col_at[t][e] = ring + (((4 * g + e) * RPR + ((4 * (tile0 + t) + (r >> 2)) ^ (4 * g + e))) * 4 + (r & 3)) * 4;
     }
     f32x4 k[NT], q[NT];
-    // A row's number of u that is not finite makes all rows of its column so (a zero of T times one is NaN), and the results of the rows
+    // A number of T or the rest that is not finite makes a whole column of u so (a zero times it is NaN), and with it the results of the rows
     // before it.  Their results again: row i is bad if T or the rest has such a number at i or, in its triangle, before; a bad row's u is
     // taken as 0 and its result as NaN.  (The column's state is not finite any more, as it is row by row.)
     auto results_again = [&](const f32x4& tr, const f32x4& rest, float ar, f32x4 of) {
